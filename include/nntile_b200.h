@@ -381,6 +381,123 @@ int nntile_b200_decode_sdpa_noalloc_bf16(nntile_b200_stream_t stream, int64_t he
 size_t nntile_b200_decode_sdpa_noalloc_max_bytes(void);
 
 /* ---------------------------------------------------------------------------
+ * Paged key/value cache: sequences of different lengths in one pool of pages
+ * ------------------------------------------------------------------------- */
+
+/* The reference keeps one contiguous cache per layer in which every sequence of the
+ * batch has the same length (wrappers/python/nntile/layer/cache_utils.py:118-228).  The
+ * entry points below have no counterpart there.  T is bfloat16 (_bf16) or IEEE half
+ * (_fp16); all arrays are Fortran order, all pointers device pointers:
+ *   k_pages, v_pages  [head, page_size, kv_heads, num_pages], T or e4m3 codes;
+ *   k_scales, v_scales  uint8 [page_size, kv_heads, num_pages], e4m3 pages only: a stored
+ *       value is code * 2^(byte - 127), byte in 1..254 (NULL for pages of T);
+ *   bounds  T [head, 2, kv_heads, num_pages]: the smallest and the largest stored key of
+ *       a page, element by element (a NaN key makes both NaN);
+ *   block_table  int32 [max_blocks, batch]: entry n of sequence b names the page of its
+ *       positions n*page_size .. (n+1)*page_size - 1; entries behind its length are not
+ *       read;
+ *   lengths  int32 [batch]: filled positions of every sequence (0 is allowed).
+ * Lengths, tables and selections are read on the device when the kernels run, so a
+ * captured graph can be replayed with other values in the same buffers.  What is out of
+ * range there is left out, never dereferenced, and reported by OR-ing one of the bits
+ * below into *status, a 32-bit word that the caller clears and reads (NULL: no report).
+ * Several sequences may share pages that are only read; a page that is written belongs to
+ * one sequence.  head 1..256; any page_size, group and alignment to the element size is
+ * right, rows of a multiple of 16 bytes on 16-byte boundaries in pages of a multiple of 16
+ * positions are fast. */
+#define NNTILE_B200_PAGES_SAME 0            /* page_format: pages hold T */
+#define NNTILE_B200_PAGES_E4M3 1            /* page_format: pages hold e4m3 and scales */
+#define NNTILE_B200_PAGED_BAD_PAGE 1u       /* a table entry is outside the pool */
+#define NNTILE_B200_PAGED_BAD_LENGTH 2u     /* a length is negative or past its buffer */
+#define NNTILE_B200_PAGED_BAD_BLOCK 4u      /* a selected block is past the table */
+
+/* Write new rows k, v (T [head, new_seq, batch, kv_heads]) behind the filled part of every
+ * sequence: row i of sequence b goes to position lengths[b] + i, for i < new_lens[b]
+ * (int32 [batch]; NULL: new_seq for all).  Neither lengths nor the table is changed; the
+ * table must already name the pages.  Rows that would pass max_blocks*page_size are
+ * dropped (PAGED_BAD_LENGTH).  e4m3 pages: per row and tensor the smallest scale 2^e, e >=
+ * -126, that brings the largest finite magnitude to 448 or less; values round to nearest
+ * even; an infinity or NaN is stored as NaN.  `bounds` (may be NULL) is brought up to date:
+ * started anew for a page whose first position is written, widened otherwise. */
+int nntile_b200_paged_kv_append_bf16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch,
+        int64_t kv_heads, int64_t new_seq, int page_format, const int32_t *lengths,
+        const int32_t *new_lens, const int32_t *block_table, const void *k, const void *v,
+        void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, void *bounds,
+        uint32_t *status);
+int nntile_b200_paged_kv_append_fp16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch,
+        int64_t kv_heads, int64_t new_seq, int page_format, const int32_t *lengths,
+        const int32_t *new_lens, const int32_t *block_table, const void *k, const void *v,
+        void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, void *bounds,
+        uint32_t *status);
+
+/* Read a cache back: k, v (T [head, max_seq, batch, kv_heads]) rows 0 .. lengths[b] - 1 of
+ * every sequence, e4m3 values rounded once to T; rows behind are left as they are.  A
+ * length above max_seq is cut there (PAGED_BAD_LENGTH). */
+int nntile_b200_paged_kv_gather_bf16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch,
+        int64_t kv_heads, int64_t max_seq, int page_format, const int32_t *lengths,
+        const int32_t *block_table, const void *k_pages, const void *v_pages,
+        const uint8_t *k_scales, const uint8_t *v_scales, void *k, void *v, uint32_t *status);
+int nntile_b200_paged_kv_gather_fp16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch,
+        int64_t kv_heads, int64_t max_seq, int page_format, const int32_t *lengths,
+        const int32_t *block_table, const void *k_pages, const void *v_pages,
+        const uint8_t *k_scales, const uint8_t *v_scales, void *k, void *v, uint32_t *status);
+
+/* nntile_b200_decode_sdpa_bf16 over a paged cache: out [head, 1, batch, group, kv_heads] =
+ * softmax(q.K^T/sqrt(head)) V over the first lengths[b] positions of every sequence, each
+ * key and value read once for the whole group; lse_out: optional fp32 [batch, group,
+ * kv_heads], natural logarithm.  With num_selected > 0 only the positions in the blocks
+ * listed in `selected` (int32 [num_selected, batch, kv_heads], as
+ * nntile_b200_paged_select_* writes it) take part: a negative entry and a block behind the
+ * sequence's length add nothing, a block that is listed twice counts twice, the order is
+ * free.  Nothing to attend to (length 0, an empty selection, scores that are all -inf):
+ * out = 0, lse = -inf.  `workspace`: nntile_b200_paged_decode_sdpa_workspace_bytes(...) bytes, 16-byte
+ * aligned, of any content; calls that may overlap on the GPU need workspaces of their own.
+ * Results do not depend on the order in which CTAs run. */
+int nntile_b200_paged_decode_sdpa_bf16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,
+        int64_t kv_heads, int64_t num_selected, int page_format, const int32_t *lengths,
+        const int32_t *block_table, const int32_t *selected, const void *q,
+        const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+        const uint8_t *v_scales, void *out, float *lse_out, void *workspace,
+        size_t workspace_bytes, uint32_t *status);
+int nntile_b200_paged_decode_sdpa_fp16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,
+        int64_t kv_heads, int64_t num_selected, int page_format, const int32_t *lengths,
+        const int32_t *block_table, const int32_t *selected, const void *q,
+        const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+        const uint8_t *v_scales, void *out, float *lse_out, void *workspace,
+        size_t workspace_bytes, uint32_t *status);
+size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, int64_t page_size,
+        int64_t max_blocks, int64_t batch, int64_t group, int64_t kv_heads,
+        int64_t num_selected);
+
+/* Choose the blocks that the new token of every sequence attends to, per kv head.  Of the
+ * n = ceil(lengths[b]/page_size) blocks of a sequence the first `first_blocks` and the last
+ * `last_blocks` are always taken, then those of the highest score
+ *     max over the group of  sum_d max(q_d, 0)*kmax_d + min(q_d, 0)*kmin_d,
+ * an upper bound on every q.k of the block, until num_selected are chosen; equal scores go
+ * to the lower block, a NaN score counts as the highest.  Scores are compared as sums in 64
+ * bits.  `selected` (int32 [num_selected, batch, kv_heads]) receives the block numbers in
+ * ascending order, then -1.  first_blocks + last_blocks <= num_selected.  `workspace`:
+ * nntile_b200_paged_select_workspace_bytes(...) bytes, 16-byte aligned, of any content. */
+int nntile_b200_paged_select_bf16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,
+        int64_t kv_heads, int64_t num_selected, int64_t first_blocks, int64_t last_blocks,
+        const int32_t *lengths, const int32_t *block_table, const void *q, const void *bounds,
+        int32_t *selected, void *workspace, size_t workspace_bytes, uint32_t *status);
+int nntile_b200_paged_select_fp16(nntile_b200_stream_t stream, int64_t head,
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,
+        int64_t kv_heads, int64_t num_selected, int64_t first_blocks, int64_t last_blocks,
+        const int32_t *lengths, const int32_t *block_table, const void *q, const void *bounds,
+        int32_t *selected, void *workspace, size_t workspace_bytes, uint32_t *status);
+size_t nntile_b200_paged_select_workspace_bytes(int64_t max_blocks, int64_t batch,
+        int64_t kv_heads);
+
+/* ---------------------------------------------------------------------------
  * Tensor level: the tile loops of the fused path
  * ------------------------------------------------------------------------- */
 

@@ -55,7 +55,18 @@ SIGNATURES = {
     "nntile_b200_transpose_rope_bf16": ([vp] + [i64]*4 + [vp]*4, ctypes.c_int),
     "nntile_b200_transpose_bias_bf16": ([vp] + [i64]*4 + [vp]*3, ctypes.c_int),
     "nntile_b200_transpose_heads_back_bf16": ([vp] + [i64]*4 + [vp]*2, ctypes.c_int),
+    "nntile_b200_paged_decode_sdpa_workspace_bytes": ([i64]*7, sz),
+    "nntile_b200_paged_select_workspace_bytes": ([i64]*3, sz),
 }
+for _sfx in ("bf16", "fp16"):
+    SIGNATURES[f"nntile_b200_paged_kv_append_{_sfx}"] = (
+        [vp] + [i64]*7 + [ctypes.c_int] + [vp]*11, ctypes.c_int)
+    SIGNATURES[f"nntile_b200_paged_kv_gather_{_sfx}"] = (
+        [vp] + [i64]*7 + [ctypes.c_int] + [vp]*9, ctypes.c_int)
+    SIGNATURES[f"nntile_b200_paged_decode_sdpa_{_sfx}"] = (
+        [vp] + [i64]*8 + [ctypes.c_int] + [vp]*11 + [sz, vp], ctypes.c_int)
+    SIGNATURES[f"nntile_b200_paged_select_{_sfx}"] = (
+        [vp] + [i64]*10 + [vp]*6 + [sz, vp], ctypes.c_int)
 for _name in ("flash_sdpa_fwd", "flash_sdpa_bwd", "flash_sdpa_fwd_gqa", "flash_sdpa_bwd_gqa",
               "tensor_flash_sdpa_fwd", "tensor_flash_sdpa_bwd", "tensor_flash_sdpa_fwd_gqa",
               "tensor_flash_sdpa_bwd_gqa"):

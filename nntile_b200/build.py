@@ -23,7 +23,7 @@ LIB = os.path.join(CSRC, "libnntile_b200.so")
 SOURCES = [
     "vanilla_ops.cu", "flash_generic.cu", "flash_api.cu", "decode.cu",
     "flash_fwd_sm100.cu", "flash_bwd_sm100.cu", "host_tensor.cu", "gemm_cublas.cu",
-    "sdpa_prologue.cu",
+    "sdpa_prologue.cu", "paged_cache.cu", "paged_decode.cu", "paged_select.cu",
 ]
 # the fused-attention sources are compiled a second time for IEEE half (elem.cuh)
 FP16_SOURCES = [

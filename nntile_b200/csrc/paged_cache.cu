@@ -1,0 +1,487 @@
+// Writing a paged key/value cache and reading it back.
+//
+// Both kernels move bytes and nothing else: the bound is HBM bandwidth for prompts and
+// launch latency for single tokens.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace nb200 {
+
+constexpr int ROW_THREADS = 128;
+
+// Elements a lane owns of a row.  VEC: eight neighbouring ones, one 16-byte access, LPR
+// lanes a row (LPR = 8, 16, 32 for heads up to 64, 128, 256).  Otherwise (a head that is
+// not a multiple of 8, or pointers off a 16-byte boundary) every 32nd one, a warp a row.
+template<bool VEC, int LPR>
+__device__ __forceinline__ int element(int lane, int i)
+{
+    return VEC ? 8*(lane & (LPR - 1)) + i : lane + 32*i;
+}
+
+template<typename T, bool VEC, int LPR>
+__device__ __forceinline__ void load_row(const T *row, int head, int lane, float (&x)[8])
+{
+    if(VEC)
+    {
+        const int h = element<VEC, LPR>(lane, 0);
+        const uint4 v = h < head ? *reinterpret_cast<const uint4 *>(row + h)
+                : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+        {
+            const float2 f = unpack2<T>(w[i]);
+            x[2*i] = f.x;
+            x[2*i + 1] = f.y;
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            const int h = element<VEC, LPR>(lane, i);
+            x[i] = h < head ? to_f(row[h]) : 0.0f;
+        }
+    }
+}
+
+template<typename T, bool VEC, int LPR>
+__device__ __forceinline__ void store_row(T *row, int head, int lane, const float (&x)[8])
+{
+    if(VEC)
+    {
+        const int h = element<VEC, LPR>(lane, 0);
+        if(h < head)
+        {
+            *reinterpret_cast<uint4 *>(row + h) = make_uint4(pack2<T>(x[0], x[1]),
+                    pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            const int h = element<VEC, LPR>(lane, i);
+            if(h < head)
+            {
+                row[h] = from_f<T>(x[i]);
+            }
+        }
+    }
+}
+
+template<bool VEC, int LPR>
+__device__ __forceinline__ void store_codes(uint8_t *row, int head, int lane,
+        const uint32_t (&c)[4])
+{
+    if(VEC)
+    {
+        const int h = element<VEC, LPR>(lane, 0);
+        if(h < head)
+        {
+            *reinterpret_cast<uint2 *>(row + h) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            const int h = element<VEC, LPR>(lane, i);
+            if(h < head)
+            {
+                row[h] = (uint8_t)(c[i >> 1] >> 8*(i & 1));
+            }
+        }
+    }
+}
+
+template<bool VEC, int LPR>
+__device__ __forceinline__ void load_codes(const uint8_t *row, int head, int lane,
+        uint32_t (&c)[4])
+{
+    if(VEC)
+    {
+        const int h = element<VEC, LPR>(lane, 0);
+        const uint2 v = h < head ? *reinterpret_cast<const uint2 *>(row + h) : make_uint2(0u, 0u);
+        c[0] = v.x & 0xFFFFu;
+        c[1] = v.x >> 16;
+        c[2] = v.y & 0xFFFFu;
+        c[3] = v.y >> 16;
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+        {
+            const int lo = element<VEC, LPR>(lane, 2*i), hi = element<VEC, LPR>(lane, 2*i + 1);
+            c[i] = (lo < head ? (uint32_t)row[lo] : 0u) | (hi < head ? (uint32_t)row[hi] << 8 : 0u);
+        }
+    }
+}
+
+// Quantise the eight elements a lane owns (its row shared by the LPR lanes around it):
+// returns the exponent byte, leaves the codes in `c` and the stored values in `x`.
+template<int LPR>
+__device__ __forceinline__ uint32_t quantise_row(float (&x)[8], uint32_t (&c)[4])
+{
+    float amax = 0.0f;
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+    {
+        const float a = fabsf(x[i]);
+        amax = a < CUDART_INF_F ? fmaxf(amax, a) : amax;     // infinities and NaN do not count
+    }
+#pragma unroll
+    for(int o = LPR/2; o > 0; o >>= 1)
+    {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    const uint32_t byte = scale_byte(amax);
+    const float inv = inverse_scale(byte), scale = scale_value(byte);
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+    {
+        // the format has no infinity: what is not finite is kept as NaN
+        x[i] = fabsf(x[i]) < CUDART_INF_F ? x[i]*inv : CUDART_NAN_F;
+    }
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+    {
+        c[i] = f2_to_e4m3x2(x[2*i], x[2*i + 1]);
+        const float2 back = e4m3x2_to_f2(c[i]);
+        x[2*i] = back.x*scale;
+        x[2*i + 1] = back.y*scale;
+    }
+    return byte;
+}
+
+// One CTA owns one (sequence, kv head, touched block): the block's new rows of K and V,
+// and, because no other CTA writes this (page, kv head), its key bounds without atomics.
+// A block's bounds are those of its stored (for 8-bit pages: quantised) keys, rounded to T;
+// rows that were in the page before are merged in unless the block starts with this call.
+template<typename T, bool E4M3, bool VEC, int LPR>
+__global__ void __launch_bounds__(ROW_THREADS)
+paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
+        int kv_heads, int new_seq, int touched, const int32_t *__restrict__ lengths,
+        const int32_t *__restrict__ new_lens, const int32_t *__restrict__ block_table,
+        const T *__restrict__ k, const T *__restrict__ v, void *__restrict__ k_pages,
+        void *__restrict__ v_pages, uint8_t *__restrict__ k_scales,
+        uint8_t *__restrict__ v_scales, T *__restrict__ bounds, uint32_t *__restrict__ status)
+{
+    constexpr int SLOTS = ROW_THREADS/LPR;       // rows in flight per CTA
+    const int lane = threadIdx.x & 31;
+    const int slot = threadIdx.x/LPR;
+    const int unit = blockIdx.x/touched, j = blockIdx.x - unit*touched;
+    const int b = unit % batch, kvh = unit/batch;
+    const int capacity = max_blocks*page_size;
+    const int start = checked_length(lengths, b, capacity, status);
+    bool bad = false;
+    const int count = held_count(new_lens ? new_lens[b] : new_seq, new_seq, start, capacity, bad);
+    if(bad)
+    {
+        report(status, NNTILE_B200_PAGED_BAD_LENGTH);
+    }
+    const int block = start/page_size + j;
+    int first, last;
+    rows_in_block(start, count, block, page_size, first, last);
+    if(first >= last)
+    {
+        return;
+    }
+    const int page = checked_page(block_table + (size_t)b*max_blocks, block, num_pages, status);
+    if(page < 0)
+    {
+        return;
+    }
+    const size_t dst0 = ((size_t)page*kv_heads + kvh)*page_size;
+    const int rows = last - first;
+    const size_t src0 = ((size_t)unit*new_seq + ((size_t)block*page_size + first - start));
+    float low[8], high[8];
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+    {
+        low[i] = CUDART_INF_F;
+        high[i] = -CUDART_INF_F;
+    }
+    // warps stay converged: the quantiser shuffles within a row's lanes
+    for(int r0 = 0; r0 < 2*rows; r0 += SLOTS)
+    {
+        const int r = r0 + slot;
+        const bool live = r < 2*rows;
+        const bool is_k = r < rows;
+        const int row = is_k ? r : r - rows;
+        float x[8];
+        if(live)
+        {
+            load_row<T, VEC, LPR>((is_k ? k : v) + (src0 + row)*head, head, lane, x);
+        }
+        else
+        {
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+            {
+                x[i] = 0.0f;
+            }
+        }
+        const size_t dst = dst0 + first + row;
+        if(E4M3)
+        {
+            uint32_t c[4];
+            const uint32_t byte = quantise_row<LPR>(x, c);
+            if(live)
+            {
+                store_codes<VEC, LPR>((uint8_t *)(is_k ? k_pages : v_pages) + dst*head, head,
+                        lane, c);
+                if((lane & (LPR - 1)) == 0)
+                {
+                    (is_k ? k_scales : v_scales)[dst] = (uint8_t)byte;
+                }
+            }
+        }
+        else if(live)
+        {
+            store_row<T, VEC, LPR>((T *)(is_k ? k_pages : v_pages) + dst*head, head, lane, x);
+        }
+        if(bounds && live && is_k)
+        {
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+            {
+                low[i] = min_nan(low[i], x[i]);
+                high[i] = max_nan(high[i], x[i]);
+            }
+        }
+    }
+    if(!bounds)
+    {
+        return;
+    }
+    __shared__ float low_s[SLOTS][8*LPR], high_s[SLOTS][8*LPR];
+#pragma unroll
+    for(int i = 0; i < 8; ++i)
+    {
+        low_s[slot][element<VEC, LPR>(lane, i)] = low[i];
+        high_s[slot][element<VEC, LPR>(lane, i)] = high[i];
+    }
+    __syncthreads();
+    T *low_g = bounds + ((size_t)page*kv_heads + kvh)*2*head, *high_g = low_g + head;
+    for(int h = threadIdx.x; h < head; h += ROW_THREADS)
+    {
+        float a = low_s[0][h], z = high_s[0][h];
+#pragma unroll
+        for(int s = 1; s < SLOTS; ++s)
+        {
+            a = min_nan(a, low_s[s][h]);
+            z = max_nan(z, high_s[s][h]);
+        }
+        if(first > 0)
+        {
+            a = min_nan(a, to_f(low_g[h]));
+            z = max_nan(z, to_f(high_g[h]));
+        }
+        low_g[h] = from_f<T>(a);
+        high_g[h] = from_f<T>(z);
+    }
+}
+
+// Rows [0, lengths[b]) of every sequence, K and V, out of the pages; rows behind are left
+// as they are.  blockIdx.y: 0 = K, 1 = V.
+template<typename T, bool E4M3, bool VEC, int LPR>
+__global__ void __launch_bounds__(ROW_THREADS)
+paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
+        int kv_heads, int max_seq, int rows_per_cta, int chunks,
+        const int32_t *__restrict__ lengths, const int32_t *__restrict__ block_table,
+        const void *__restrict__ k_pages, const void *__restrict__ v_pages,
+        const uint8_t *__restrict__ k_scales, const uint8_t *__restrict__ v_scales,
+        T *__restrict__ k, T *__restrict__ v, uint32_t *__restrict__ status)
+{
+    constexpr int SLOTS = ROW_THREADS/LPR;
+    const int lane = threadIdx.x & 31;
+    const int slot = threadIdx.x/LPR;
+    const int unit = blockIdx.x/chunks, chunk = blockIdx.x - unit*chunks;
+    const int b = unit % batch, kvh = unit/batch;
+    int len = checked_length(lengths, b, max_blocks*page_size, status);
+    if(len > max_seq)
+    {
+        report(status, NNTILE_B200_PAGED_BAD_LENGTH);
+        len = max_seq;
+    }
+    const bool is_k = blockIdx.y == 0;
+    const void *pages = is_k ? k_pages : v_pages;
+    const uint8_t *scales = is_k ? k_scales : v_scales;
+    T *out = (is_k ? k : v) + (size_t)unit*max_seq*head;
+    const int64_t begin = (int64_t)chunk*rows_per_cta;
+    const int end = (int)min((int64_t)len, begin + rows_per_cta);
+    for(int64_t r = begin + slot; r < end; r += SLOTS)
+    {
+        const int block = (int)r/page_size;
+        const int page = checked_page(block_table + (size_t)b*max_blocks, block, num_pages,
+                status);
+        if(page < 0)
+        {
+            continue;
+        }
+        const size_t src = ((size_t)page*kv_heads + kvh)*page_size + ((int)r - block*page_size);
+        float x[8];
+        if(E4M3)
+        {
+            uint32_t c[4];
+            load_codes<VEC, LPR>((const uint8_t *)pages + src*head, head, lane, c);
+            const float scale = scale_value(scales[src]);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                const float2 f = e4m3x2_to_f2(c[i]);
+                x[2*i] = f.x*scale;
+                x[2*i + 1] = f.y*scale;
+            }
+        }
+        else
+        {
+            load_row<T, VEC, LPR>((const T *)pages + src*head, head, lane, x);
+        }
+        store_row<T, VEC, LPR>(out + (size_t)r*head, head, lane, x);
+    }
+}
+
+// 16-byte accesses need rows of a multiple of 8 elements on 16-byte boundaries (8 bytes for
+// codes); everything else goes element by element.
+static bool vector_rows(int64_t head, bool e4m3, const void *a, const void *b, const void *pa,
+        const void *pb)
+{
+    const uintptr_t rows = (uintptr_t)a | (uintptr_t)b, pages = (uintptr_t)pa | (uintptr_t)pb;
+    return head % 8 == 0 && (rows & 15) == 0 && (pages & (e4m3 ? 7 : 15)) == 0;
+}
+
+template<typename T>
+static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_size,
+        int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t kv_heads, int64_t new_seq,
+        int page_format, const int32_t *lengths, const int32_t *new_lens,
+        const int32_t *block_table, const void *k, const void *v, void *k_pages, void *v_pages,
+        uint8_t *k_scales, uint8_t *v_scales, void *bounds, uint32_t *status)
+{
+    const int st = check_paged(head, page_size, num_pages, max_blocks, batch, kv_heads,
+            page_format);
+    if(st != NNTILE_B200_OK) return st;
+    if(new_seq < 0) return NNTILE_B200_E_BADARG;
+    if(new_seq > INT32_MAX/2) return NNTILE_B200_E_SHAPE;
+    if(batch == 0 || kv_heads == 0 || new_seq == 0) return NNTILE_B200_OK;
+    const bool e4m3 = page_format == NNTILE_B200_PAGES_E4M3;
+    if(max_blocks == 0 || num_pages == 0) return NNTILE_B200_E_BADARG;      // no room at all
+    if(!lengths || !block_table || !k || !v || !k_pages || !v_pages
+            || (e4m3 && (!k_scales || !v_scales)))
+    {
+        return NNTILE_B200_E_BADARG;
+    }
+    if(((uintptr_t)k | (uintptr_t)v | (uintptr_t)bounds) & 1) return NNTILE_B200_E_ALIGN;
+    if(!e4m3 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 1)) return NNTILE_B200_E_ALIGN;
+    if(((uintptr_t)lengths | (uintptr_t)new_lens | (uintptr_t)block_table | (uintptr_t)status) & 3)
+    {
+        return NNTILE_B200_E_ALIGN;
+    }
+    const int64_t touched = std::min(most_touched(new_seq, page_size), max_blocks);
+    if(touched*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    const unsigned grid = (unsigned)(touched*batch*kv_heads);
+    const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
+    cudaStream_t s = as_stream(stream);
+#define NB200_APPEND(E, V, L) paged_append_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
+        (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
+        (int)new_seq, (int)touched, lengths, new_lens, block_table, (const T *)k, (const T *)v, \
+        k_pages, v_pages, k_scales, v_scales, (T *)bounds, status)
+#define NB200_APPEND_L(E) \
+    do { \
+        if(!vec) NB200_APPEND(E, false, 32); \
+        else if(head <= 64) NB200_APPEND(E, true, 8); \
+        else if(head <= 128) NB200_APPEND(E, true, 16); \
+        else NB200_APPEND(E, true, 32); \
+    } while(0)
+    if(e4m3) NB200_APPEND_L(true);
+    else NB200_APPEND_L(false);
+#undef NB200_APPEND_L
+#undef NB200_APPEND
+    return launch_status();
+}
+
+template<typename T>
+static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_size,
+        int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t kv_heads, int64_t max_seq,
+        int page_format, const int32_t *lengths, const int32_t *block_table,
+        const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+        const uint8_t *v_scales, void *k, void *v, uint32_t *status)
+{
+    const int st = check_paged(head, page_size, num_pages, max_blocks, batch, kv_heads,
+            page_format);
+    if(st != NNTILE_B200_OK) return st;
+    if(max_seq < 0) return NNTILE_B200_E_BADARG;
+    if(max_seq > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    if(batch == 0 || kv_heads == 0 || max_seq == 0 || max_blocks == 0) return NNTILE_B200_OK;
+    const bool e4m3 = page_format == NNTILE_B200_PAGES_E4M3;
+    if(!lengths || !block_table || !k || !v || (num_pages > 0 && (!k_pages || !v_pages
+            || (e4m3 && (!k_scales || !v_scales)))))
+    {
+        return NNTILE_B200_E_BADARG;
+    }
+    if(((uintptr_t)k | (uintptr_t)v) & 1) return NNTILE_B200_E_ALIGN;
+    if(!e4m3 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 1)) return NNTILE_B200_E_ALIGN;
+    if(((uintptr_t)lengths | (uintptr_t)block_table | (uintptr_t)status) & 3)
+    {
+        return NNTILE_B200_E_ALIGN;
+    }
+    const int64_t reach = std::min(max_seq, max_blocks*page_size);
+    const int64_t rows_per_cta = 64;
+    const int64_t chunks = (reach + rows_per_cta - 1)/rows_per_cta;
+    if(chunks*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    const dim3 grid((unsigned)(chunks*batch*kv_heads), 2);
+    const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
+    cudaStream_t s = as_stream(stream);
+#define NB200_GATHER(E, V, L) paged_gather_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
+        (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
+        (int)max_seq, (int)rows_per_cta, (int)chunks, lengths, block_table, k_pages, v_pages, \
+        k_scales, v_scales, (T *)k, (T *)v, status)
+#define NB200_GATHER_L(E) \
+    do { \
+        if(!vec) NB200_GATHER(E, false, 32); \
+        else if(head <= 64) NB200_GATHER(E, true, 8); \
+        else if(head <= 128) NB200_GATHER(E, true, 16); \
+        else NB200_GATHER(E, true, 32); \
+    } while(0)
+    if(e4m3) NB200_GATHER_L(true);
+    else NB200_GATHER_L(false);
+#undef NB200_GATHER_L
+#undef NB200_GATHER
+    return launch_status();
+}
+
+} // namespace nb200
+
+using namespace nb200;
+
+#define NB200_PAGED_CACHE_ENTRY(SFX, T) \
+extern "C" int nntile_b200_paged_kv_append_##SFX(nntile_b200_stream_t stream, int64_t head, \
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, \
+        int64_t kv_heads, int64_t new_seq, int page_format, const int32_t *lengths, \
+        const int32_t *new_lens, const int32_t *block_table, const void *k, const void *v, \
+        void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales, void *bounds, \
+        uint32_t *status) \
+{ \
+    return append_impl<T>(stream, head, page_size, num_pages, max_blocks, batch, kv_heads, \
+            new_seq, page_format, lengths, new_lens, block_table, k, v, k_pages, v_pages, \
+            k_scales, v_scales, bounds, status); \
+} \
+extern "C" int nntile_b200_paged_kv_gather_##SFX(nntile_b200_stream_t stream, int64_t head, \
+        int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, \
+        int64_t kv_heads, int64_t max_seq, int page_format, const int32_t *lengths, \
+        const int32_t *block_table, const void *k_pages, const void *v_pages, \
+        const uint8_t *k_scales, const uint8_t *v_scales, void *k, void *v, uint32_t *status) \
+{ \
+    return gather_impl<T>(stream, head, page_size, num_pages, max_blocks, batch, kv_heads, \
+            max_seq, page_format, lengths, block_table, k_pages, v_pages, k_scales, v_scales, \
+            k, v, status); \
+}
+
+NB200_PAGED_CACHE_ENTRY(bf16, bf16)
+NB200_PAGED_CACHE_ENTRY(fp16, __half)

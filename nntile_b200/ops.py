@@ -201,3 +201,83 @@ def decode_sdpa(head, max_seq, length, batch, group, kv_heads, q, Kcache, Vcache
     _call("nntile_b200_decode_sdpa_bf16", _stream(), head, max_seq, length, batch, group,
           kv_heads, _ptr(q), _ptr(Kcache), _ptr(Vcache), _ptr(out), _ptr(lse_out),
           _ptr(workspace), workspace.numel()*workspace.element_size())
+
+
+# ---- paged key/value cache --------------------------------------------------------
+# Unlike the rest of this module these calls run on the stream of the device that their
+# tensors are on, whichever device is current.
+
+def _paged_call(name, dev, args):
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _call(name, torch.cuda.current_stream(dev).cuda_stream, *args)
+    else:
+        _call(name, torch.cuda.current_stream(dev).cuda_stream, *args)
+
+
+def _paged_ptrs(dev, *tensors):
+    """Device addresses (None stays None) of contiguous tensors, all on device `dev`."""
+    if dev < 0:
+        raise ValueError("nntile_b200 ops need CUDA tensors (there is no CPU path)")
+    ptrs = []
+    for t in tensors:
+        if t is None:
+            ptrs.append(None)
+            continue
+        if t.get_device() != dev:
+            raise ValueError("paged cache operations need CUDA tensors on one device")
+        if not t.is_contiguous():
+            raise ValueError("nntile_b200 ops need contiguous buffers")
+        ptrs.append(t.data_ptr())
+    return ptrs
+
+
+def paged_kv_append(head, page_size, num_pages, max_blocks, batch, kv_heads, new_seq, page_format,
+                    lengths, new_lens, block_table, k, v, k_pages, v_pages, k_scales, v_scales,
+                    bounds, status):
+    dev = k.get_device()
+    _paged_call(f"nntile_b200_paged_kv_append_{_sfx16(k)}", dev,
+                (head, page_size, num_pages, max_blocks, batch, kv_heads, new_seq, page_format,
+                 *_paged_ptrs(dev, lengths, new_lens, block_table, k, v, k_pages, v_pages,
+                              k_scales, v_scales, bounds, status)))
+
+
+def paged_kv_gather(head, page_size, num_pages, max_blocks, batch, kv_heads, max_seq, page_format,
+                    lengths, block_table, k_pages, v_pages, k_scales, v_scales, k, v, status):
+    dev = k.get_device()
+    _paged_call(f"nntile_b200_paged_kv_gather_{_sfx16(k)}", dev,
+                (head, page_size, num_pages, max_blocks, batch, kv_heads, max_seq, page_format,
+                 *_paged_ptrs(dev, lengths, block_table, k_pages, v_pages, k_scales, v_scales,
+                              k, v, status)))
+
+
+def paged_decode_workspace_bytes(head, page_size, max_blocks, batch, group, kv_heads,
+                                 num_selected=0) -> int:
+    return int(_lib.load().nntile_b200_paged_decode_sdpa_workspace_bytes(
+        head, page_size, max_blocks, batch, group, kv_heads, num_selected))
+
+
+def paged_decode_sdpa(head, page_size, num_pages, max_blocks, batch, group, kv_heads,
+                      num_selected, page_format, lengths, block_table, selected, q, k_pages,
+                      v_pages, k_scales, v_scales, out, lse_out, workspace, status):
+    dev = q.get_device()
+    ptrs = _paged_ptrs(dev, lengths, block_table, selected, q, k_pages, v_pages, k_scales,
+                       v_scales, out, lse_out, workspace, status)
+    _paged_call(f"nntile_b200_paged_decode_sdpa_{_sfx16(q)}", dev,
+                (head, page_size, num_pages, max_blocks, batch, group, kv_heads, num_selected,
+                 page_format, *ptrs[:-1], workspace.numel()*workspace.element_size(), ptrs[-1]))
+
+
+def paged_select_workspace_bytes(max_blocks, batch, kv_heads) -> int:
+    return int(_lib.load().nntile_b200_paged_select_workspace_bytes(max_blocks, batch, kv_heads))
+
+
+def paged_select(head, page_size, num_pages, max_blocks, batch, group, kv_heads, num_selected,
+                 first_blocks, last_blocks, lengths, block_table, q, bounds, selected, workspace,
+                 status):
+    dev = q.get_device()
+    ptrs = _paged_ptrs(dev, lengths, block_table, q, bounds, selected, workspace, status)
+    _paged_call(f"nntile_b200_paged_select_{_sfx16(q)}", dev,
+                (head, page_size, num_pages, max_blocks, batch, group, kv_heads, num_selected,
+                 first_blocks, last_blocks, *ptrs[:-1],
+                 workspace.numel()*workspace.element_size(), ptrs[-1]))

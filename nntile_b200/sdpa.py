@@ -435,3 +435,269 @@ class KVCache:
 
     def __len__(self):
         return self.k_cache_size
+
+
+class KVPages:
+    """Buffers of a paged cache: what the paged_* functions read and write.
+
+    Torch shapes: k, v (num_pages, kv_heads, page_size, head), bfloat16 or float16, or 8-bit
+    e4m3 codes (uint8 or float8_e4m3fn) with k_scales, v_scales uint8 (num_pages, kv_heads,
+    page_size), value = code * 2**(byte - 127); bounds, for paged_select, (num_pages,
+    kv_heads, 2, head) in the type of the rows: least and largest stored key of a page."""
+
+    __slots__ = ("k", "v", "k_scales", "v_scales", "bounds", "e4m3")
+
+    def __init__(self, k, v, k_scales=None, v_scales=None, bounds=None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v pages must be two equal (num_pages, kv_heads, page_size, "
+                             "head) buffers")
+        self.e4m3 = k.dtype not in (torch.bfloat16, torch.float16)
+        if self.e4m3:
+            if k.dtype not in (torch.uint8, torch.float8_e4m3fn):
+                raise TypeError(f"pages hold bfloat16, float16 or 8-bit codes, not {k.dtype}")
+            for s in (k_scales, v_scales):
+                if s is None or s.shape != k.shape[:3] or s.dtype != torch.uint8:
+                    raise ValueError("8-bit pages need uint8 scales (num_pages, kv_heads, "
+                                     "page_size) for k and v")
+        elif k_scales is not None or v_scales is not None:
+            raise ValueError("only 8-bit pages have scales")
+        if bounds is not None and (bounds.shape != (k.shape[0], k.shape[1], 2, k.shape[3])
+                                   or (not self.e4m3 and bounds.dtype != k.dtype)):
+            raise ValueError("bounds must be (num_pages, kv_heads, 2, head) in the type of the rows")
+        self.k, self.v, self.k_scales, self.v_scales, self.bounds = k, v, k_scales, v_scales, bounds
+
+    @classmethod
+    def empty(cls, num_pages, page_size, kv_heads, head, dtype=torch.bfloat16, e4m3=False,
+              bounds=False, device="cuda"):
+        shape = (num_pages, kv_heads, page_size, head)
+        k, v = (torch.zeros(shape, dtype=torch.uint8 if e4m3 else dtype, device=device)
+                for _ in range(2))
+        ks, vs = ((torch.full(shape[:3], 127, dtype=torch.uint8, device=device)
+                   for _ in range(2)) if e4m3 else (None, None))
+        bd = torch.zeros((num_pages, kv_heads, 2, head), dtype=dtype, device=device) \
+            if bounds else None
+        return cls(k, v, ks, vs, bd)
+
+    def _check_rows(self, t, what):
+        if t.dtype not in (torch.bfloat16, torch.float16) \
+                or (not self.e4m3 and t.dtype != self.k.dtype):
+            raise TypeError(f"{what} is {t.dtype}, the pages hold {self.k.dtype}")
+
+
+def _check_table(pages, lengths, block_table, batch):
+    if lengths.dtype != torch.int32 or block_table.dtype != torch.int32:
+        raise TypeError("lengths and block_table must be int32")
+    if lengths.shape != (batch,) or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError("lengths must be (batch,) and block_table (batch, max_blocks)")
+
+
+def _check_status(status):
+    if status is not None and (status.dtype not in (torch.int32, torch.uint32)
+                               or status.numel() != 1):
+        raise ValueError("status must be one 32-bit word")
+
+
+def paged_append(pages, lengths, block_table, k, v, new_lens=None, status=None):
+    """Write rows k, v (kv_heads, batch, new_seq, head) behind the lengths[b] filled positions
+    of every sequence (the first new_lens[b] of them; default all).  Changes the pages, their
+    scales and bounds, not `lengths` and `block_table`.  `status`: optional 32-bit word that
+    receives NNTILE_B200_PAGED_BAD_* bits."""
+    N, H, P, D = pages.k.shape
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != H or k.shape[3] != D:
+        raise ValueError("k and v must be (kv_heads, batch, new_seq, head) rows for these pages")
+    pages._check_rows(k, "k")
+    if v.dtype != k.dtype or (pages.bounds is not None and pages.bounds.dtype != k.dtype):
+        raise TypeError("k, v and the bounds must have one type")
+    B, n = k.shape[1], k.shape[2]
+    _check_table(pages, lengths, block_table, B)
+    if new_lens is not None and (new_lens.dtype != torch.int32 or new_lens.shape != (B,)):
+        raise ValueError("new_lens must be int32 (batch,)")
+    _check_status(status)
+    ops.paged_kv_append(D, P, N, block_table.shape[1], B, H, n, int(pages.e4m3), lengths, new_lens,
+                        block_table, k, v, pages.k, pages.v, pages.k_scales, pages.v_scales,
+                        pages.bounds, status)
+
+
+def paged_gather(pages, lengths, block_table, k, v, status=None):
+    """Read the cache into k, v (kv_heads, batch, max_seq, head): rows 0 .. lengths[b] - 1 of
+    every sequence; rows behind them are left as they are."""
+    N, H, P, D = pages.k.shape
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != H or k.shape[3] != D:
+        raise ValueError("k and v must be (kv_heads, batch, max_seq, head) buffers for these pages")
+    pages._check_rows(k, "k")
+    if v.dtype != k.dtype:
+        raise TypeError("k and v must have one type")
+    B = k.shape[1]
+    _check_table(pages, lengths, block_table, B)
+    _check_status(status)
+    ops.paged_kv_gather(D, P, N, block_table.shape[1], B, H, k.shape[2], int(pages.e4m3), lengths,
+                        block_table, pages.k, pages.v, pages.k_scales, pages.v_scales, k, v,
+                        status)
+
+
+def _check_query(q, pages):
+    N, H, P, D = pages.k.shape
+    if q.dim() != 5 or q.shape[0] != H or q.shape[3] != 1 or q.shape[4] != D:
+        raise ValueError("q must be (kv_heads, group, batch, 1, head) for these pages")
+    pages._check_rows(q, "q")
+
+
+def paged_select(q, pages, lengths, block_table, num_selected, first_blocks=1, last_blocks=1,
+                 out=None, workspace=None, status=None):
+    """Blocks that the new token of every sequence attends to, per kv head: the first and the
+    last ones and those whose bounds allow the highest score.  Returns int32 (kv_heads,
+    batch, num_selected), ascending block numbers, then -1."""
+    _check_query(q, pages)
+    if pages.bounds is None:
+        raise ValueError("these pages keep no bounds")
+    if pages.bounds.dtype != q.dtype:
+        raise TypeError("q and the bounds must have one type")
+    H, G, B, one, D = q.shape
+    N, P = pages.k.shape[0], pages.k.shape[2]
+    _check_table(pages, lengths, block_table, B)
+    _check_status(status)
+    M = block_table.shape[1]
+    if out is None:
+        out = torch.empty((H, B, num_selected), dtype=torch.int32, device=q.device)
+    elif out.shape != (H, B, num_selected) or out.dtype != torch.int32:
+        raise ValueError("out must be int32 (kv_heads, batch, num_selected)")
+    if workspace is None:
+        need = ops.paged_select_workspace_bytes(M, B, H)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    ops.paged_select(D, P, N, M, B, G, H, num_selected, first_blocks, last_blocks, lengths,
+                     block_table, q, pages.bounds, out, workspace, status)
+    return out
+
+
+def paged_decode(q, pages, lengths, block_table, selected=None, out=None, lse_out=None,
+                 workspace=None, status=None):
+    """decode_sdpa over a paged cache: one new token q (kv_heads, group, batch, 1, head) per
+    sequence against its first lengths[b] positions, or against those of them in the blocks
+    of `selected` (int32 (kv_heads, batch, num_selected), as paged_select returns).  Returns
+    out shaped like q; lse_out: optional float32 (kv_heads, group, batch)."""
+    _check_query(q, pages)
+    H, G, B, one, D = q.shape
+    N, P = pages.k.shape[0], pages.k.shape[2]
+    _check_table(pages, lengths, block_table, B)
+    _check_status(status)
+    M, S = block_table.shape[1], 0
+    if selected is not None:
+        if selected.dtype != torch.int32 or selected.dim() != 3 or selected.shape[:2] != (H, B) \
+                or selected.shape[2] == 0:
+            raise ValueError("selected must be int32 (kv_heads, batch, num_selected)")
+        S = selected.shape[2]
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must be like q")
+    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.numel() != H*G*B):
+        raise ValueError("lse_out must be float32 (kv_heads, group, batch)")
+    if workspace is None:
+        need = ops.paged_decode_workspace_bytes(D, P, M, B, G, H, S)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    ops.paged_decode_sdpa(D, P, N, M, B, G, H, S, int(pages.e4m3), lengths, block_table, selected,
+                          q, pages.k, pages.v, pages.k_scales, pages.v_scales, out, lse_out,
+                          workspace, status)
+    return out
+
+
+class PagedKVCache:
+    """Key/value cache of one attention layer in a pool of pages; sequences grow, and are
+    released, independently of one another.
+
+    The paged counterpart of KVCache, with the same `append`, `decode`, `clear` and `len()`
+    (the longest sequence), so `Sdpa.forward_dynamic` takes either.  Pages are handed out and
+    taken back on the host; tables and lengths are kept on the device.  `e4m3` halves the
+    cache; `bounds` keeps what `decode(..., num_selected=...)` needs to attend to selected
+    blocks only.  For a captured graph call paged_append / paged_select / paged_decode on
+    `pages`, `lengths` and `block_table`: append() here does host bookkeeping."""
+
+    def __init__(self, num_pages, page_size, kv_heads, batch, head, max_blocks=None,
+                 dtype=torch.bfloat16, e4m3=False, bounds=False, device="cuda"):
+        self.pages = KVPages.empty(num_pages, page_size, kv_heads, head, dtype, e4m3, bounds,
+                                   device)
+        self.dtype, self.page_size = dtype, int(page_size)
+        self.max_blocks = int(num_pages if max_blocks is None else max_blocks)
+        self.block_table = torch.full((batch, self.max_blocks), -1, dtype=torch.int32,
+                                      device=device)
+        self.lengths = torch.zeros((batch,), dtype=torch.int32, device=device)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._tables = [[] for _ in range(batch)]
+        self._filled = [0]*batch
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def sequence_lengths(self) -> list[int]:
+        return list(self._filled)
+
+    def append(self, k_partial, v_partial, new_lens=None):
+        """Rows (kv_heads, batch, new_seq, head); new_lens: how many of them count for every
+        sequence (a list of ints; default all).  Raises, with nothing changed, when the pool
+        or a sequence's table has no room."""
+        batch = len(self._filled)
+        if k_partial.dim() != 4 or k_partial.shape != v_partial.shape \
+                or k_partial.shape[1] != batch:
+            raise ValueError("k_partial / v_partial do not match the cache")
+        self.pages._check_rows(k_partial, "k_partial")
+        if k_partial.dtype != self.dtype:
+            raise TypeError(f"rows are {k_partial.dtype}, the cache keeps {self.dtype}")
+        n = k_partial.shape[2]
+        new = [n]*batch if new_lens is None else [int(x) for x in new_lens]
+        if len(new) != batch or any(x < 0 or x > n for x in new):
+            raise ValueError("new_lens must be batch numbers between 0 and new_seq")
+        P = self.page_size
+        more = [-(-(f + x)//P) - len(t) for f, x, t in zip(self._filled, new, self._tables)]
+        if any(len(t) + m > self.max_blocks for t, m in zip(self._tables, more)):
+            raise ValueError("a sequence would pass max_blocks pages")
+        if sum(more) > len(self._free):
+            raise ValueError(f"the pool has {len(self._free)} free pages, {sum(more)} are needed")
+        device = self.lengths.device
+        entries = []
+        for b, m in enumerate(more):
+            for _ in range(m):
+                entries.append((b, len(self._tables[b]), self._free[-1]))
+                self._tables[b].append(self._free.pop())
+        if entries:
+            rows = torch.tensor(entries, dtype=torch.int64).to(device)
+            self.block_table[rows[:, 0], rows[:, 1]] = rows[:, 2].to(torch.int32)
+        lens = None if new_lens is None else torch.tensor(new, dtype=torch.int32).to(device)
+        paged_append(self.pages, self.lengths, self.block_table, k_partial.contiguous(),
+                     v_partial.contiguous(), lens)
+        self.lengths += n if lens is None else lens
+        self._filled = [f + x for f, x in zip(self._filled, new)]
+
+    def decode(self, q, out=None, lse_out=None, num_selected=None, first_blocks=1, last_blocks=1):
+        """Attention of one new token per sequence over everything that is filled, or over
+        num_selected blocks per kv head."""
+        selected = None
+        if num_selected is not None:
+            selected = paged_select(q, self.pages, self.lengths, self.block_table, num_selected,
+                                    first_blocks, last_blocks)
+        return paged_decode(q, self.pages, self.lengths, self.block_table, selected, out, lse_out)
+
+    def read(self):
+        """The filled part as contiguous k, v (kv_heads, batch, len(self), head); zeros behind
+        shorter sequences."""
+        N, H, P, D = self.pages.k.shape
+        k = torch.zeros((H, len(self._filled), len(self), D), dtype=self.dtype,
+                        device=self.lengths.device)
+        v = torch.zeros_like(k)
+        paged_gather(self.pages, self.lengths, self.block_table, k, v)
+        return k, v
+
+    def release(self, b: int):
+        """Sequence b ends: its pages go back to the pool, its slot is empty."""
+        self._free.extend(reversed(self._tables[b]))
+        self._tables[b] = []
+        self._filled[b] = 0
+        self.lengths[b] = 0
+        self.block_table[b] = -1
+
+    def clear(self):
+        for b in range(len(self._filled)):
+            self.release(b)
+
+    def __len__(self):
+        return max(self._filled, default=0)
