@@ -2,9 +2,29 @@
 //
 // o = sum_i p_i v_i / sum_i p_i,  p_i = exp(q.k_i/sqrt(head)), over the filled positions of
 // a sequence, or over those of them that lie in the blocks a list selects.
+//
+// Every key and value is used for 2*group multiply-adds per byte or less: the kernel is
+// bound by HBM bandwidth when the cache is long and by latency when it is short, so the
+// design is about bytes in flight and about even shares:
+//   - work is cut into tiles of 16 positions.  All tiles of all (sequence, kv head) units
+//     stand in one row, and every worker takes the same number of neighbours, whatever
+//     the lengths are (they are only known on the device).  A unit that falls into several
+//     shares is joined by a second, small kernel;
+//   - a warp copies its own tiles into a private ring in shared memory (cp.async, 16 bytes a
+//     lane, swizzled; rows behind the length are zero-filled, never read) and is its own
+//     consumer: no barrier inside a share.  24 KB a warp, 192 KB an SM, more than four times
+//     what HBM latency times bandwidth asks for; the ring runs on across units;
+//   - page numbers are looked up 32 tiles at a time, a lane each, ahead of the ring;
+//   - scores and weighted values go through the warp-level tensor instruction (m16n8k16, fp32
+//     accumulate).  Its 16 rows hold 8 query heads twice: for P.V the upper 8 rows take the
+//     weights rounded to 16 bits and the lower 8 what that rounding lost, so the weights count
+//     with 16 (bf16) or 22 (fp16) bits at no further instruction;
+//   - the running maximum is only applied to the accumulators when it moves.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
+#include "per_device.hh"
 
 namespace nb200 {
 
@@ -22,7 +42,9 @@ struct PagedDecodeArgs
     void *out;
     float *lse_out;
     float *part_o, *part_lse;
+    float2 *part_sums;
     uint32_t *status;
+    int whole;                           // > 0: whole units only, that many warps each
     int nsplit, chunk;                   // chunk: list positions per split (blocks)
 };
 
@@ -210,27 +232,1091 @@ paged_decode_join_kernel(const PagedDecodeArgs a, int heads)
     }
 }
 
+// ------------------------------------------------------------------ tensor-core kernel
+
+constexpr int PD_SMS = 148;
+constexpr int PD_TILE = 16;                  // positions of a tile
+constexpr int PD_TILES_PER_WARP = 32;        // from here on a warp is a worker of its own
+
+// Layout of one kernel variant.  DP: head size rounded up to 64, 128 or 256 (columns behind
+// the head stay zero in the ring); MT: tiles of 8 query heads that share a pass.
+template<bool E4M3, int DP>
+struct PagedTile
+{
+    static constexpr int WARPS = DP == 256 ? 4 : 8;
+    static constexpr int ROW_BYTES = DP*(E4M3 ? 1 : 2);
+    static constexpr int CHUNKS = ROW_BYTES/16;          // 16-byte pieces of a row
+    static constexpr int KV_BYTES = PD_TILE*ROW_BYTES;   // one of K, V
+    static constexpr int STAGE = 2*KV_BYTES + (E4M3 ? 2*PD_TILE : 0);
+    static constexpr int RING = 196608/WARPS;
+    static constexpr int STAGES = RING/STAGE < 8 ? RING/STAGE : 8;
+    static constexpr int NBLK = DP/8;                    // 8-column blocks of the output
+    static constexpr int MERGE = WARPS*8*DP*4;           // one tile of 8 heads of every warp
+    static constexpr int SMEM = WARPS*STAGES*STAGE + MERGE;
+
+    // Offset of piece c of row r.  A 128-byte line holds 8 pieces; which of them is piece c
+    // depends on the row, so that the lanes that load together hit different banks: 8 rows,
+    // one piece (ldmatrix, 16-bit rows); 2 neighbouring rows, 4 pieces (8-bit keys: `rot`
+    // puts the row's last bit on top); 4 even rows, 2 pieces (8-bit values).
+    static __device__ __forceinline__ int offset(int r, int c, bool rot)
+    {
+        if(ROW_BYTES == 64)      // two rows a line
+        {
+            return (r >> 1)*128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4);
+        }
+        const int x = rot ? ((r & 1) << 2) | ((r >> 1) & 3) : r & 7;
+        return r*ROW_BYTES + ((c ^ x) << 4);
+    }
+    // Column of the output that accumulator block e holds for B column c.
+    static __device__ __forceinline__ int column(int e, int c)
+    {
+        if(!E4M3) return 8*e + c;
+        return DP == 64 ? 8*c + e : (e >> 4)*128 + 16*c + (e & 15);
+    }
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p)
+{
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" :: "r"(dst), "l"(src),
+            "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template<int N>
+__device__ __forceinline__ void copy_wait()
+{
+    asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// T: the operand format, bf16 or __half
+template<typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+        uint32_t a3, uint32_t b0, uint32_t b1);
+template<>
+__device__ __forceinline__ void mma16<bf16>(float (&c)[4], uint32_t a0, uint32_t a1,
+        uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template<>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], uint32_t a0, uint32_t a1,
+        uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t word4(const uint4 &v, int i)
+{
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// Tiles of one unit of sequence b.
+__device__ __forceinline__ int unit_tiles(const PagedDecodeArgs &a, int len)
+{
+    if(a.selected)
+    {
+        return len > 0 ? a.num_selected*(a.page_size/PD_TILE) : 0;
+    }
+    return (len + PD_TILE - 1)/PD_TILE;
+}
+
+// Exclusive prefix sums of the tiles of the sequences, prefix[0..batch]; all threads of the
+// block, a barrier at the end.
+__device__ __forceinline__ void tile_prefix(const PagedDecodeArgs &a, int units_per_seq,
+        int *prefix, int *warp_sums, bool reporting)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
+    const int per = (a.batch + nthreads - 1)/nthreads;
+    const int b0 = min(a.batch, tid*per), b1 = min(a.batch, b0 + per);
+    int sum = 0;
+    for(int b = b0; b < b1; ++b)
+    {
+        const int len = checked_length(a.lengths, b, a.max_blocks*a.page_size,
+                reporting ? a.status : nullptr);
+        sum += unit_tiles(a, len)*units_per_seq;
+        prefix[b + 1] = sum;
+    }
+    int scan = sum;
+#pragma unroll
+    for(int o = 1; o < 32; o <<= 1)
+    {
+        const int up = __shfl_up_sync(0xffffffffu, scan, o);
+        scan += lane >= o ? up : 0;
+    }
+    if(lane == 31)
+    {
+        warp_sums[warp] = scan;
+    }
+    __syncthreads();
+    int before = scan - sum;
+    for(int w = 0; w < warp; ++w)
+    {
+        before += warp_sums[w];
+    }
+    for(int b = b0; b < b1; ++b)
+    {
+        prefix[b + 1] += before;
+    }
+    if(tid == 0)
+    {
+        prefix[0] = 0;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ int held_len(const PagedDecodeArgs &a, int b)
+{
+    bool bad = false;
+    return held_length(a.lengths[b], a.max_blocks*a.page_size, bad);
+}
+
+// Two columns of head 8m + n, either final or into part `part` of the workspace, which
+// keeps a lane's values in the order of the accumulators: [part][m][2*block + i][lane].
+template<typename T, bool E4M3, int DP, int MT>
+__device__ __forceinline__ void write_part(const PagedDecodeArgs &a, bool complete, int part,
+        int m, int lane, int e, float z0, float z1, float den, int kvh, int h0, int heads, int b)
+{
+    const int n = lane >> 2, t = lane & 3;
+    if(!complete)
+    {
+        float *o = a.part_o + ((size_t)part*MT + m)*8*DP;
+        o[(2*e)*32 + lane] = z0;
+        o[(2*e + 1)*32 + lane] = z1;
+        return;
+    }
+    const int g = 8*m + n;
+    if(g < heads)
+    {
+        using L = PagedTile<E4M3, DP>;
+        const float inv = den == 0.0f ? 0.0f : 1.0f/den;
+        T *out = (T *)a.out + (((size_t)kvh*a.group + h0 + g)*a.batch + b)*a.head;
+        const int c0 = L::column(e, 2*t), c1 = L::column(e, 2*t + 1);
+        if(c0 < a.head)
+        {
+            out[c0] = from_f<T>(z0*inv);
+        }
+        if(c1 < a.head)
+        {
+            out[c1] = from_f<T>(z1*inv);
+        }
+    }
+}
+
+template<int MT>
+__device__ __forceinline__ void write_sums(const PagedDecodeArgs &a, bool complete, int part,
+        int m, int n, float top, float sum, int kvh, int h0, int heads, int b)
+{
+    const int g = 8*m + n;
+    if(!complete)
+    {
+        a.part_sums[((size_t)part*MT + m)*8 + n] = make_float2(top, sum);
+    }
+    else if(g < heads && a.lse_out)
+    {
+        a.lse_out[((size_t)kvh*a.group + h0 + g)*a.batch + b] = sum == 0.0f ? -CUDART_INF_F
+                : ((top == -CUDART_INF_F ? 0.0f : top) + log2f(sum))*PD_LN2;
+    }
+}
+
+// How the tiles are dealt out: `workers` shares of `share` neighbouring tiles, a worker
+// being a warp (wpw = 1) or a block (wpw = its warps).
+struct PagedShares
+{
+    int wpw, workers, share;
+};
+
+template<int WARPS>
+__host__ __device__ inline PagedShares paged_shares(int total, int blocks)
+{
+    PagedShares s;
+    s.wpw = total >= blocks*WARPS*PD_TILES_PER_WARP ? 1 : WARPS;
+    s.workers = blocks*(WARPS/s.wpw);
+    s.share = (total + s.workers - 1)/s.workers;
+    s.share = (s.share + s.wpw - 1)/s.wpw*s.wpw;
+    return s;
+}
+
+template<typename T, bool E4M3, int DP, int MT>
+__global__ void __launch_bounds__(PagedTile<E4M3, DP>::WARPS*32, 1)
+paged_decode_kernel(const PagedDecodeArgs a)
+{
+    using L = PagedTile<E4M3, DP>;
+    using M = typename std::conditional<E4M3, __half, T>::type;      // operand format
+    constexpr bool HALF = std::is_same<M, __half>::value;
+    // fp16 weights are lifted by 2^14 (they are at most 1), which keeps those down to 2^-38
+    // of the largest; bf16 has fp32's range
+    constexpr int LIFT = HALF ? 14 : 0;
+    constexpr int KSTEPS = DP/16, NBLK = L::NBLK, WARPS = L::WARPS, STAGES = L::STAGES;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int nv_s[WARPS][STAGES];
+    __shared__ float top_s[WARPS][8], sum_s[WARPS][8];
+    __shared__ int scan_s[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = lane >> 2, t = lane & 3;
+    uint8_t *ring = smem + warp*STAGES*L::STAGE;
+    float *merge = reinterpret_cast<float *>(smem + WARPS*STAGES*L::STAGE);
+    const int D = a.head, P = a.page_size;
+    const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
+    const int tpb = P/PD_TILE;
+
+    // lets the joining kernel start its own preparations
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // columns behind the head are never copied: zero for good
+    if(D < DP)
+    {
+        uint4 *z = reinterpret_cast<uint4 *>(ring);
+        for(int i = lane; i < STAGES*L::STAGE/16; i += 32)
+        {
+            z[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+    }
+
+    // ---- this worker's share: tiles [begin, end) of the row of all tiles
+    int *prefix = reinterpret_cast<int *>(merge);
+    tile_prefix(a, HU, prefix, scan_s, blockIdx.x == 0);
+    const int total = prefix[a.batch];
+    int wpw, worker, begin, end;
+    if(a.whole)
+    {
+        // whole units, no joining: unit = sequence*HU + (kv head, head tile)
+        wpw = a.whole;
+        worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
+        const long long units = (long long)a.batch*HU;
+        const int workers = gridDim.x*(WARPS/wpw);
+        int x[2];
+#pragma unroll
+        for(int i = 0; i < 2; ++i)
+        {
+            const int u = (int)(units*(worker + i)/workers);
+            const int b = u/HU;
+            x[i] = b < a.batch ? prefix[b] + (prefix[b + 1] - prefix[b])/HU*(u - b*HU) : total;
+        }
+        begin = x[0];
+        end = x[1];
+        // units with nothing to attend to
+        const int u0 = (int)(units*worker/workers), u1 = (int)(units*(worker + 1)/workers);
+        for(int u = u0 + (wpw > 1 ? warp : 0); u < u1; u += wpw)
+        {
+            const int b = u/HU, hu = u - b*HU;
+            if(prefix[b + 1] == prefix[b])
+            {
+                const int h0 = hu % htiles*8*MT, heads = min(8*MT, a.group - h0);
+                for(int g = 0; g < heads; ++g)
+                {
+                    const size_t qh = ((size_t)(hu/htiles)*a.group + h0 + g)*a.batch + b;
+                    for(int d = lane; d < D; d += 32)
+                    {
+                        ((T *)a.out)[qh*D + d] = from_f<T>(0.0f);
+                    }
+                    if(lane == 0 && a.lse_out)
+                    {
+                        a.lse_out[qh] = -CUDART_INF_F;
+                    }
+                }
+            }
+        }
+    }
+    else
+    {
+        const PagedShares sh = paged_shares<WARPS>(total, gridDim.x);
+        wpw = sh.wpw;
+        worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
+        begin = (int)min((long long)total, (long long)worker*sh.share);
+        end = (int)min((long long)total, (long long)begin + sh.share);
+    }
+    int b = 0;
+    if(begin < end)
+    {
+        int lo = 0, hi = a.batch;             // prefix[lo] <= begin < prefix[hi]
+        while(hi - lo > 1)
+        {
+            const int mid = (lo + hi) >> 1;
+            if(prefix[mid] <= begin) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+    }
+    const int seq_begin = prefix[b];
+    __syncthreads();                          // the prefix sums give way to the merge buffer
+    if(begin >= end)
+    {
+        return;                               // the whole block when wpw > 1: same share
+    }
+
+    // ---- issuing side: runs STAGES - 1 tiles ahead of the consuming side
+    const int step = wpw, slot0 = wpw > 1 ? warp : 0;
+    int ib = b, ix = begin + slot0 - seq_begin;          // next tile, counted inside sequence ib
+    int ileft = end - begin > slot0 ? (end - begin - slot0 + step - 1)/step : 0;
+    int ilen = held_len(a, ib), int_ = unit_tiles(a, ilen);
+    int ipos = 32;                                       // used up: look up at once
+    int look_nv = 0;
+    long long look_row = 0;
+    const int elt = E4M3 ? 1 : (int)sizeof(T);
+    const int row_bytes = D*elt, chunks = row_bytes/16;
+    constexpr int RPP = 32/L::CHUNKS > 0 ? 32/L::CHUNKS : 1;     // rows a warp copies at once
+    const int crow = lane/L::CHUNKS, cchunk = lane % L::CHUNKS;
+
+    auto issue = [&](int stage)
+    {
+        if(ileft > 0)
+        {
+            if(ix >= int_*HU)
+            {
+                while(ix >= int_*HU)
+                {
+                    ix -= int_*HU;
+                    ++ib;
+                    ilen = held_len(a, ib);
+                    int_ = unit_tiles(a, ilen);
+                }
+                ipos = 32;
+            }
+            if(ipos == 32)
+            {
+                // pages of this warp's next 32 tiles in the sequence
+                ipos = 0;
+                look_nv = 0;
+                look_row = 0;
+                const long long x = ix + (long long)lane*step;
+                if(x < (long long)int_*HU && lane < ileft)
+                {
+                    const int unit = (int)x/int_, j = (int)x - unit*int_, kvh = unit/htiles;
+                    const int li = j/tpb, sub = (j - li*tpb)*PD_TILE;
+                    int block = li;
+                    if(a.selected)
+                    {
+                        bool bad = false;
+                        block = held_block(a.selected[((size_t)kvh*a.batch + ib)*a.num_selected
+                                + li], blocks_of(ilen, P), a.max_blocks, bad);
+                        if(bad)
+                        {
+                            report(a.status, NNTILE_B200_PAGED_BAD_BLOCK);
+                        }
+                    }
+                    if(block >= 0)
+                    {
+                        const int left = ilen - block*P - sub;
+                        const int page = left > 0 ? checked_page(a.block_table
+                                + (size_t)ib*a.max_blocks, block, a.num_pages, a.status) : -1;
+                        if(page >= 0)
+                        {
+                            look_nv = min(left, PD_TILE);
+                            look_row = ((long long)page*a.kv_heads + kvh)*P + sub;
+                        }
+                    }
+                }
+            }
+            const int nv = __shfl_sync(0xffffffffu, look_nv, ipos);
+            const long long row = __shfl_sync(0xffffffffu, look_row, ipos);
+            if(lane == 0)
+            {
+                nv_s[warp][stage] = nv;
+            }
+            if(nv > 0)
+            {
+                const uint32_t dst = smem_addr(ring + stage*L::STAGE);
+                const long long at = row*row_bytes + crow*row_bytes + cchunk*16;
+                const uint8_t *ks = (const uint8_t *)a.k_pages + at;
+                const uint8_t *vs = (const uint8_t *)a.v_pages + at;
+                if(cchunk < chunks)
+                {
+#pragma unroll
+                    for(int i = 0; i < PD_TILE/RPP; ++i)
+                    {
+                        const int r = crow + i*RPP;
+                        const int bytes = r < nv ? 16 : 0;
+                        copy16(dst + L::offset(r, cchunk, E4M3), ks + (size_t)i*RPP*row_bytes,
+                                bytes);
+                        copy16(dst + L::KV_BYTES + L::offset(r, cchunk, false),
+                                vs + (size_t)i*RPP*row_bytes, bytes);
+                    }
+                }
+                if(E4M3 && lane < 2)
+                {
+                    copy16(dst + 2*L::KV_BYTES + lane*PD_TILE,
+                            (lane == 0 ? a.k_scales : a.v_scales) + row, 16);
+                }
+            }
+            ++ipos;
+            ix += step;
+            --ileft;
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for(int s = 0; s < STAGES - 1; ++s)
+    {
+        issue(s);
+    }
+
+    // ---- consuming side, unit by unit
+    int stage = 0;
+    int seq_len = held_len(a, b);
+    int nt = unit_tiles(a, seq_len);
+    int hu = (begin - seq_begin)/nt;
+    int x = begin;                                       // first tile of the segment
+    int unit_begin = seq_begin + hu*nt;
+    int mine = begin + slot0;                            // this warp's next tile
+    while(x < end)
+    {
+        const int unit_end = unit_begin + nt;
+        const int seg_end = min(end, unit_end);
+        const int kvh = hu/htiles, h0 = (hu - kvh*htiles)*8*MT;
+        const int heads = min(8*MT, a.group - h0);
+
+        uint32_t qa[MT][KSTEPS][2];
+        float qscale[MT];
+#pragma unroll
+        for(int m = 0; m < MT; ++m)
+        {
+            const int g = 8*m + n;
+            const T *qr = (const T *)a.q + (((size_t)kvh*a.group + h0 + min(g, heads - 1))
+                    *a.batch + b)*D;
+            qscale[m] = a.scale_log2;
+#pragma unroll
+            for(int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+                for(int x2 = 0; x2 < 2; ++x2)
+                {
+                    // head elements of this lane's operand word: in order for 16-bit rows; for
+                    // codes a lane's 16-byte piece t + 4j feeds four steps, four codes each
+                    const int d = E4M3 ? 16*(t + 4*(k >> 2)) + 4*(k & 3) + 2*x2
+                            : 16*k + 8*x2 + 2*t;
+                    qa[m][k][x2] = d < D && g < heads
+                            ? *reinterpret_cast<const uint32_t *>(qr + d) : 0u;
+                }
+            if(E4M3 && !std::is_same<T, __half>::value)
+            {
+                // bf16 queries as fp16 operands: a power of two brings the row's largest element
+                // to [2^14, 2^15); what fp16 then loses is below 2^-38 of it
+                float amax = 0.0f;
+#pragma unroll
+                for(int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+                    for(int x2 = 0; x2 < 2; ++x2)
+                    {
+                        const float2 f = unpack2<T>(qa[m][k][x2]);
+                        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = (int)(__float_as_uint(amax) >> 23);        // 0 and 255: as it is
+                const int up = e == 255 ? 0 : max(-113, min(126, 141 - e));
+                const float lift = __uint_as_float((uint32_t)(127 + up) << 23);
+                qscale[m] *= __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+                for(int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+                    for(int x2 = 0; x2 < 2; ++x2)
+                    {
+                        const float2 f = unpack2<T>(qa[m][k][x2]);
+                        qa[m][k][x2] = pack2<__half>(f.x*lift, f.y*lift);
+                    }
+            }
+        }
+        float acc[MT][NBLK][4], top[MT], sum[MT];
+#pragma unroll
+        for(int m = 0; m < MT; ++m)
+        {
+            top[m] = -CUDART_INF_F;
+            sum[m] = 0.0f;
+#pragma unroll
+            for(int e = 0; e < NBLK; ++e)
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                    acc[m][e][i] = 0.0f;
+        }
+        // 8-bit values: the accumulators count in units of 2^(vref - 127), the largest value
+        // scale so far
+        int vref = 0;
+
+        while(mine < seg_end)
+        {
+            mine += step;
+            copy_wait<STAGES - 2>();
+            __syncwarp();
+            // the stage that was consumed last is free for every lane now
+            issue(stage == 0 ? STAGES - 1 : stage - 1);
+            const uint8_t *st = ring + stage*L::STAGE;
+            const int nv = nv_s[warp][stage];
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            if(nv == 0)
+            {
+                continue;
+            }
+            // ---- scores: two blocks of 8 positions
+            float s[MT][2][4];
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for(int i = 0; i < 4; ++i)
+                        s[m][blk][i] = 0.0f;
+            if(!E4M3)
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+                for(int k = 0; k < KSTEPS; ++k)
+                {
+                    uint32_t kb[4];
+                    ldmatrix4(kb, smem_addr(st + L::offset(r, 2*k + half, false)));
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+                    {
+                        mma16<M>(s[m][0], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[0], kb[1]);
+                        mma16<M>(s[m][1], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[2], kb[3]);
+                    }
+                }
+            }
+            else
+            {
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for(int j = 0; j < DP/64; ++j)
+                    {
+                        const uint4 kc = *reinterpret_cast<const uint4 *>(st
+                                + L::offset(8*blk + n, t + 4*j, true));
+#pragma unroll
+                        for(int w = 0; w < 4; ++w)
+                        {
+                            const uint32_t c = word4(kc, w);
+                            const uint32_t b0 = e4m3x2_to_half2(c & 0xFFFFu);
+                            const uint32_t b1 = e4m3x2_to_half2(c >> 16);
+#pragma unroll
+                            for(int m = 0; m < MT; ++m)
+                            {
+                                mma16<M>(s[m][blk], qa[m][4*j + w][0], 0u, qa[m][4*j + w][1], 0u,
+                                        b0, b1);
+                            }
+                        }
+                    }
+            }
+            // this lane: head n (+8m), positions 8*blk + 2t + {0, 1}
+            float kscale[2][2], vfactor[2][2];
+            int vtop = vref;
+            if(E4M3)
+            {
+                uint32_t vb[2];
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+                {
+                    const uint32_t kb = *reinterpret_cast<const uint16_t *>(st + 2*L::KV_BYTES
+                            + 8*blk + 2*t);
+                    kscale[blk][0] = scale_value(kb & 0xFFu);
+                    kscale[blk][1] = scale_value(kb >> 8);
+                    vb[blk] = *reinterpret_cast<const uint16_t *>(st + 2*L::KV_BYTES + PD_TILE
+                            + 8*blk + 2*t);
+#pragma unroll
+                    for(int i = 0; i < 2; ++i)
+                    {
+                        const int e = 8*blk + 2*t + i < nv ? (int)(vb[blk] >> 8*i & 0xFFu) : 0;
+                        vtop = max(vtop, e);
+                    }
+                }
+                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for(int i = 0; i < 2; ++i)
+                    {
+                        // the scale of a row behind the length may be anything: keep it out
+                        const int e = 8*blk + 2*t + i < nv
+                                ? (int)(vb[blk] >> 8*i & 0xFFu) - vtop + 127 + LIFT : 0;
+                        vfactor[blk][i] = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
+                    }
+            }
+            float ntop[MT];
+            bool moved = E4M3 && vtop != vref;
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+            {
+                ntop[m] = top[m];
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for(int i = 0; i < 2; ++i)
+                    {
+                        float z = s[m][blk][i]*qscale[m];
+                        if(E4M3)
+                        {
+                            z *= kscale[blk][i];
+                        }
+                        z = 8*blk + 2*t + i < nv ? z : -CUDART_INF_F;
+                        s[m][blk][i] = z;
+                        ntop[m] = fmaxf(ntop[m], z);
+                    }
+                ntop[m] = fmaxf(ntop[m], __shfl_xor_sync(0xffffffffu, ntop[m], 1));
+                ntop[m] = fmaxf(ntop[m], __shfl_xor_sync(0xffffffffu, ntop[m], 2));
+                moved = moved || ntop[m] != top[m];
+            }
+            if(__any_sync(0xffffffffu, moved))
+            {
+                float back = 1.0f;
+                if(E4M3)
+                {
+                    const int e = vref - vtop + 127;
+                    back = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
+                    vref = vtop;
+                }
+#pragma unroll
+                for(int m = 0; m < MT; ++m)
+                {
+                    const float shrink = ntop[m] == top[m] ? 1.0f : ex2(top[m] - ntop[m]);
+                    top[m] = ntop[m];
+                    sum[m] *= shrink;
+                    const float f = shrink*back;
+#pragma unroll
+                    for(int e = 0; e < NBLK; ++e)
+#pragma unroll
+                        for(int i = 0; i < 4; ++i)
+                            acc[m][e][i] *= f;
+                }
+            }
+            uint32_t pa[MT][4];
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+            {
+                // no finite score yet: every weight is exp2(-inf) = 0
+                const float ref = top[m] == -CUDART_INF_F ? 0.0f : top[m];
+#pragma unroll
+                for(int blk = 0; blk < 2; ++blk)
+                {
+                    float p[2];
+#pragma unroll
+                    for(int i = 0; i < 2; ++i)
+                    {
+                        p[i] = ex2(s[m][blk][i] - ref);
+                        sum[m] += p[i];
+                        if(E4M3)
+                        {
+                            p[i] *= vfactor[blk][i];
+                        }
+                        else if(HALF)
+                        {
+                            p[i] *= (float)(1 << LIFT);
+                        }
+                    }
+                    const uint32_t up = pack2<M>(p[0], p[1]);
+                    const float2 kept = unpack2<M>(up);
+                    pa[m][2*blk] = up;
+                    pa[m][2*blk + 1] = pack2<M>(p[0] - kept.x, p[1] - kept.y);
+                }
+            }
+            // ---- O += P V
+            if(!E4M3)
+            {
+                const int r = lane & 15, col = lane >> 4;
+#pragma unroll
+                for(int e = 0; e < NBLK; e += 2)
+                {
+                    uint32_t vb[4];
+                    ldmatrix4_trans(vb, smem_addr(st + L::KV_BYTES + L::offset(r, e + col, false)));
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+                    {
+                        mma16<M>(acc[m][e], pa[m][0], pa[m][1], pa[m][2], pa[m][3], vb[0], vb[1]);
+                        mma16<M>(acc[m][e + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], vb[2],
+                                vb[3]);
+                    }
+                }
+            }
+            else
+            {
+                constexpr int VW = DP == 64 ? 2 : 4;         // words of a lane's piece of a row
+#pragma unroll
+                for(int q4 = 0; q4 < (DP + 127)/128; ++q4)
+                {
+                    uint32_t vw[4][VW];
+#pragma unroll
+                    for(int role = 0; role < 4; ++role)
+                    {
+                        const int r = 2*t + (role & 1) + 8*(role >> 1);
+                        if(DP == 64)
+                        {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(st + L::KV_BYTES
+                                    + L::offset(r, n >> 1, false) + 8*(n & 1));
+                            vw[role][0] = v.x;
+                            vw[role][1] = v.y;
+                        }
+                        else
+                        {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(st + L::KV_BYTES
+                                    + L::offset(r, n + 8*q4, false));
+                            vw[role][0] = v.x;
+                            vw[role][1] = v.y;
+                            vw[role][VW - 2] = DP == 64 ? v.x : v.z;
+                            vw[role][VW - 1] = DP == 64 ? v.y : v.w;
+                        }
+                    }
+#pragma unroll
+                    for(int w = 0; w < VW; ++w)
+#pragma unroll
+                        for(int pair = 0; pair < 2; ++pair)
+                        {
+                            // codes 2*pair, 2*pair + 1 of the word, positions 2t and 2t + 1
+                            const uint32_t sel = pair ? 0x7362u : 0x5140u;
+                            const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], sel);
+                            const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], sel);
+#pragma unroll
+                            for(int odd = 0; odd < 2; ++odd)
+                            {
+                                const int e = 16*q4 + 4*w + 2*pair + odd;
+                                const uint32_t b0 = e4m3x2_to_half2(odd ? lo >> 16 : lo & 0xFFFFu);
+                                const uint32_t b1 = e4m3x2_to_half2(odd ? hi >> 16 : hi & 0xFFFFu);
+#pragma unroll
+                                for(int m = 0; m < MT; ++m)
+                                {
+                                    mma16<M>(acc[m][e], pa[m][0], pa[m][1], pa[m][2], pa[m][3],
+                                            b0, b1);
+                                }
+                            }
+                        }
+                }
+            }
+        }
+
+        // ---- end of the segment: join the warps of the worker, then write the unit, or
+        // this share's part of it
+        const bool complete = x == unit_begin && seg_end == unit_end;
+        const int part = 2*worker + (x == unit_begin ? 1 : 0);
+        const float drop = HALF ? 1.0f/(float)(1 << LIFT) : 1.0f;
+        const float vscale = E4M3 ? scale_value((uint32_t)vref) : 1.0f;
+#pragma unroll
+        for(int m = 0; m < MT; ++m)
+        {
+            sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
+            sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
+            float o[NBLK][2];
+#pragma unroll
+            for(int e = 0; e < NBLK; ++e)
+            {
+                o[e][0] = (acc[m][e][0] + acc[m][e][2])*drop*vscale;
+                o[e][1] = (acc[m][e][1] + acc[m][e][3])*drop*vscale;
+            }
+            if(wpw > 1)
+            {
+                if(t == 0)
+                {
+                    top_s[warp][n] = top[m];
+                    sum_s[warp][n] = sum[m];
+                }
+                float *mw = merge + warp*8*DP;
+#pragma unroll
+                for(int e = 0; e < NBLK; ++e)
+                {
+                    mw[(2*e)*32 + lane] = o[e][0];
+                    mw[(2*e + 1)*32 + lane] = o[e][1];
+                }
+                __syncthreads();
+                // every warp joins NBLK/WARPS blocks of the columns, same lanes, same heads
+                float big = -CUDART_INF_F;
+#pragma unroll
+                for(int w = 0; w < WARPS; ++w)
+                {
+                    big = fmaxf(big, top_s[w][n]);
+                }
+                const float ref = big == -CUDART_INF_F ? 0.0f : big;
+                float den = 0.0f, wgt[WARPS];
+#pragma unroll
+                for(int w = 0; w < WARPS; ++w)
+                {
+                    wgt[w] = ex2(top_s[w][n] - ref);
+                    den = fmaf(wgt[w], sum_s[w][n], den);
+                }
+                constexpr int MY = NBLK/WARPS;
+#pragma unroll
+                for(int i = 0; i < MY; ++i)
+                {
+                    const int e = warp*MY + i;
+                    float z0 = 0.0f, z1 = 0.0f;
+#pragma unroll
+                    for(int w = 0; w < WARPS; ++w)
+                    {
+                        z0 = fmaf(wgt[w], merge[w*8*DP + (2*e)*32 + lane], z0);
+                        z1 = fmaf(wgt[w], merge[w*8*DP + (2*e + 1)*32 + lane], z1);
+                    }
+                    write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, e, z0, z1, den, kvh,
+                            h0, heads, b);
+                }
+                if(warp == 0 && t == 0)
+                {
+                    write_sums<MT>(a, complete, part, m, n, big, den, kvh, h0, heads, b);
+                }
+                __syncthreads();
+            }
+            else
+            {
+#pragma unroll
+                for(int e = 0; e < NBLK; ++e)
+                {
+                    write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, e, o[e][0], o[e][1],
+                            sum[m], kvh, h0, heads, b);
+                }
+                if(t == 0)
+                {
+                    write_sums<MT>(a, complete, part, m, n, top[m], sum[m], kvh, h0, heads, b);
+                }
+            }
+        }
+
+        // ---- next unit
+        x = seg_end;
+        unit_begin = unit_end;
+        if(++hu == HU && x < end)
+        {
+            hu = 0;
+            do
+            {
+                ++b;
+                nt = unit_tiles(a, held_len(a, b));
+            }
+            while(nt == 0);
+        }
+    }
+}
+
+// Joins the parts of the units that fell into several shares, and answers those with
+// nothing to attend to.  A block takes 256 values of a unit.
+constexpr int PD_JOIN_THREADS = 256;
+constexpr int PD_JOIN_PARTS = 64;            // parts whose weights are held at a time
+
+template<typename T, bool E4M3, int DP, int MT>
+__global__ void __launch_bounds__(PD_JOIN_THREADS)
+paged_join_kernel(const PagedDecodeArgs a, int blocks)
+{
+    using L = PagedTile<E4M3, DP>;
+    constexpr int PIECES = MT*8*DP/PD_JOIN_THREADS;
+    __shared__ int red_s[3][PD_JOIN_THREADS/32];
+    __shared__ float weight_s[PD_JOIN_PARTS][8];
+    __shared__ float big_s[8][PD_JOIN_THREADS/8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
+    const int unit = blockIdx.x/PIECES, piece = blockIdx.x - unit*PIECES;
+    const int b = unit/HU, hu = unit - b*HU;
+    // tiles of all sequences, and of those before this one
+    int total = 0, before = 0;
+    for(int i = tid; i < a.batch; i += PD_JOIN_THREADS)
+    {
+        const int tiles = unit_tiles(a, held_len(a, i))*HU;
+        total += tiles;
+        before += i < b ? tiles : 0;
+    }
+#pragma unroll
+    for(int o = 16; o > 0; o >>= 1)
+    {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if(lane == 0)
+    {
+        red_s[0][warp] = total;
+        red_s[1][warp] = before;
+    }
+    __syncthreads();
+    total = before = 0;
+    for(int w = 0; w < PD_JOIN_THREADS/32; ++w)
+    {
+        total += red_s[0][w];
+        before += red_s[1][w];
+    }
+    const int nt = unit_tiles(a, held_len(a, b));
+    const PagedShares sh = paged_shares<L::WARPS>(total, blocks);
+    const int x0 = before + hu*nt;
+    const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
+    const int kvh = hu/htiles, h0 = (hu - kvh*htiles)*8*MT, heads = min(8*MT, a.group - h0);
+    // before any return: the block's end must not come before the first kernel's
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if(first == last)
+    {
+        return;                              // one worker had it all and wrote it
+    }
+    // value `piece*256 + tid` of the unit, in the order of write_part
+    const int value = piece*PD_JOIN_THREADS + tid;
+    const int m = value/(8*DP), reg = (value - m*8*DP) >> 5;
+    const int n = lane >> 2, c = 2*(lane & 3) + (reg & 1), col = L::column(reg >> 1, c);
+    const int g = 8*m + n;
+    const size_t qh = ((size_t)kvh*a.group + h0 + g)*a.batch + b;
+    // the first share holds the unit's beginning in its second part, the others in their first
+    const int parts = last - first + 1;
+    float big = -CUDART_INF_F;
+    for(int i = tid >> 3; i < parts; i += PD_JOIN_THREADS/8)
+    {
+        const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
+        big = fmaxf(big, a.part_sums[(p*MT + m)*8 + (tid & 7)].x);
+    }
+    big_s[tid & 7][tid >> 3] = big;
+    __syncthreads();
+    float ref = -CUDART_INF_F;
+    for(int i = 0; i < PD_JOIN_THREADS/8; ++i)
+    {
+        ref = fmaxf(ref, big_s[n][i]);
+    }
+    float other = -CUDART_INF_F;
+    for(int i = 0; i < PD_JOIN_THREADS/8; ++i)
+    {
+        other = fmaxf(other, big_s[tid & 7][i]);
+    }
+    ref = ref == -CUDART_INF_F ? 0.0f : ref;
+    other = other == -CUDART_INF_F ? 0.0f : other;
+    __shared__ float share_s[PD_JOIN_PARTS][8];
+    float num = 0.0f, den = 0.0f;
+    for(int i0 = 0; i0 < parts; i0 += PD_JOIN_PARTS)
+    {
+        const int count = min(PD_JOIN_PARTS, parts - i0);
+        __syncthreads();
+        for(int i = tid >> 3; i < count; i += PD_JOIN_THREADS/8)
+        {
+            const size_t p = 2*(size_t)(first + i0 + i) + (i0 + i == 0 ? 1 : 0);
+            const float2 ts = a.part_sums[(p*MT + m)*8 + (tid & 7)];
+            const float w = ex2(ts.x - other);
+            weight_s[i][tid & 7] = w;
+            share_s[i][tid & 7] = w*ts.y;
+        }
+        __syncthreads();
+#pragma unroll 8
+        for(int i = 0; i < count; ++i)
+        {
+            const size_t p = 2*(size_t)(first + i0 + i) + (i0 + i == 0 ? 1 : 0);
+            num = fmaf(weight_s[i][n], a.part_o[(p*MT + m)*8*DP + reg*32 + lane], num);
+            den += share_s[i][n];
+        }
+    }
+    if(g < heads)
+    {
+        if(col < a.head)
+        {
+            ((T *)a.out)[qh*a.head + col] = from_f<T>(den == 0.0f ? 0.0f : num/den);
+        }
+        if(reg == 0 && (lane & 3) == 0 && a.lse_out)
+        {
+            a.lse_out[qh] = den == 0.0f ? -CUDART_INF_F : (ref + log2f(den))*PD_LN2;
+        }
+    }
+}
+
+// Tensor-core kernel: rows of a multiple of 16 bytes on 16-byte boundaries, pages of a
+// multiple of 16 positions, tiles and prefix sums that fit their integers and buffers.
 struct PagedDecodePlan
 {
-    int nsplit, chunk;
+    bool fast;
+    int dp, mt, grid, whole;             // fast
+    int nsplit, chunk;                   // generic
     size_t bytes;
 };
 
 static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_t max_blocks,
-        int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected)
+        int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected, int page_format)
 {
-    PagedDecodePlan p;
+    PagedDecodePlan p = {};
     const int64_t listed = num_selected > 0 ? num_selected : max_blocks;
     const int64_t heads = batch*group*kv_heads;
-    int64_t nsplit = (148*8 + heads - 1)/std::max<int64_t>(heads, 1);
+    const bool e4m3 = page_format == NNTILE_B200_PAGES_E4M3;
+    p.dp = head <= 64 ? 64 : head <= 128 ? 128 : 256;
+    // two tiles of heads a pass halve the reads of groups above 8; the accumulators of 256
+    // columns leave no registers for it
+    p.mt = group > 8 && p.dp < 256 ? 2 : 1;
+    const int64_t htiles = (group + 8*p.mt - 1)/(8*p.mt);
+    const int64_t unit_tiles = listed*(page_size/PD_TILE);
+    const int64_t units = batch*kv_heads*htiles;
+    p.fast = page_size % PD_TILE == 0 && head % (e4m3 ? 16 : 8) == 0 && batch < 4096
+            && unit_tiles*units < (int64_t)1 << 30 && units < (int64_t)1 << 24;
+    if(p.fast)
+    {
+        const int warps = p.dp == 256 ? 4 : 8;
+        const int64_t total = unit_tiles*units;
+        if(unit_tiles <= 2*warps)
+        {
+            // short units: a block each while there are few, a warp each when there are many
+            p.whole = units >= 2*PD_SMS ? 1 : warps;
+            const int64_t per = warps/p.whole;
+            p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(PD_SMS, (units + per - 1)/per));
+        }
+        else
+        {
+            p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(PD_SMS, (total + warps - 1)/warps));
+            p.bytes = (size_t)2*p.grid*warps*p.mt*8*(p.dp*sizeof(float) + sizeof(float2));
+        }
+    }
     const int64_t rows = listed*page_size;
+    int64_t nsplit = (PD_SMS*8 + heads - 1)/std::max<int64_t>(heads, 1);
     nsplit = std::min(nsplit, (rows + 255)/256);
     nsplit = std::max<int64_t>(1, std::min(nsplit, std::max<int64_t>(listed, 1)));
     const int64_t chunk = std::max<int64_t>(1, (listed + nsplit - 1)/nsplit);
     p.chunk = (int)chunk;
     p.nsplit = (int)std::max<int64_t>(1, (listed + chunk - 1)/chunk);
-    p.bytes = (size_t)heads*p.nsplit*(size_t)(head + 1)*sizeof(float);
     return p;
+}
+
+static size_t paged_generic_bytes(const PagedDecodePlan &p, int64_t head, int64_t heads)
+{
+    return (size_t)heads*p.nsplit*(size_t)(head + 1)*sizeof(float);
+}
+
+template<typename T, bool E4M3, int DP, int MT>
+static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDecodePlan &plan)
+{
+    using L = PagedTile<E4M3, DP>;
+    static PerDeviceOnce once;
+    int dev = -1;
+    if(cudaGetDevice(&dev) != cudaSuccess || !once.ensure(dev, []
+    {
+        return cudaFuncSetAttribute(paged_decode_kernel<T, E4M3, DP, MT>,
+                cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) == cudaSuccess;
+    }))
+    {
+        return NNTILE_B200_E_LAUNCH;
+    }
+    paged_decode_kernel<T, E4M3, DP, MT><<<plan.grid, L::WARPS*32, L::SMEM, s>>>(a);
+    if(launch_status() != NNTILE_B200_OK) return NNTILE_B200_E_LAUNCH;
+    if(a.whole) return NNTILE_B200_OK;
+    // starts while the first kernel still runs and waits for its results on the device
+    const int htiles = (a.group + 8*MT - 1)/(8*MT);
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.batch*a.kv_heads*htiles*(MT*8*DP/PD_JOIN_THREADS));
+    cfg.blockDim = dim3(PD_JOIN_THREADS);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, E4M3, DP, MT>, a, plan.grid) != cudaSuccess)
+    {
+        cudaGetLastError();
+        return NNTILE_B200_E_LAUNCH;
+    }
+    return launch_status();
 }
 
 template<typename T>
@@ -265,11 +1351,18 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
         return NNTILE_B200_E_ALIGN;
     }
     if(!aligned16(workspace)) return NNTILE_B200_E_ALIGN;
-    const PagedDecodePlan plan = paged_decode_plan(head, page_size, max_blocks, batch, group,
-            kv_heads, num_selected);
-    if(workspace_bytes < plan.bytes) return NNTILE_B200_E_SCRATCH;
+    PagedDecodePlan plan = paged_decode_plan(head, page_size, max_blocks, batch, group, kv_heads,
+            num_selected, page_format);
     const int64_t heads = batch*group*kv_heads;
-    if(heads*plan.nsplit > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    const uintptr_t rows16 = (uintptr_t)k_pages | (uintptr_t)v_pages
+            | (e4m3 ? (uintptr_t)k_scales | (uintptr_t)v_scales : 0);
+    plan.fast = plan.fast && (rows16 & 15) == 0 && ((uintptr_t)q & 3) == 0;
+    if(!plan.fast)
+    {
+        plan.bytes = paged_generic_bytes(plan, head, heads);
+        if(heads*plan.nsplit > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    }
+    if(workspace_bytes < plan.bytes) return NNTILE_B200_E_SCRATCH;
     PagedDecodeArgs a;
     a.head = (int)head;
     a.page_size = (int)page_size;
@@ -291,11 +1384,24 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.out = out;
     a.lse_out = lse_out;
     a.part_o = static_cast<float *>(workspace);
-    a.part_lse = a.part_o + (size_t)heads*plan.nsplit*(size_t)head;
+    a.part_lse = a.part_o + (size_t)heads*plan.nsplit*(size_t)head;      // generic kernel
+    a.part_sums = reinterpret_cast<float2 *>(a.part_o + (plan.fast
+            ? (size_t)2*plan.grid*(plan.dp == 256 ? 4 : 8)*plan.mt*8*plan.dp : 0));
+    a.whole = plan.whole;
     a.status = status;
     a.nsplit = plan.nsplit;
     a.chunk = plan.chunk;
     cudaStream_t s = as_stream(stream);
+    if(plan.fast)
+    {
+#define NB200_PD(E, P, M) launch_fast<T, E, P, M>(s, a, plan)
+#define NB200_PD_P(E) (plan.dp == 64 ? (plan.mt == 1 ? NB200_PD(E, 64, 1) : NB200_PD(E, 64, 2)) \
+        : plan.dp == 128 ? (plan.mt == 1 ? NB200_PD(E, 128, 1) : NB200_PD(E, 128, 2)) \
+        : NB200_PD(E, 256, 1))
+        return e4m3 ? NB200_PD_P(true) : NB200_PD_P(false);
+#undef NB200_PD_P
+#undef NB200_PD
+    }
     const unsigned grid = (unsigned)(heads*plan.nsplit);
     const int epl = (int)((head + 31)/32);
 #define NB200_PD(E, N) paged_decode_generic_kernel<T, E, N><<<grid, PD_WARPS*32, 0, s>>>(a)
@@ -328,8 +1434,16 @@ extern "C" size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, in
     {
         return 0;
     }
-    return paged_decode_plan(head, page_size, max_blocks, batch, group, kv_heads,
-            num_selected).bytes;
+    // enough for either page format and any alignment of the pages
+    size_t most = 16;
+    for(int format : {NNTILE_B200_PAGES_SAME, NNTILE_B200_PAGES_E4M3})
+    {
+        const PagedDecodePlan p = paged_decode_plan(head, page_size, max_blocks, batch, group,
+                kv_heads, num_selected, format);
+        most = std::max(most, std::max(p.bytes, paged_generic_bytes(p, head,
+                batch*group*kv_heads)));
+    }
+    return most;
 }
 
 #define NB200_PAGED_DECODE_ENTRY(SFX, T) \
