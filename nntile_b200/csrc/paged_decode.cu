@@ -1283,6 +1283,21 @@ static size_t paged_generic_bytes(const PagedDecodePlan &p, int64_t head, int64_
     return (size_t)heads*p.nsplit*(size_t)(head + 1)*sizeof(float);
 }
 
+// What a caller provides: enough for either page format and any alignment of the pages.
+static size_t paged_decode_bytes(int64_t head, int64_t page_size, int64_t max_blocks,
+        int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected)
+{
+    size_t most = 16;
+    for(int format : {NNTILE_B200_PAGES_SAME, NNTILE_B200_PAGES_E4M3})
+    {
+        const PagedDecodePlan p = paged_decode_plan(head, page_size, max_blocks, batch, group,
+                kv_heads, num_selected, format);
+        most = std::max(most, std::max(p.bytes, paged_generic_bytes(p, head,
+                batch*group*kv_heads)));
+    }
+    return most;
+}
+
 template<typename T, bool E4M3, int DP, int MT>
 static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDecodePlan &plan)
 {
@@ -1357,12 +1372,12 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     const uintptr_t rows16 = (uintptr_t)k_pages | (uintptr_t)v_pages
             | (e4m3 ? (uintptr_t)k_scales | (uintptr_t)v_scales : 0);
     plan.fast = plan.fast && (rows16 & 15) == 0 && ((uintptr_t)q & 3) == 0;
-    if(!plan.fast)
+    if(!plan.fast && heads*plan.nsplit > INT32_MAX) return NNTILE_B200_E_SHAPE;
+    if(workspace_bytes < paged_decode_bytes(head, page_size, max_blocks, batch, group, kv_heads,
+            num_selected))
     {
-        plan.bytes = paged_generic_bytes(plan, head, heads);
-        if(heads*plan.nsplit > INT32_MAX) return NNTILE_B200_E_SHAPE;
+        return NNTILE_B200_E_SCRATCH;
     }
-    if(workspace_bytes < plan.bytes) return NNTILE_B200_E_SCRATCH;
     PagedDecodeArgs a;
     a.head = (int)head;
     a.page_size = (int)page_size;
@@ -1434,16 +1449,7 @@ extern "C" size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, in
     {
         return 0;
     }
-    // enough for either page format and any alignment of the pages
-    size_t most = 16;
-    for(int format : {NNTILE_B200_PAGES_SAME, NNTILE_B200_PAGES_E4M3})
-    {
-        const PagedDecodePlan p = paged_decode_plan(head, page_size, max_blocks, batch, group,
-                kv_heads, num_selected, format);
-        most = std::max(most, std::max(p.bytes, paged_generic_bytes(p, head,
-                batch*group*kv_heads)));
-    }
-    return most;
+    return paged_decode_bytes(head, page_size, max_blocks, batch, group, kv_heads, num_selected);
 }
 
 #define NB200_PAGED_DECODE_ENTRY(SFX, T) \
