@@ -44,7 +44,8 @@ struct PagedDecodeArgs
     float *part_o, *part_lse;
     float2 *part_sums;
     uint32_t *status;
-    int whole;                           // > 0: whole units only, that many warps each
+    int wpw;                             // warps of a worker
+    int whole;                           // workers take whole units, nothing is joined
     int nsplit, chunk;                   // chunk: list positions per split (blocks)
 };
 
@@ -236,7 +237,6 @@ paged_decode_join_kernel(const PagedDecodeArgs a, int heads)
 
 constexpr int PD_SMS = 148;
 constexpr int PD_TILE = 16;                  // positions of a tile
-constexpr int PD_TILES_PER_WARP = 32;        // from here on a warp is a worker of its own
 
 // Layout of one kernel variant.  DP: head size rounded up to 64, 128 or 256 (columns behind
 // the head stay zero in the ring); MT: tiles of 8 query heads that share a pass.
@@ -452,10 +452,10 @@ struct PagedShares
 };
 
 template<int WARPS>
-__host__ __device__ inline PagedShares paged_shares(int total, int blocks)
+__host__ __device__ inline PagedShares paged_shares(int total, int blocks, int wpw)
 {
     PagedShares s;
-    s.wpw = total >= blocks*WARPS*PD_TILES_PER_WARP ? 1 : WARPS;
+    s.wpw = wpw;
     s.workers = blocks*(WARPS/s.wpw);
     s.share = (total + s.workers - 1)/s.workers;
     s.share = (s.share + s.wpw - 1)/s.wpw*s.wpw;
@@ -507,7 +507,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
     if(a.whole)
     {
         // whole units, no joining: unit = sequence*HU + (kv head, head tile)
-        wpw = a.whole;
+        wpw = a.wpw;
         worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
         const long long units = (long long)a.batch*HU;
         const int workers = gridDim.x*(WARPS/wpw);
@@ -546,7 +546,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
     }
     else
     {
-        const PagedShares sh = paged_shares<WARPS>(total, gridDim.x);
+        const PagedShares sh = paged_shares<WARPS>(total, gridDim.x, a.wpw);
         wpw = sh.wpw;
         worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
         begin = (int)min((long long)total, (long long)worker*sh.share);
@@ -1107,120 +1107,118 @@ paged_decode_kernel(const PagedDecodeArgs a)
 }
 
 // Joins the parts of the units that fell into several shares, and answers those with
-// nothing to attend to.  A block takes 256 values of a unit.
-constexpr int PD_JOIN_THREADS = 256;
-constexpr int PD_JOIN_PARTS = 64;            // parts whose weights are held at a time
+// nothing to attend to.  A piece is 128 of the 8*DP values of 8 heads, four a lane, all of
+// head lane % 8; `wpp` warps share the parts of a piece and meet in shared memory: one warp
+// while units are many and their parts few, eight when a few units have many parts each.
+constexpr int PD_JOIN_WARPS = 8;
+
+struct JoinState                         // four values of a head, not yet divided by the sum
+{
+    float top, sum;
+    float4 o;
+};
+
+__device__ __forceinline__ void join_add(JoinState &s, float top, float sum, const float4 &o)
+{
+    const float ntop = fmaxf(s.top, top);
+    const float ref = ntop == -CUDART_INF_F ? 0.0f : ntop;
+    const float x = ex2(s.top - ref), y = ex2(top - ref);
+    s.top = ntop;
+    s.sum = s.sum*x + sum*y;
+    s.o.x = s.o.x*x + o.x*y;
+    s.o.y = s.o.y*x + o.y*y;
+    s.o.z = s.o.z*x + o.z*y;
+    s.o.w = s.o.w*x + o.w*y;
+}
 
 template<typename T, bool E4M3, int DP, int MT>
-__global__ void __launch_bounds__(PD_JOIN_THREADS)
-paged_join_kernel(const PagedDecodeArgs a, int blocks)
+__global__ void __launch_bounds__(PD_JOIN_WARPS*32)
+paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
 {
     using L = PagedTile<E4M3, DP>;
-    constexpr int PIECES = MT*8*DP/PD_JOIN_THREADS;
-    __shared__ int red_s[3][PD_JOIN_THREADS/32];
-    __shared__ float weight_s[PD_JOIN_PARTS][8];
-    __shared__ float big_s[8][PD_JOIN_THREADS/8];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int PIECES = MT*8*DP/128;
+    __shared__ float2 sums_s[PD_JOIN_WARPS][32];
+    __shared__ float4 o_s[PD_JOIN_WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
-    const int unit = blockIdx.x/PIECES, piece = blockIdx.x - unit*PIECES;
-    const int b = unit/HU, hu = unit - b*HU;
+    const int id = (blockIdx.x*PD_JOIN_WARPS + warp)/wpp;
+    const int unit = id/PIECES, piece = id - unit*PIECES;
+    const int b = min(unit/HU, a.batch - 1), hu = unit - b*HU;
     // tiles of all sequences, and of those before this one
     int total = 0, before = 0;
-    for(int i = tid; i < a.batch; i += PD_JOIN_THREADS)
+    for(int i = lane; i < a.batch; i += 32)
     {
         const int tiles = unit_tiles(a, held_len(a, i))*HU;
         total += tiles;
         before += i < b ? tiles : 0;
     }
-#pragma unroll
-    for(int o = 16; o > 0; o >>= 1)
-    {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if(lane == 0)
-    {
-        red_s[0][warp] = total;
-        red_s[1][warp] = before;
-    }
-    __syncthreads();
-    total = before = 0;
-    for(int w = 0; w < PD_JOIN_THREADS/32; ++w)
-    {
-        total += red_s[0][w];
-        before += red_s[1][w];
-    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    before = __reduce_add_sync(0xffffffffu, before);
     const int nt = unit_tiles(a, held_len(a, b));
-    const PagedShares sh = paged_shares<L::WARPS>(total, blocks);
+    const PagedShares sh = paged_shares<L::WARPS>(total, blocks, a.wpw);
     const int x0 = before + hu*nt;
     const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
-    const int kvh = hu/htiles, h0 = (hu - kvh*htiles)*8*MT, heads = min(8*MT, a.group - h0);
+    const int m = piece*128/(8*DP), off = piece*128 - m*8*DP + 4*lane;   // in the part's values
     // before any return: the block's end must not come before the first kernel's
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if(first == last)
+    // one worker had it all and wrote it, or (the last block) there is no such unit
+    const bool none = first == last || unit >= a.batch*HU;
+    JoinState s = {-CUDART_INF_F, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    if(!none)
     {
-        return;                              // one worker had it all and wrote it
+        // the first share holds the unit's beginning in its second part, the others in their
+        // first
+        const int parts = last - first + 1;
+#pragma unroll 4
+        for(int i = warp % wpp; i < parts; i += wpp)
+        {
+            const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
+            const float2 ts = a.part_sums[(p*MT + m)*8 + (lane & 7)];
+            const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (p*MT + m)*8*DP + off);
+            join_add(s, ts.x, ts.y, o);
+        }
     }
-    // value `piece*256 + tid` of the unit, in the order of write_part
-    const int value = piece*PD_JOIN_THREADS + tid;
-    const int m = value/(8*DP), reg = (value - m*8*DP) >> 5;
-    const int n = lane >> 2, c = 2*(lane & 3) + (reg & 1), col = L::column(reg >> 1, c);
-    const int g = 8*m + n;
-    const size_t qh = ((size_t)kvh*a.group + h0 + g)*a.batch + b;
-    // the first share holds the unit's beginning in its second part, the others in their first
-    const int parts = last - first + 1;
-    float big = -CUDART_INF_F;
-    for(int i = tid >> 3; i < parts; i += PD_JOIN_THREADS/8)
+    if(wpp > 1)
     {
-        const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
-        big = fmaxf(big, a.part_sums[(p*MT + m)*8 + (tid & 7)].x);
-    }
-    big_s[tid & 7][tid >> 3] = big;
-    __syncthreads();
-    float ref = -CUDART_INF_F;
-    for(int i = 0; i < PD_JOIN_THREADS/8; ++i)
-    {
-        ref = fmaxf(ref, big_s[n][i]);
-    }
-    float other = -CUDART_INF_F;
-    for(int i = 0; i < PD_JOIN_THREADS/8; ++i)
-    {
-        other = fmaxf(other, big_s[tid & 7][i]);
-    }
-    ref = ref == -CUDART_INF_F ? 0.0f : ref;
-    other = other == -CUDART_INF_F ? 0.0f : other;
-    __shared__ float share_s[PD_JOIN_PARTS][8];
-    float num = 0.0f, den = 0.0f;
-    for(int i0 = 0; i0 < parts; i0 += PD_JOIN_PARTS)
-    {
-        const int count = min(PD_JOIN_PARTS, parts - i0);
+        sums_s[warp][lane] = make_float2(s.top, s.sum);
+        o_s[warp][lane] = s.o;
         __syncthreads();
-        for(int i = tid >> 3; i < count; i += PD_JOIN_THREADS/8)
+        if(warp % wpp != 0)
         {
-            const size_t p = 2*(size_t)(first + i0 + i) + (i0 + i == 0 ? 1 : 0);
-            const float2 ts = a.part_sums[(p*MT + m)*8 + (tid & 7)];
-            const float w = ex2(ts.x - other);
-            weight_s[i][tid & 7] = w;
-            share_s[i][tid & 7] = w*ts.y;
+            return;
         }
-        __syncthreads();
-#pragma unroll 8
-        for(int i = 0; i < count; ++i)
+        for(int w = 1; w < wpp; ++w)
         {
-            const size_t p = 2*(size_t)(first + i0 + i) + (i0 + i == 0 ? 1 : 0);
-            num = fmaf(weight_s[i][n], a.part_o[(p*MT + m)*8*DP + reg*32 + lane], num);
-            den += share_s[i][n];
+            const float2 ts = sums_s[warp + w][lane];
+            join_add(s, ts.x, ts.y, o_s[warp + w][lane]);
         }
     }
-    if(g < heads)
+    if(none)
     {
-        if(col < a.head)
+        return;
+    }
+    // values off .. off + 3: accumulator register off/32, lanes off%32 .. + 3, which are the
+    // four quads of head n's two columns each
+    const int n = lane & 7, reg = off >> 5;
+    const int kvh = hu/htiles, h0 = (hu - kvh*htiles)*8*MT, g = 8*m + n;
+    if(h0 + g < a.group)
+    {
+        const size_t qh = ((size_t)kvh*a.group + h0 + g)*a.batch + b;
+        const float inv = s.sum == 0.0f ? 0.0f : 1.0f/s.sum;
+        const float v[4] = {s.o.x, s.o.y, s.o.z, s.o.w};
+#pragma unroll
+        for(int t = 0; t < 4; ++t)
         {
-            ((T *)a.out)[qh*a.head + col] = from_f<T>(den == 0.0f ? 0.0f : num/den);
+            const int col = L::column(reg >> 1, 2*t + (reg & 1));
+            if(col < a.head)
+            {
+                ((T *)a.out)[qh*a.head + col] = from_f<T>(v[t]*inv);
+            }
         }
-        if(reg == 0 && (lane & 3) == 0 && a.lse_out)
+        if(a.lse_out && reg == 0)
         {
-            a.lse_out[qh] = den == 0.0f ? -CUDART_INF_F : (ref + log2f(den))*PD_LN2;
+            a.lse_out[qh] = s.sum == 0.0f ? -CUDART_INF_F
+                    : ((s.top == -CUDART_INF_F ? 0.0f : s.top) + log2f(s.sum))*PD_LN2;
         }
     }
 }
@@ -1230,7 +1228,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks)
 struct PagedDecodePlan
 {
     bool fast;
-    int dp, mt, grid, whole;             // fast
+    int dp, mt, grid, wpw, whole;        // fast
     int nsplit, chunk;                   // generic
     size_t bytes;
 };
@@ -1255,11 +1253,14 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
     {
         const int warps = p.dp == 256 ? 4 : 8;
         const int64_t total = unit_tiles*units;
+        // Workers are warps when there are units enough for most of a warp's share to be of
+        // one or two of them; with fewer units the warps of a block work together, which
+        // makes a part of a unit eight times as long and the parts to join eight times fewer.
+        p.wpw = units >= 2*PD_SMS ? 1 : warps;
         if(unit_tiles <= 2*warps)
         {
-            // short units: a block each while there are few, a warp each when there are many
-            p.whole = units >= 2*PD_SMS ? 1 : warps;
-            const int64_t per = warps/p.whole;
+            p.whole = 1;
+            const int64_t per = warps/p.wpw;
             p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(PD_SMS, (units + per - 1)/per));
         }
         else
@@ -1321,12 +1322,14 @@ static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDeco
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.batch*a.kv_heads*htiles*(MT*8*DP/PD_JOIN_THREADS));
-    cfg.blockDim = dim3(PD_JOIN_THREADS);
+    const int wpp = a.wpw == 1 ? 1 : PD_JOIN_WARPS;
+    const unsigned warps = (unsigned)a.batch*a.kv_heads*htiles*(MT*8*DP/128)*wpp;
+    cfg.gridDim = dim3((warps + PD_JOIN_WARPS - 1)/PD_JOIN_WARPS);
+    cfg.blockDim = dim3(PD_JOIN_WARPS*32);
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, E4M3, DP, MT>, a, plan.grid) != cudaSuccess)
+    if(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, E4M3, DP, MT>, a, plan.grid, wpp) != cudaSuccess)
     {
         cudaGetLastError();
         return NNTILE_B200_E_LAUNCH;
@@ -1402,6 +1405,7 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.part_lse = a.part_o + (size_t)heads*plan.nsplit*(size_t)head;      // generic kernel
     a.part_sums = reinterpret_cast<float2 *>(a.part_o + (plan.fast
             ? (size_t)2*plan.grid*(plan.dp == 256 ? 4 : 8)*plan.mt*8*plan.dp : 0));
+    a.wpw = plan.wpw;
     a.whole = plan.whole;
     a.status = status;
     a.nsplit = plan.nsplit;

@@ -15,6 +15,7 @@
 // most 17 units of 2^-23 of the sum of magnitudes a step; head <= 256 takes 32 steps, so
 // 32*17*2^-23 < 2^-13 of sum_d |q_d||k_d|, which a second product of magnitudes delivers.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.cuh"
 #include "per_device.hh"
@@ -39,6 +40,11 @@ __device__ __forceinline__ uint32_t score_key32(float s)
 {
     const uint32_t u = __float_as_uint(s + 0.0f);
     return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float score_of_key(uint32_t key)
+{
+    return __uint_as_float((key >> 31) ? key & 0x7FFFFFFFu : ~key);
 }
 
 struct PagedSelectArgs
@@ -145,156 +151,297 @@ __device__ __forceinline__ void score_mma<__half>(float (&c)[4], uint32_t a0, ui
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The positive or the negative halves of a word; NaN stays.
-template<typename T, bool POSITIVE>
-__device__ __forceinline__ uint32_t half_of(uint32_t w)
+// The positive and the negative parts of the two values of a word; NaN stays.
+template<typename T> __device__ __forceinline__ uint32_t positive2(uint32_t w);
+template<typename T> __device__ __forceinline__ uint32_t negative2(uint32_t w);
+template<> __device__ __forceinline__ uint32_t positive2<bf16>(uint32_t w)
 {
-    const float2 f = unpack2<T>(w);
-    return POSITIVE ? pack2<T>(max_nan(f.x, 0.0f), max_nan(f.y, 0.0f))
-            : pack2<T>(min_nan(f.x, 0.0f), min_nan(f.y, 0.0f));
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t negative2<bf16>(uint32_t w)
+{
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t positive2<__half>(uint32_t w)
+{
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t negative2<__half>(uint32_t w)
+{
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0u));
+    return r;
 }
 
-// A warp scores 8*NT neighbouring blocks of a unit against 16 heads at a time.  The order of
-// the head elements is free in a sum, so a lane's 16-byte piece t + 4j of a bounds row is the
-// operand of two steps as it comes from memory: no staging, 16 bytes a load, and with
-// NT = 2 for heads up to 128 sixteen loads (8 KB a warp) in flight at once.
-constexpr int SCORE_WARPS = 4;
+// Layout of the scoring kernel: a tile is 8 blocks of a unit, whose bounds (kmin, then kmax:
+// 4*head contiguous bytes each) a warp copies into its private ring in shared memory and
+// consumes itself; every warp of the grid takes the same number of neighbouring tiles.  The
+// order of the head elements is free in a sum, so a lane's 16-byte piece t + 4j of a row is
+// the operand of two steps of the tensor instruction as it lies in memory.
+constexpr int SCORE_WARPS = 8;
+constexpr int SCORE_SMS = 148;
 
-template<typename T, int DP, int NT, bool WIDE>
-__global__ void __launch_bounds__(SCORE_WARPS*32)
+template<int DP>
+struct ScoreTile
+{
+    static constexpr int HALF = DP/8;                    // 16-byte pieces of kmin, of kmax
+    static constexpr int STAGE = 8*2*HALF*16;
+    static constexpr int STAGES = 24576/STAGE < 8 ? 24576/STAGE : 8;
+    static constexpr int SMEM = SCORE_WARPS*STAGES*STAGE;
+    static constexpr int PASSES = 8*2*HALF/32;           // copies a lane issues a tile
+    // the lanes that read together hold 4 pieces of 2 neighbouring rows: different banks
+    static __device__ __forceinline__ int offset(int r, int c)
+    {
+        return r*2*HALF*16 + ((c ^ (((r & 1) << 2) | ((r >> 1) & 3))) << 4);
+    }
+};
+
+// Tiles of a unit of sequence b, b's table held to its blocks.
+__device__ __forceinline__ int score_tiles(const PagedSelectArgs &a, int b, uint32_t *status)
+{
+    const int blocks = filled_blocks(a, b, status);
+    return blocks > a.num_selected ? (blocks + 7)/8 : 0;  // otherwise all of them are taken
+}
+
+template<typename T, int DP, bool WIDE>
+__global__ void __launch_bounds__(SCORE_WARPS*32, 1)
 paged_score_kernel(const PagedSelectArgs a)
 {
-    constexpr int JN = DP/32, PER_CTA = SCORE_WARPS*8*NT;
+    using L = ScoreTile<DP>;
+    constexpr int JN = DP/32, STAGES = L::STAGES, ROWS = WIDE ? 16 : 8, MT = WIDE ? 2 : 1;
+    extern __shared__ __align__(128) uint8_t score_smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = lane >> 2, t = lane & 3;
-    const int chunks = (a.max_blocks + PER_CTA - 1)/PER_CTA;
-    const int unit = blockIdx.x/chunks, chunk = blockIdx.x - unit*chunks;
-    const int b = unit % a.batch, kvh = unit/a.batch;
-    const int count = filled_blocks(a, b, a.status);
-    const int block0 = chunk*PER_CTA + warp*8*NT;
-    if(block0 >= count)
+    uint8_t *ring = score_smem + warp*STAGES*L::STAGE;
+    const int chunks = a.head/8;                          // of kmin
+    for(int i = lane; a.head < DP && i < STAGES*L::STAGE/16; i += 32)
+    {
+        reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncwarp();
+
+    // ---- this warp's share of all tiles, and the sequence it begins in
+    int total = 0;
+    for(int i0 = 0; i0 < a.batch; i0 += 32)
+    {
+        total += i0 + lane < a.batch ? score_tiles(a, i0 + lane,
+                blockIdx.x == 0 && warp == 0 ? a.status : nullptr)*a.kv_heads : 0;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    const int workers = gridDim.x*SCORE_WARPS, worker = blockIdx.x*SCORE_WARPS + warp;
+    const int share = (total + workers - 1)/workers;
+    const int begin = (int)min((long long)total, (long long)worker*share);
+    int left = min(share, total - begin);
+    if(left <= 0)
     {
         return;
     }
-    // bounds of block n of each tile: kmin rows first, then kmax
-    uint4 kb[NT][2][JN];
-    bool missing[NT];
-#pragma unroll
-    for(int i = 0; i < NT; ++i)
+    int b = 0, seq_begin = 0;
+    for(int i0 = 0; i0 < a.batch; i0 += 32)
     {
-        const int block = block0 + 8*i + n;
-        const int page = block < count ? checked_page(a.block_table + (size_t)b*a.max_blocks,
-                block, a.num_pages, a.status) : -1;
-        missing[i] = page < 0;
-        const T *row = (const T *)a.bounds + ((size_t)max(page, 0)*a.kv_heads + kvh)*2*a.head;
+        const int mine = i0 + lane < a.batch ? score_tiles(a, i0 + lane, nullptr)*a.kv_heads : 0;
+        int scan = mine;
 #pragma unroll
-        for(int j = 0; j < JN; ++j)
+        for(int o = 1; o < 32; o <<= 1)
         {
-            const int h = 8*(t + 4*j);
-            const bool on = page >= 0 && h < a.head;
-            kb[i][0][j] = on ? __ldg(reinterpret_cast<const uint4 *>(row + h))
-                    : make_uint4(0u, 0u, 0u, 0u);
-            kb[i][1][j] = on ? __ldg(reinterpret_cast<const uint4 *>(row + a.head + h))
-                    : make_uint4(0u, 0u, 0u, 0u);
+            const int up = __shfl_up_sync(0xffffffffu, scan, o);
+            scan += lane >= o ? up : 0;
         }
+        const int all = __shfl_sync(0xffffffffu, scan, 31);
+        if(seq_begin + all > begin)
+        {
+            const unsigned hit = __ballot_sync(0xffffffffu, seq_begin + scan > begin);
+            const int k = __ffs((int)hit) - 1;
+            b = i0 + k;
+            seq_begin += __shfl_sync(0xffffffffu, scan - mine, k);
+            break;
+        }
+        seq_begin += all;
     }
-    float best[NT][2], error[NT][2];
-#pragma unroll
-    for(int i = 0; i < NT; ++i)
-#pragma unroll
-        for(int x = 0; x < 2; ++x)
-        {
-            best[i][x] = -CUDART_INF_F;
-            error[i][x] = 0.0f;
-        }
-    constexpr int ROWS = WIDE ? 16 : 8;
-    for(int g0 = 0; g0 < a.group; g0 += ROWS)
+
+    // ---- issuing side
+    int ib = b, ix = begin - seq_begin, ileft = left;
+    int icount = filled_blocks(a, ib, nullptr), int_ = score_tiles(a, ib, nullptr);
+    int ipos = 4;
+    long long look_row = -1;
+    auto issue = [&](int stage)
     {
-        // s: scores; up, down: sums of magnitudes, of the two halves of q (down is negative)
-        float s[NT][4], up[NT][4], down[NT][4];
-#pragma unroll
-        for(int i = 0; i < NT; ++i)
-#pragma unroll
-            for(int x = 0; x < 4; ++x)
-                s[i][x] = up[i][x] = down[i][x] = 0.0f;
-#pragma unroll
-        for(int j = 0; j < JN; ++j)
+        if(ileft > 0)
         {
-            uint32_t qw[WIDE ? 2 : 1][4];
-#pragma unroll
-            for(int m = 0; m < (WIDE ? 2 : 1); ++m)
+            if(ix >= int_*a.kv_heads)
             {
-                const int g = g0 + 8*m + n, h = 8*(t + 4*j);
-                const uint4 v = g < a.group && h < a.head ? *reinterpret_cast<const uint4 *>(
-                        (const T *)a.q + (((size_t)kvh*a.group + g)*a.batch + b)*a.head + h)
-                        : make_uint4(0u, 0u, 0u, 0u);
-                qw[m][0] = v.x;
-                qw[m][1] = v.y;
-                qw[m][2] = v.z;
-                qw[m][3] = v.w;
-            }
-#pragma unroll
-            for(int w = 0; w < 4; w += 2)
-            {
-                const uint32_t p0 = half_of<T, true>(qw[0][w]), p2 = half_of<T, true>(qw[0][w + 1]);
-                const uint32_t m0 = half_of<T, false>(qw[0][w]),
-                        m2 = half_of<T, false>(qw[0][w + 1]);
-                uint32_t p1 = 0u, p3 = 0u, m1 = 0u, m3 = 0u;
-                if(WIDE)
+                while(ix >= int_*a.kv_heads)
                 {
-                    p1 = half_of<T, true>(qw[WIDE][w]);
-                    p3 = half_of<T, true>(qw[WIDE][w + 1]);
-                    m1 = half_of<T, false>(qw[WIDE][w]);
-                    m3 = half_of<T, false>(qw[WIDE][w + 1]);
+                    ix -= int_*a.kv_heads;
+                    ++ib;
+                    int_ = score_tiles(a, ib, nullptr);
                 }
-#pragma unroll
-                for(int i = 0; i < NT; ++i)
+                icount = filled_blocks(a, ib, nullptr);
+                ipos = 4;
+            }
+            if(ipos == 4)
+            {
+                // pages of the next 32 blocks: four tiles, which may be of several units
+                ipos = 0;
+                look_row = -1;
+                const long long x = ix + (long long)(lane >> 3);
+                if(x < (long long)int_*a.kv_heads && (lane >> 3) < ileft)
                 {
-                    const uint4 lo = kb[i][0][j], hi = kb[i][1][j];
+                    const int kvh = (int)x/int_, block = ((int)x - kvh*int_)*8 + (lane & 7);
+                    if(block < icount)
+                    {
+                        const int page = checked_page(a.block_table + (size_t)ib*a.max_blocks,
+                                block, a.num_pages, a.status);
+                        look_row = page < 0 ? -1 : (long long)page*a.kv_heads + kvh;
+                    }
+                }
+            }
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage*L::STAGE);
+#pragma unroll
+            for(int i = 0; i < L::PASSES; ++i)
+            {
+                const int at = i*32 + lane, r = at/(2*L::HALF), c = at % (2*L::HALF);
+                const long long row = __shfl_sync(0xffffffffu, look_row, 8*ipos + r);
+                const int piece = c % L::HALF;
+                if(row >= 0 && piece < chunks)
+                {
+                    const uint8_t *src = (const uint8_t *)a.bounds + row*4*a.head
+                            + (piece + (c < L::HALF ? 0 : chunks))*16;
+                    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;"
+                            :: "r"(dst + L::offset(r, c)), "l"(src) : "memory");
+                }
+            }
+            ++ipos;
+            ++ix;
+            --ileft;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for(int s = 0; s < STAGES - 1; ++s)
+    {
+        issue(s);
+    }
+
+    // ---- consuming side
+    int nt = score_tiles(a, b, nullptr), count = filled_blocks(a, b, nullptr);
+    int kvh = (begin - seq_begin)/nt, tile = (begin - seq_begin) - kvh*nt;
+    bool fresh = true;
+    uint32_t q[MT][JN][4];
+    int stage = 0;
+    while(left-- > 0)
+    {
+        asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 2) : "memory");
+        __syncwarp();
+        issue(stage == 0 ? STAGES - 1 : stage - 1);
+        const uint8_t *st = ring + stage*L::STAGE;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        float best[2] = {-CUDART_INF_F, -CUDART_INF_F}, error[2] = {0.0f, 0.0f};
+        for(int g0 = 0; g0 < a.group; g0 += ROWS)
+        {
+            if(fresh || a.group > ROWS)
+            {
+#pragma unroll
+                for(int m = 0; m < MT; ++m)
+#pragma unroll
+                    for(int j = 0; j < JN; ++j)
+                    {
+                        const int g = g0 + 8*m + n, h = 8*(t + 4*j);
+                        const uint4 v = g < a.group && h < a.head
+                                ? *reinterpret_cast<const uint4 *>((const T *)a.q
+                                        + (((size_t)kvh*a.group + g)*a.batch + b)*a.head + h)
+                                : make_uint4(0u, 0u, 0u, 0u);
+                        q[m][j][0] = v.x;
+                        q[m][j][1] = v.y;
+                        q[m][j][2] = v.z;
+                        q[m][j][3] = v.w;
+                    }
+                fresh = false;
+            }
+            // s: scores; up, down: sums of magnitudes by the two parts of q (down is negative)
+            float s[4] = {}, up[4] = {}, down[4] = {};
+#pragma unroll
+            for(int j = 0; j < JN; ++j)
+            {
+                const uint4 lo = *reinterpret_cast<const uint4 *>(st + L::offset(n, t + 4*j));
+                const uint4 hi = *reinterpret_cast<const uint4 *>(st
+                        + L::offset(n, L::HALF + t + 4*j));
+#pragma unroll
+                for(int w = 0; w < 4; w += 2)
+                {
                     const uint32_t l0 = w ? lo.z : lo.x, l1 = w ? lo.w : lo.y;
                     const uint32_t h0 = w ? hi.z : hi.x, h1 = w ? hi.w : hi.y;
-                    score_mma<T>(s[i], p0, p1, p2, p3, h0, h1);
-                    score_mma<T>(s[i], m0, m1, m2, m3, l0, l1);
-                    score_mma<T>(up[i], p0, p1, p2, p3, h0 & 0x7FFF7FFFu, h1 & 0x7FFF7FFFu);
-                    score_mma<T>(down[i], m0, m1, m2, m3, l0 & 0x7FFF7FFFu, l1 & 0x7FFF7FFFu);
+                    const uint32_t p0 = positive2<T>(q[0][j][w]);
+                    const uint32_t p2 = positive2<T>(q[0][j][w + 1]);
+                    const uint32_t m0 = negative2<T>(q[0][j][w]);
+                    const uint32_t m2 = negative2<T>(q[0][j][w + 1]);
+                    const uint32_t p1 = WIDE ? positive2<T>(q[MT - 1][j][w]) : 0u;
+                    const uint32_t p3 = WIDE ? positive2<T>(q[MT - 1][j][w + 1]) : 0u;
+                    const uint32_t m1 = WIDE ? negative2<T>(q[MT - 1][j][w]) : 0u;
+                    const uint32_t m3 = WIDE ? negative2<T>(q[MT - 1][j][w + 1]) : 0u;
+                    score_mma<T>(s, p0, p1, p2, p3, h0, h1);
+                    score_mma<T>(up, p0, p1, p2, p3, h0 & 0x7FFF7FFFu, h1 & 0x7FFF7FFFu);
+                    score_mma<T>(s, m0, m1, m2, m3, l0, l1);
+                    score_mma<T>(down, m0, m1, m2, m3, l0 & 0x7FFF7FFFu, l1 & 0x7FFF7FFFu);
                 }
             }
-        }
 #pragma unroll
-        for(int i = 0; i < NT; ++i)
-#pragma unroll
-            for(int m = 0; m < (WIDE ? 2 : 1); ++m)
+            for(int m = 0; m < MT; ++m)
 #pragma unroll
                 for(int x = 0; x < 2; ++x)
                 {
                     if(g0 + 8*m + n < a.group)
                     {
-                        best[i][x] = max_nan(best[i][x], s[i][2*m + x]);
-                        error[i][x] = max_nan(error[i][x], up[i][2*m + x] - down[i][2*m + x]);
+                        best[x] = max_nan(best[x], s[2*m + x]);
+                        error[x] = max_nan(error[x], up[2*m + x] - down[2*m + x]);
                     }
                 }
-    }
+        }
 #pragma unroll
-    for(int i = 0; i < NT; ++i)
-    {
+        for(int o = 4; o < 32; o <<= 1)
+        {
+#pragma unroll
+            for(int x = 0; x < 2; ++x)
+            {
+                best[x] = max_nan(best[x], __shfl_xor_sync(0xffffffffu, best[x], o));
+                error[x] = max_nan(error[x], __shfl_xor_sync(0xffffffffu, error[x], o));
+            }
+        }
+        const int block = tile*8 + 2*t;
+        float2 *out = a.scores + ((size_t)kvh*a.batch + b)*a.max_blocks + block;
 #pragma unroll
         for(int x = 0; x < 2; ++x)
         {
-#pragma unroll
-            for(int o = 4; o < 32; o <<= 1)
+            // the copying side has reported a missing page; its score is the lowest
+            if(n == 0 && block + x < count)
             {
-                best[i][x] = max_nan(best[i][x], __shfl_xor_sync(0xffffffffu, best[i][x], o));
-                error[i][x] = max_nan(error[i][x], __shfl_xor_sync(0xffffffffu, error[i][x], o));
+                const bool gone = !page_in_pool(a.block_table[(size_t)b*a.max_blocks + block + x],
+                        a.num_pages);
+                out[x] = gone ? make_float2(-CUDART_INF_F, 0.0f)
+                        : make_float2(best[x], error[x]*SCORE_ERROR + SCORE_FLOOR);
             }
-            // column 2t + x of the tile is block 2t + x, whose bounds lane 4*(2t + x) loaded
-            const bool gone = __shfl_sync(0xffffffffu, (int)missing[i], 4*(2*t + x)) != 0;
-            const int block = block0 + 8*i + 2*t + x;
-            if(n == 0 && block < count)
+        }
+        if(++tile == nt)
+        {
+            tile = 0;
+            fresh = true;
+            if(++kvh == a.kv_heads && left > 0)
             {
-                a.scores[(size_t)unit*a.max_blocks + block] = gone
-                        ? make_float2(-CUDART_INF_F, 0.0f)
-                        : make_float2(best[i][x], error[i][x]*SCORE_ERROR + SCORE_FLOOR);
+                kvh = 0;
+                do
+                {
+                    ++b;
+                    nt = score_tiles(a, b, nullptr);
+                }
+                while(nt == 0);
+                count = filled_blocks(a, b, nullptr);
             }
         }
     }
@@ -333,10 +480,11 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ float fred[PICK_WARPS];
     __shared__ int listed_s, list_s[PICK_LIST];
     __shared__ unsigned long long list_key_s[PICK_LIST], cut_s;
-    __shared__ int equal_want_s;
+    __shared__ int equal_want_s, bin_s[256], hit_s, hits_s, rank_s;
+    __shared__ uint32_t low_s, high_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int unit = blockIdx.x, b = unit % a.batch, kvh = unit/a.batch;
-    const int n = filled_blocks(a, b, nullptr), S = a.num_selected;
+    const int n = filled_blocks(a, b, a.status), S = a.num_selected;
     int32_t *out = a.selected + (size_t)unit*S;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if(n <= S)
@@ -391,47 +539,98 @@ paged_pick_kernel(const PagedSelectArgs a)
     float sure_in = CUDART_INF_F, sure_out = -CUDART_INF_F;
     if(want > 0 && !unsure)
     {
-        // the want-th highest score: halve the range of keys; a threshold that exactly
-        // `want` scores reach ends the search early
-        uint32_t lo = score_key32(low), hi = score_key32(high);      // count(>= lo) >= want
-        while(lo < hi)
+        // The want-th highest score: count the scores in 256 equal bins of the range that holds
+        // it, go on with the bin it lies in; two or three rounds leave a single score, or a
+        // threshold that exactly the wanted number reaches.  Missing pages (-inf) go into the
+        // lowest bin.
+        int rank = want;                         // from the top of [low, high]
+        low = fmaxf(low, -FLT_MAX);
+        high = fmaxf(high, -FLT_MAX);
+        while(low < high)
         {
-            const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;
-            int c = 0;
+            for(int i = tid; i < 256; i += PICK_THREADS)
+            {
+                bin_s[i] = 0;
+            }
+            if(tid == 0)
+            {
+                low_s = ~0u;
+                high_s = 0u;
+            }
+            __syncthreads();
+            // halves: the range of finite numbers may itself not be one
+            const float origin = 0.5f*low, scale = 256.0f/(0.5f*high - origin);
+            auto bin = [&](float s) { return min(255, (int)((0.5f*s - origin)*scale)); };
             for(int i = begin + tid; i < end; i += PICK_THREADS)
             {
-                c += score_key32(score(i)) >= mid ? 1 : 0;
+                const float s = fmaxf(score(i), -FLT_MAX);
+                if(s >= low && s <= high)
+                {
+                    atomicAdd(&bin_s[bin(s)], 1);
+                }
             }
-            c = block_sum(c, red);
-            if(c >= want) lo = mid;
-            else hi = mid - 1u;
-            if(c == want)
+            __syncthreads();
+            if(warp == 0)
             {
-                break;
-            }
-        }
-        // the least score that reaches it is the want-th highest
-        float last = CUDART_INF_F;
-        for(int i = begin + tid; i < end; i += PICK_THREADS)
-        {
-            const float s = score(i);
-            last = score_key32(s) >= lo ? fminf(last, s) : last;
-        }
+                // lane 0 has the top eight bins
+                int c[8], sum = 0;
 #pragma unroll
-        for(int o = 16; o > 0; o >>= 1)
-        {
-            last = fminf(last, __shfl_xor_sync(0xffffffffu, last, o));
+                for(int k = 0; k < 8; ++k)
+                {
+                    c[k] = bin_s[255 - 8*lane - k];
+                    sum += c[k];
+                }
+                int scan = sum;
+#pragma unroll
+                for(int o = 1; o < 32; o <<= 1)
+                {
+                    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+                    scan += lane >= o ? up : 0;
+                }
+                int above = scan - sum;
+                if(above < rank && scan >= rank)
+                {
+#pragma unroll
+                    for(int k = 0; k < 8; ++k)
+                    {
+                        if(above < rank && above + c[k] >= rank)
+                        {
+                            hit_s = 255 - 8*lane - k;
+                            rank_s = rank - above;
+                            hits_s = c[k];
+                        }
+                        above += c[k];
+                    }
+                }
+            }
+            __syncthreads();
+            const int hit = hit_s, hits = hits_s;
+            rank = rank_s;
+            // the scores in that bin
+            uint32_t least = ~0u, most = 0u;
+            for(int i = begin + tid; i < end; i += PICK_THREADS)
+            {
+                const float s = fmaxf(score(i), -FLT_MAX);
+                if(s >= low && s <= high && bin(s) == hit)
+                {
+                    const uint32_t key = score_key32(s);
+                    least = min(least, key);
+                    most = max(most, key);
+                }
+            }
+            least = __reduce_min_sync(0xffffffffu, least);
+            most = __reduce_max_sync(0xffffffffu, most);
+            if(lane == 0 && most != 0u)
+            {
+                atomicMin(&low_s, least);
+                atomicMax(&high_s, most);
+            }
+            __syncthreads();
+            low = score_of_key(low_s);
+            high = rank == hits ? low : score_of_key(high_s);     // the bin's least it is
+            __syncthreads();
         }
-        __syncthreads();
-        if(lane == 0)
-        {
-            fred[warp] = last;
-        }
-        __syncthreads();
-        for(int w = 0; w < PICK_WARPS; ++w)
-        {
-            last = fminf(last, fred[w]);
-        }
+        const float last = low > -FLT_MAX ? low : -CUDART_INF_F;
         // exact values are within `error` of the scores, the want-th of each as well; a few
         // units in the last place more cover these two sums
         const float band = last > -CUDART_INF_F ? 2.0f*error + fabsf(last)*4e-7f : 0.0f;
@@ -604,15 +803,31 @@ static size_t select_bytes(int64_t units, int64_t max_blocks)
     return (size_t)units*max_blocks*(sizeof(float2) + sizeof(unsigned long long));
 }
 
-template<typename T, int DP, int NT>
+template<typename T, int DP, bool WIDE>
+static int launch_score_as(cudaStream_t s, const PagedSelectArgs &a, unsigned grid)
+{
+    static PerDeviceOnce once;
+    int dev = -1;
+    if(cudaGetDevice(&dev) != cudaSuccess || !once.ensure(dev, []
+    {
+        return cudaFuncSetAttribute(paged_score_kernel<T, DP, WIDE>,
+                cudaFuncAttributeMaxDynamicSharedMemorySize, ScoreTile<DP>::SMEM) == cudaSuccess;
+    }))
+    {
+        return NNTILE_B200_E_LAUNCH;
+    }
+    paged_score_kernel<T, DP, WIDE><<<grid, SCORE_WARPS*32, ScoreTile<DP>::SMEM, s>>>(a);
+    return launch_status();
+}
+
+template<typename T, int DP>
 static int launch_score(cudaStream_t s, const PagedSelectArgs &a)
 {
-    const int64_t per = SCORE_WARPS*8*NT;
-    const int64_t ctas = (int64_t)a.batch*a.kv_heads*((a.max_blocks + per - 1)/per);
-    if(ctas > INT32_MAX) return NNTILE_B200_E_SHAPE;
-    if(a.group > 8) paged_score_kernel<T, DP, NT, true><<<(unsigned)ctas, SCORE_WARPS*32, 0, s>>>(a);
-    else paged_score_kernel<T, DP, NT, false><<<(unsigned)ctas, SCORE_WARPS*32, 0, s>>>(a);
-    return launch_status();
+    const int64_t tiles = (int64_t)a.batch*a.kv_heads*((a.max_blocks + 7)/8);
+    const unsigned grid = (unsigned)std::min<int64_t>(SCORE_SMS,
+            (tiles + SCORE_WARPS - 1)/SCORE_WARPS);
+    return a.group > 8 ? launch_score_as<T, DP, true>(s, a, grid)
+            : launch_score_as<T, DP, false>(s, a, grid);
 }
 
 constexpr int PICK_CACHE_BYTES = 160 << 10;
@@ -702,14 +917,16 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.scores = static_cast<float2 *>(workspace);
     a.keys = reinterpret_cast<unsigned long long *>(a.scores + (size_t)units*max_blocks);
     a.status = status;
-    const bool vec = head % 8 == 0 && aligned16(q) && aligned16(bounds);
+    // 16-byte rows, and tiles that 30 bits can count
+    const bool vec = head % 8 == 0 && aligned16(q) && aligned16(bounds)
+            && units*((max_blocks + 7)/8) < (int64_t)1 << 30;
     cudaStream_t s = as_stream(stream);
     int st2 = NNTILE_B200_OK;
     if(max_blocks > num_selected)                // otherwise everything is taken
     {
-        if(vec && head <= 64) st2 = launch_score<T, 64, 4>(s, a);
-        else if(vec && head <= 128) st2 = launch_score<T, 128, 2>(s, a);
-        else if(vec) st2 = launch_score<T, 256, 1>(s, a);
+        if(vec && head <= 64) st2 = launch_score<T, 64>(s, a);
+        else if(vec && head <= 128) st2 = launch_score<T, 128>(s, a);
+        else if(vec) st2 = launch_score<T, 256>(s, a);
         else
         {
             const int64_t ctas = units*((max_blocks + 3)/4);
