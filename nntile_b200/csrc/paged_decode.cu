@@ -248,8 +248,14 @@ struct PagedTile
     static constexpr int CHUNKS = ROW_BYTES/16;          // 16-byte pieces of a row
     static constexpr int KV_BYTES = PD_TILE*ROW_BYTES;   // one of K, V
     static constexpr int STAGE = 2*KV_BYTES + (E4M3 ? 2*PD_TILE : 0);
-    static constexpr int RING = 196608/WARPS;
-    static constexpr int STAGES = RING/STAGE < 8 ? RING/STAGE : 8;
+    static constexpr int RING = 198144/WARPS;
+    static constexpr int STAGES = RING/STAGE < 12 ? RING/STAGE : 12;
+    // Tiles a warp takes at once.  A tile is one chain (scores, maximum, weights, values) of
+    // about a thousand cycles; short rows put two or four side by side, so that 8 warps ask
+    // for bytes as fast as HBM delivers them.
+    static constexpr int ABREAST = 8192/(2*KV_BYTES) < 1 ? 1 : 8192/(2*KV_BYTES);
+    static constexpr int AHEAD = STAGES - ABREAST;       // tiles in flight or waiting
+    static_assert(AHEAD >= ABREAST, "the ring must hold what is consumed and what is coming");
     static constexpr int NBLK = DP/8;                    // 8-column blocks of the output
     static constexpr int MERGE = WARPS*8*DP*4;           // one tile of 8 heads of every warp
     static constexpr int SMEM = WARPS*STAGES*STAGE + MERGE;
@@ -640,30 +646,27 @@ paged_decode_kernel(const PagedDecodeArgs a)
             {
                 nv_s[warp][stage] = nv;
             }
-            if(nv > 0)
+            // rows behind the length, and all of a tile without a page, are filled with zeros
+            const uint32_t dst = smem_addr(ring + stage*L::STAGE);
+            const long long at = row*row_bytes + crow*row_bytes + cchunk*16;
+            const uint8_t *ks = (const uint8_t *)a.k_pages + at;
+            const uint8_t *vs = (const uint8_t *)a.v_pages + at;
+            if(cchunk < chunks)
             {
-                const uint32_t dst = smem_addr(ring + stage*L::STAGE);
-                const long long at = row*row_bytes + crow*row_bytes + cchunk*16;
-                const uint8_t *ks = (const uint8_t *)a.k_pages + at;
-                const uint8_t *vs = (const uint8_t *)a.v_pages + at;
-                if(cchunk < chunks)
-                {
 #pragma unroll
-                    for(int i = 0; i < PD_TILE/RPP; ++i)
-                    {
-                        const int r = crow + i*RPP;
-                        const int bytes = r < nv ? 16 : 0;
-                        copy16(dst + L::offset(r, cchunk, E4M3), ks + (size_t)i*RPP*row_bytes,
-                                bytes);
-                        copy16(dst + L::KV_BYTES + L::offset(r, cchunk, false),
-                                vs + (size_t)i*RPP*row_bytes, bytes);
-                    }
-                }
-                if(E4M3 && lane < 2)
+                for(int i = 0; i < PD_TILE/RPP; ++i)
                 {
-                    copy16(dst + 2*L::KV_BYTES + lane*PD_TILE,
-                            (lane == 0 ? a.k_scales : a.v_scales) + row, 16);
+                    const int r = crow + i*RPP;
+                    const int bytes = r < nv ? 16 : 0;
+                    copy16(dst + L::offset(r, cchunk, E4M3), ks + (size_t)i*RPP*row_bytes, bytes);
+                    copy16(dst + L::KV_BYTES + L::offset(r, cchunk, false),
+                            vs + (size_t)i*RPP*row_bytes, bytes);
                 }
+            }
+            if(E4M3 && lane < 2)
+            {
+                copy16(dst + 2*L::KV_BYTES + lane*PD_TILE,
+                        (lane == 0 ? a.k_scales : a.v_scales) + row, nv > 0 ? 16 : 0);
             }
             ++ipos;
             ix += step;
@@ -672,7 +675,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
         copy_commit();
     };
 #pragma unroll
-    for(int s = 0; s < STAGES - 1; ++s)
+    for(int s = 0; s < L::AHEAD; ++s)
     {
         issue(s);
     }
@@ -758,26 +761,36 @@ paged_decode_kernel(const PagedDecodeArgs a)
         // scale so far
         int vref = 0;
 
-        while(mine < seg_end)
+        // N tiles at once: positions 16*j + 8*blk + 2t + {0, 1} of head n (+8m) are this lane's
+        auto process = [&](auto tiles)
         {
-            mine += step;
-            copy_wait<STAGES - 2>();
+            constexpr int N = decltype(tiles)::value;
+            copy_wait<L::AHEAD - L::ABREAST>();
             __syncwarp();
-            // the stage that was consumed last is free for every lane now
-            issue(stage == 0 ? STAGES - 1 : stage - 1);
-            const uint8_t *st = ring + stage*L::STAGE;
-            const int nv = nv_s[warp][stage];
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
-            if(nv == 0)
+            // what was consumed last is free for every lane now
+            const uint8_t *st[N];
+            int nv[N], some = 0;
+#pragma unroll
+            for(int j = 0; j < N; ++j)
             {
-                continue;
+                int to = stage + L::AHEAD;
+                to -= to >= STAGES ? STAGES : 0;
+                issue(to);
+                st[j] = ring + stage*L::STAGE;
+                nv[j] = nv_s[warp][stage];
+                some |= nv[j];
+                stage = stage + 1 == STAGES ? 0 : stage + 1;
             }
-            // ---- scores: two blocks of 8 positions
-            float s[MT][2][4];
+            if(some == 0)
+            {
+                return;
+            }
+            // ---- scores: two blocks of 8 positions a tile
+            float s[MT][2*N][4];
 #pragma unroll
             for(int m = 0; m < MT; ++m)
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int blk = 0; blk < 2*N; ++blk)
 #pragma unroll
                     for(int i = 0; i < 4; ++i)
                         s[m][blk][i] = 0.0f;
@@ -786,72 +799,79 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
 #pragma unroll
                 for(int k = 0; k < KSTEPS; ++k)
-                {
-                    uint32_t kb[4];
-                    ldmatrix4(kb, smem_addr(st + L::offset(r, 2*k + half, false)));
 #pragma unroll
-                    for(int m = 0; m < MT; ++m)
+                    for(int j = 0; j < N; ++j)
                     {
-                        mma16<M>(s[m][0], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[0], kb[1]);
-                        mma16<M>(s[m][1], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[2], kb[3]);
+                        uint32_t kb[4];
+                        ldmatrix4(kb, smem_addr(st[j] + L::offset(r, 2*k + half, false)));
+#pragma unroll
+                        for(int m = 0; m < MT; ++m)
+                        {
+                            mma16<M>(s[m][2*j], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[0], kb[1]);
+                            mma16<M>(s[m][2*j + 1], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[2],
+                                    kb[3]);
+                        }
                     }
-                }
             }
             else
             {
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int c4 = 0; c4 < DP/64; ++c4)
+                {
+                    uint4 kc[2*N];
 #pragma unroll
-                    for(int j = 0; j < DP/64; ++j)
+                    for(int blk = 0; blk < 2*N; ++blk)
                     {
-                        const uint4 kc = *reinterpret_cast<const uint4 *>(st
-                                + L::offset(8*blk + n, t + 4*j, true));
+                        kc[blk] = *reinterpret_cast<const uint4 *>(st[blk >> 1]
+                                + L::offset(8*(blk & 1) + n, t + 4*c4, true));
+                    }
 #pragma unroll
-                        for(int w = 0; w < 4; ++w)
+                    for(int w = 0; w < 4; ++w)
+#pragma unroll
+                        for(int blk = 0; blk < 2*N; ++blk)
                         {
-                            const uint32_t c = word4(kc, w);
+                            const uint32_t c = word4(kc[blk], w);
                             const uint32_t b0 = e4m3x2_to_half2(c & 0xFFFFu);
                             const uint32_t b1 = e4m3x2_to_half2(c >> 16);
 #pragma unroll
                             for(int m = 0; m < MT; ++m)
                             {
-                                mma16<M>(s[m][blk], qa[m][4*j + w][0], 0u, qa[m][4*j + w][1], 0u,
-                                        b0, b1);
+                                mma16<M>(s[m][blk], qa[m][4*c4 + w][0], 0u, qa[m][4*c4 + w][1],
+                                        0u, b0, b1);
                             }
                         }
-                    }
+                }
             }
-            // this lane: head n (+8m), positions 8*blk + 2t + {0, 1}
-            float kscale[2][2], vfactor[2][2];
+            float kscale[2*N][2], vfactor[2*N][2];
             int vtop = vref;
             if(E4M3)
             {
-                uint32_t vb[2];
+                uint32_t vb[2*N];
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int blk = 0; blk < 2*N; ++blk)
                 {
-                    const uint32_t kb = *reinterpret_cast<const uint16_t *>(st + 2*L::KV_BYTES
-                            + 8*blk + 2*t);
+                    const uint8_t *sc = st[blk >> 1] + 2*L::KV_BYTES + 8*(blk & 1) + 2*t;
+                    const uint32_t kb = *reinterpret_cast<const uint16_t *>(sc);
                     kscale[blk][0] = scale_value(kb & 0xFFu);
                     kscale[blk][1] = scale_value(kb >> 8);
-                    vb[blk] = *reinterpret_cast<const uint16_t *>(st + 2*L::KV_BYTES + PD_TILE
-                            + 8*blk + 2*t);
+                    vb[blk] = *reinterpret_cast<const uint16_t *>(sc + PD_TILE);
 #pragma unroll
                     for(int i = 0; i < 2; ++i)
                     {
-                        const int e = 8*blk + 2*t + i < nv ? (int)(vb[blk] >> 8*i & 0xFFu) : 0;
+                        const int e = 8*(blk & 1) + 2*t + i < nv[blk >> 1]
+                                ? (int)(vb[blk] >> 8*i & 0xFFu) : 0;
                         vtop = max(vtop, e);
                     }
                 }
                 vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
                 vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int blk = 0; blk < 2*N; ++blk)
 #pragma unroll
                     for(int i = 0; i < 2; ++i)
                     {
                         // the scale of a row behind the length may be anything: keep it out
-                        const int e = 8*blk + 2*t + i < nv
+                        const int e = 8*(blk & 1) + 2*t + i < nv[blk >> 1]
                                 ? (int)(vb[blk] >> 8*i & 0xFFu) - vtop + 127 + LIFT : 0;
                         vfactor[blk][i] = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
                     }
@@ -863,7 +883,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
             {
                 ntop[m] = top[m];
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int blk = 0; blk < 2*N; ++blk)
 #pragma unroll
                     for(int i = 0; i < 2; ++i)
                     {
@@ -872,7 +892,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         {
                             z *= kscale[blk][i];
                         }
-                        z = 8*blk + 2*t + i < nv ? z : -CUDART_INF_F;
+                        z = 8*(blk & 1) + 2*t + i < nv[blk >> 1] ? z : -CUDART_INF_F;
                         s[m][blk][i] = z;
                         ntop[m] = fmaxf(ntop[m], z);
                     }
@@ -903,14 +923,14 @@ paged_decode_kernel(const PagedDecodeArgs a)
                             acc[m][e][i] *= f;
                 }
             }
-            uint32_t pa[MT][4];
+            uint32_t pa[MT][N][4];
 #pragma unroll
             for(int m = 0; m < MT; ++m)
             {
                 // no finite score yet: every weight is exp2(-inf) = 0
                 const float ref = top[m] == -CUDART_INF_F ? 0.0f : top[m];
 #pragma unroll
-                for(int blk = 0; blk < 2; ++blk)
+                for(int blk = 0; blk < 2*N; ++blk)
                 {
                     float p[2];
 #pragma unroll
@@ -929,80 +949,101 @@ paged_decode_kernel(const PagedDecodeArgs a)
                     }
                     const uint32_t up = pack2<M>(p[0], p[1]);
                     const float2 kept = unpack2<M>(up);
-                    pa[m][2*blk] = up;
-                    pa[m][2*blk + 1] = pack2<M>(p[0] - kept.x, p[1] - kept.y);
+                    pa[m][blk >> 1][2*(blk & 1)] = up;
+                    pa[m][blk >> 1][2*(blk & 1) + 1] = pack2<M>(p[0] - kept.x, p[1] - kept.y);
                 }
             }
             // ---- O += P V
-            if(!E4M3)
+#pragma unroll
+            for(int j = 0; j < N; ++j)
             {
-                const int r = lane & 15, col = lane >> 4;
-#pragma unroll
-                for(int e = 0; e < NBLK; e += 2)
+                const uint8_t *sv = st[j] + L::KV_BYTES;
+                if(!E4M3)
                 {
-                    uint32_t vb[4];
-                    ldmatrix4_trans(vb, smem_addr(st + L::KV_BYTES + L::offset(r, e + col, false)));
+                    const int r = lane & 15, col = lane >> 4;
 #pragma unroll
-                    for(int m = 0; m < MT; ++m)
+                    for(int e = 0; e < NBLK; e += 2)
                     {
-                        mma16<M>(acc[m][e], pa[m][0], pa[m][1], pa[m][2], pa[m][3], vb[0], vb[1]);
-                        mma16<M>(acc[m][e + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], vb[2],
-                                vb[3]);
+                        uint32_t vb[4];
+                        ldmatrix4_trans(vb, smem_addr(sv + L::offset(r, e + col, false)));
+#pragma unroll
+                        for(int m = 0; m < MT; ++m)
+                        {
+                            mma16<M>(acc[m][e], pa[m][j][0], pa[m][j][1], pa[m][j][2],
+                                    pa[m][j][3], vb[0], vb[1]);
+                            mma16<M>(acc[m][e + 1], pa[m][j][0], pa[m][j][1], pa[m][j][2],
+                                    pa[m][j][3], vb[2], vb[3]);
+                        }
+                    }
+                }
+                else
+                {
+                    constexpr int VW = DP == 64 ? 2 : 4;     // words of a lane's piece of a row
+#pragma unroll
+                    for(int q4 = 0; q4 < (DP + 127)/128; ++q4)
+                    {
+                        uint32_t vw[4][VW];
+#pragma unroll
+                        for(int role = 0; role < 4; ++role)
+                        {
+                            const int r = 2*t + (role & 1) + 8*(role >> 1);
+                            if(DP == 64)
+                            {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(sv
+                                        + L::offset(r, n >> 1, false) + 8*(n & 1));
+                                vw[role][0] = v.x;
+                                vw[role][1] = v.y;
+                            }
+                            else
+                            {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(sv
+                                        + L::offset(r, n + 8*q4, false));
+                                vw[role][0] = v.x;
+                                vw[role][1] = v.y;
+                                vw[role][VW - 2] = DP == 64 ? v.x : v.z;
+                                vw[role][VW - 1] = DP == 64 ? v.y : v.w;
+                            }
+                        }
+#pragma unroll
+                        for(int w = 0; w < VW; ++w)
+#pragma unroll
+                            for(int pair = 0; pair < 2; ++pair)
+                            {
+                                // codes 2*pair, 2*pair + 1 of the word, positions 2t and 2t + 1
+                                const uint32_t sel = pair ? 0x7362u : 0x5140u;
+                                const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], sel);
+                                const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], sel);
+#pragma unroll
+                                for(int odd = 0; odd < 2; ++odd)
+                                {
+                                    const int e = 16*q4 + 4*w + 2*pair + odd;
+                                    const uint32_t b0 = e4m3x2_to_half2(odd ? lo >> 16
+                                            : lo & 0xFFFFu);
+                                    const uint32_t b1 = e4m3x2_to_half2(odd ? hi >> 16
+                                            : hi & 0xFFFFu);
+#pragma unroll
+                                    for(int m = 0; m < MT; ++m)
+                                    {
+                                        mma16<M>(acc[m][e], pa[m][j][0], pa[m][j][1],
+                                                pa[m][j][2], pa[m][j][3], b0, b1);
+                                    }
+                                }
+                            }
                     }
                 }
             }
+        };
+        while(mine < seg_end)
+        {
+            if(L::ABREAST > 1 && mine + (L::ABREAST - 1)*step < seg_end)
+            {
+                mine += L::ABREAST*step;
+                process(std::integral_constant<int, L::ABREAST>());
+            }
             else
             {
-                constexpr int VW = DP == 64 ? 2 : 4;         // words of a lane's piece of a row
-#pragma unroll
-                for(int q4 = 0; q4 < (DP + 127)/128; ++q4)
-                {
-                    uint32_t vw[4][VW];
-#pragma unroll
-                    for(int role = 0; role < 4; ++role)
-                    {
-                        const int r = 2*t + (role & 1) + 8*(role >> 1);
-                        if(DP == 64)
-                        {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(st + L::KV_BYTES
-                                    + L::offset(r, n >> 1, false) + 8*(n & 1));
-                            vw[role][0] = v.x;
-                            vw[role][1] = v.y;
-                        }
-                        else
-                        {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(st + L::KV_BYTES
-                                    + L::offset(r, n + 8*q4, false));
-                            vw[role][0] = v.x;
-                            vw[role][1] = v.y;
-                            vw[role][VW - 2] = DP == 64 ? v.x : v.z;
-                            vw[role][VW - 1] = DP == 64 ? v.y : v.w;
-                        }
-                    }
-#pragma unroll
-                    for(int w = 0; w < VW; ++w)
-#pragma unroll
-                        for(int pair = 0; pair < 2; ++pair)
-                        {
-                            // codes 2*pair, 2*pair + 1 of the word, positions 2t and 2t + 1
-                            const uint32_t sel = pair ? 0x7362u : 0x5140u;
-                            const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], sel);
-                            const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], sel);
-#pragma unroll
-                            for(int odd = 0; odd < 2; ++odd)
-                            {
-                                const int e = 16*q4 + 4*w + 2*pair + odd;
-                                const uint32_t b0 = e4m3x2_to_half2(odd ? lo >> 16 : lo & 0xFFFFu);
-                                const uint32_t b1 = e4m3x2_to_half2(odd ? hi >> 16 : hi & 0xFFFFu);
-#pragma unroll
-                                for(int m = 0; m < MT; ++m)
-                                {
-                                    mma16<M>(acc[m][e], pa[m][0], pa[m][1], pa[m][2], pa[m][3],
-                                            b0, b1);
-                                }
-                            }
-                        }
-                }
+                mine += step;
+                process(std::integral_constant<int, 1>());
             }
         }
 
@@ -1234,7 +1275,8 @@ struct PagedDecodePlan
 };
 
 static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_t max_blocks,
-        int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected, int page_format)
+        int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected, int page_format,
+        int64_t num_pages = 1)
 {
     PagedDecodePlan p = {};
     const int64_t listed = num_selected > 0 ? num_selected : max_blocks;
@@ -1248,7 +1290,7 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
     const int64_t unit_tiles = listed*(page_size/PD_TILE);
     const int64_t units = batch*kv_heads*htiles;
     p.fast = page_size % PD_TILE == 0 && head % (e4m3 ? 16 : 8) == 0 && batch < 4096
-            && unit_tiles*units < (int64_t)1 << 30 && units < (int64_t)1 << 24;
+            && unit_tiles*units < (int64_t)1 << 30 && units < (int64_t)1 << 24 && num_pages > 0;
     if(p.fast)
     {
         const int warps = p.dp == 256 ? 4 : 8;
@@ -1370,7 +1412,7 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     }
     if(!aligned16(workspace)) return NNTILE_B200_E_ALIGN;
     PagedDecodePlan plan = paged_decode_plan(head, page_size, max_blocks, batch, group, kv_heads,
-            num_selected, page_format);
+            num_selected, page_format, num_pages);
     const int64_t heads = batch*group*kv_heads;
     const uintptr_t rows16 = (uintptr_t)k_pages | (uintptr_t)v_pages
             | (e4m3 ? (uintptr_t)k_scales | (uintptr_t)v_scales : 0);

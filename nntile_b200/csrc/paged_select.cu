@@ -365,8 +365,9 @@ paged_score_kernel(const PagedSelectArgs a)
                     }
                 fresh = false;
             }
-            // s: scores; up, down: sums of magnitudes by the two parts of q (down is negative)
-            float s[4] = {}, up[4] = {}, down[4] = {};
+            // scores (s, less) and sums of magnitudes (up, down; down is negative) by the
+            // positive and the negative part of q: four chains of products
+            float s[4] = {}, less[4] = {}, up[4] = {}, down[4] = {};
 #pragma unroll
             for(int j = 0; j < JN; ++j)
             {
@@ -388,7 +389,7 @@ paged_score_kernel(const PagedSelectArgs a)
                     const uint32_t m3 = WIDE ? negative2<T>(q[MT - 1][j][w + 1]) : 0u;
                     score_mma<T>(s, p0, p1, p2, p3, h0, h1);
                     score_mma<T>(up, p0, p1, p2, p3, h0 & 0x7FFF7FFFu, h1 & 0x7FFF7FFFu);
-                    score_mma<T>(s, m0, m1, m2, m3, l0, l1);
+                    score_mma<T>(less, m0, m1, m2, m3, l0, l1);
                     score_mma<T>(down, m0, m1, m2, m3, l0 & 0x7FFF7FFFu, l1 & 0x7FFF7FFFu);
                 }
             }
@@ -399,7 +400,7 @@ paged_score_kernel(const PagedSelectArgs a)
                 {
                     if(g0 + 8*m + n < a.group)
                     {
-                        best[x] = max_nan(best[x], s[2*m + x]);
+                        best[x] = max_nan(best[x], s[2*m + x] + less[2*m + x]);
                         error[x] = max_nan(error[x], up[2*m + x] - down[2*m + x]);
                     }
                 }
