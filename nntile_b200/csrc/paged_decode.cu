@@ -16,10 +16,13 @@
 //     what HBM latency times bandwidth asks for; the ring runs on across units;
 //   - page numbers are looked up 32 tiles at a time, a lane each, ahead of the ring;
 //   - scores and weighted values go through the warp-level tensor instruction (m16n8k16, fp32
-//     accumulate).  Its 16 rows hold 8 query heads twice: for P.V the upper 8 rows take the
-//     weights rounded to 16 bits and the lower 8 what that rounding lost, so the weights count
-//     with 16 (bf16) or 22 (fp16) bits at no further instruction;
-//   - the running maximum is only applied to the accumulators when it moves.
+//     accumulate), transposed: keys and columns of V are its 16 rows, 8 query heads its
+//     columns, so no row is idle for groups up to 8 and the accumulators take half the
+//     registers of the other way round.  The weights go in twice, rounded to 16 bits and what
+//     that rounding lost, and so count with 16 (bf16) or 22 (fp16) bits;
+//   - weights refer to an exponent that follows the maximum only when a score passes it by
+//     2^4: most tiles need one vote instead of a maximum over lanes and a pass over the
+//     accumulators.
 #include <algorithm>
 #include <type_traits>
 
@@ -256,7 +259,7 @@ struct PagedTile
     static constexpr int ABREAST = 8192/(2*KV_BYTES) < 1 ? 1 : 8192/(2*KV_BYTES);
     static constexpr int AHEAD = STAGES - ABREAST;       // tiles in flight or waiting
     static_assert(AHEAD >= ABREAST, "the ring must hold what is consumed and what is coming");
-    static constexpr int NBLK = DP/8;                    // 8-column blocks of the output
+    static constexpr int MBLK = DP/16;                   // 16-column blocks of the output
     static constexpr int MERGE = WARPS*8*DP*4;           // one tile of 8 heads of every warp
     static constexpr int SMEM = WARPS*STAGES*STAGE + MERGE;
 
@@ -273,11 +276,11 @@ struct PagedTile
         const int x = rot ? ((r & 1) << 2) | ((r >> 1) & 3) : r & 7;
         return r*ROW_BYTES + ((c ^ x) << 4);
     }
-    // Column of the output that accumulator block e holds for B column c.
-    static __device__ __forceinline__ int column(int e, int c)
+    // Column of the output that row n (x = 0) or n + 8 (x = 1) of accumulator block i holds.
+    static __device__ __forceinline__ int column(int i, int x, int n)
     {
-        if(!E4M3) return 8*e + c;
-        return DP == 64 ? 8*c + e : (e >> 4)*128 + 16*c + (e & 15);
+        if(!E4M3) return 16*i + 8*x + n;
+        return DP == 64 ? 8*n + 2*i + x : (i >> 3)*128 + 16*n + 2*(i & 7) + x;
     }
 };
 
@@ -330,6 +333,13 @@ __device__ __forceinline__ void mma16<__half>(float (&c)[4], uint32_t a0, uint32
             "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transposes an 8x8 matrix of 16-bit values held as an accumulator's words
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t w)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
 }
 __device__ __forceinline__ float ex2(float x)
 {
@@ -402,46 +412,51 @@ __device__ __forceinline__ int held_len(const PagedDecodeArgs &a, int b)
     return held_length(a.lengths[b], a.max_blocks*a.page_size, bad);
 }
 
-// Two columns of head 8m + n, either final or into part `part` of the workspace, which
-// keeps a lane's values in the order of the accumulators: [part][m][2*block + i][lane].
+// The four values of accumulator block i (columns n and n + 8 of it, heads 8m + 2t and
+// 8m + 2t + 1), either final or into part `part` of the workspace: [part][m][head][column].
 template<typename T, bool E4M3, int DP, int MT>
 __device__ __forceinline__ void write_part(const PagedDecodeArgs &a, bool complete, int part,
-        int m, int lane, int e, float z0, float z1, float den, int kvh, int h0, int heads, int b)
+        int m, int lane, int i, const float (&z)[4], const float (&den)[2], int kvh, int h0,
+        int heads, int b)
 {
+    using L = PagedTile<E4M3, DP>;
     const int n = lane >> 2, t = lane & 3;
-    if(!complete)
+#pragma unroll
+    for(int y = 0; y < 2; ++y)
     {
-        float *o = a.part_o + ((size_t)part*MT + m)*8*DP;
-        o[(2*e)*32 + lane] = z0;
-        o[(2*e + 1)*32 + lane] = z1;
-        return;
-    }
-    const int g = 8*m + n;
-    if(g < heads)
-    {
-        using L = PagedTile<E4M3, DP>;
-        const float inv = den == 0.0f ? 0.0f : 1.0f/den;
-        T *out = (T *)a.out + (((size_t)kvh*a.group + h0 + g)*a.batch + b)*a.head;
-        const int c0 = L::column(e, 2*t), c1 = L::column(e, 2*t + 1);
-        if(c0 < a.head)
+        const int g = 8*m + 2*t + y;
+        if(!complete)
         {
-            out[c0] = from_f<T>(z0*inv);
+            float *o = a.part_o + (((size_t)part*MT + m)*8 + 2*t + y)*DP;
+            o[L::column(i, 0, n)] = z[y];
+            o[L::column(i, 1, n)] = z[2 + y];
         }
-        if(c1 < a.head)
+        else if(g < heads)
         {
-            out[c1] = from_f<T>(z1*inv);
+            const float inv = den[y] == 0.0f ? 0.0f : 1.0f/den[y];
+            T *out = (T *)a.out + (((size_t)kvh*a.group + h0 + g)*a.batch + b)*a.head;
+            const int c0 = L::column(i, 0, n), c1 = L::column(i, 1, n);
+            if(c0 < a.head)
+            {
+                out[c0] = from_f<T>(z[y]*inv);
+            }
+            if(c1 < a.head)
+            {
+                out[c1] = from_f<T>(z[2 + y]*inv);
+            }
         }
     }
 }
 
+// Reference exponent and sum of head `head` of tile m.
 template<int MT>
 __device__ __forceinline__ void write_sums(const PagedDecodeArgs &a, bool complete, int part,
-        int m, int n, float top, float sum, int kvh, int h0, int heads, int b)
+        int m, int head, float top, float sum, int kvh, int h0, int heads, int b)
 {
-    const int g = 8*m + n;
+    const int g = 8*m + head;
     if(!complete)
     {
-        a.part_sums[((size_t)part*MT + m)*8 + n] = make_float2(top, sum);
+        a.part_sums[((size_t)part*MT + m)*8 + head] = make_float2(top, sum);
     }
     else if(g < heads && a.lse_out)
     {
@@ -475,10 +490,13 @@ paged_decode_kernel(const PagedDecodeArgs a)
     using L = PagedTile<E4M3, DP>;
     using M = typename std::conditional<E4M3, __half, T>::type;      // operand format
     constexpr bool HALF = std::is_same<M, __half>::value;
-    // fp16 weights are lifted by 2^14 (they are at most 1), which keeps those down to 2^-38
-    // of the largest; bf16 has fp32's range
-    constexpr int LIFT = HALF ? 14 : 0;
-    constexpr int KSTEPS = DP/16, NBLK = L::NBLK, WARPS = L::WARPS, STAGES = L::STAGES;
+    // A weight is exp2(score - reference), and the reference only moves when a score passes it
+    // by more than SLACK: weights stay below 2^SLACK and most tiles do without a maximum.
+    // fp16 weights are lifted by 2^LIFT, which keeps those down to 2^-34 of the reference;
+    // bf16 has fp32's range.
+    constexpr int LIFT = HALF ? 10 : 0;
+    constexpr float SLACK = 4.0f;
+    constexpr int KSTEPS = DP/16, MBLK = L::MBLK, WARPS = L::WARPS, STAGES = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int nv_s[WARPS][STAGES];
     __shared__ float top_s[WARPS][8], sum_s[WARPS][8];
@@ -696,14 +714,14 @@ paged_decode_kernel(const PagedDecodeArgs a)
         const int heads = min(8*MT, a.group - h0);
 
         uint32_t qa[MT][KSTEPS][2];
-        float qscale[MT];
+        float qscale[MT][2];                             // of heads 2t, 2t + 1
 #pragma unroll
         for(int m = 0; m < MT; ++m)
         {
             const int g = 8*m + n;
             const T *qr = (const T *)a.q + (((size_t)kvh*a.group + h0 + min(g, heads - 1))
                     *a.batch + b)*D;
-            qscale[m] = a.scale_log2;
+            qscale[m][0] = qscale[m][1] = a.scale_log2;
 #pragma unroll
             for(int k = 0; k < KSTEPS; ++k)
 #pragma unroll
@@ -734,7 +752,9 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 const int e = (int)(__float_as_uint(amax) >> 23);        // 0 and 255: as it is
                 const int up = e == 255 ? 0 : max(-113, min(126, 141 - e));
                 const float lift = __uint_as_float((uint32_t)(127 + up) << 23);
-                qscale[m] *= __uint_as_float((uint32_t)(127 - up) << 23);
+                const float undo = __uint_as_float((uint32_t)(127 - up) << 23);
+                qscale[m][0] *= __shfl_sync(0xffffffffu, undo, 8*t);         // lane of head 2t
+                qscale[m][1] *= __shfl_sync(0xffffffffu, undo, 8*t + 4);
 #pragma unroll
                 for(int k = 0; k < KSTEPS; ++k)
 #pragma unroll
@@ -745,23 +765,25 @@ paged_decode_kernel(const PagedDecodeArgs a)
                     }
             }
         }
-        float acc[MT][NBLK][4], top[MT], sum[MT];
+        float acc[MT][MBLK][4], top[MT][2], sum[MT][2];
 #pragma unroll
         for(int m = 0; m < MT; ++m)
         {
-            top[m] = -CUDART_INF_F;
-            sum[m] = 0.0f;
+            top[m][0] = top[m][1] = -CUDART_INF_F;
+            sum[m][0] = sum[m][1] = 0.0f;
 #pragma unroll
-            for(int e = 0; e < NBLK; ++e)
+            for(int i = 0; i < MBLK; ++i)
 #pragma unroll
-                for(int i = 0; i < 4; ++i)
-                    acc[m][e][i] = 0.0f;
+                for(int r = 0; r < 4; ++r)
+                    acc[m][i][r] = 0.0f;
         }
         // 8-bit values: the accumulators count in units of 2^(vref - 127), the largest value
         // scale so far
         int vref = 0;
 
-        // N tiles at once: positions 16*j + 8*blk + 2t + {0, 1} of head n (+8m) are this lane's
+        // N tiles at once.  Keys and values are the 16-row operand, the query heads the 8
+        // columns: this lane holds the scores of positions n and n + 8 of a tile for heads 2t
+        // and 2t + 1, in the order [2*(position >= 8) + (head odd)].
         auto process = [&](auto tiles)
         {
             constexpr int N = decltype(tiles)::value;
@@ -785,31 +807,30 @@ paged_decode_kernel(const PagedDecodeArgs a)
             {
                 return;
             }
-            // ---- scores: two blocks of 8 positions a tile
-            float s[MT][2*N][4];
+            // ---- scores, in two sums of every other step: half as long a chain
+            float s[MT][N][2][4];
 #pragma unroll
             for(int m = 0; m < MT; ++m)
 #pragma unroll
-                for(int blk = 0; blk < 2*N; ++blk)
+                for(int j = 0; j < N; ++j)
 #pragma unroll
-                    for(int i = 0; i < 4; ++i)
-                        s[m][blk][i] = 0.0f;
+                    for(int r = 0; r < 4; ++r)
+                        s[m][j][0][r] = s[m][j][1][r] = 0.0f;
             if(!E4M3)
             {
-                const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+                const int r = lane & 15, col = lane >> 4;
 #pragma unroll
                 for(int k = 0; k < KSTEPS; ++k)
 #pragma unroll
                     for(int j = 0; j < N; ++j)
                     {
-                        uint32_t kb[4];
-                        ldmatrix4(kb, smem_addr(st[j] + L::offset(r, 2*k + half, false)));
+                        uint32_t ka[4];
+                        ldmatrix4(ka, smem_addr(st[j] + L::offset(r, 2*k + col, false)));
 #pragma unroll
                         for(int m = 0; m < MT; ++m)
                         {
-                            mma16<M>(s[m][2*j], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[0], kb[1]);
-                            mma16<M>(s[m][2*j + 1], qa[m][k][0], 0u, qa[m][k][1], 0u, kb[2],
-                                    kb[3]);
+                            mma16<M>(s[m][j][k & 1], ka[0], ka[1], ka[2], ka[3], qa[m][k][0],
+                                    qa[m][k][1]);
                         }
                     }
             }
@@ -818,93 +839,79 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                 for(int c4 = 0; c4 < DP/64; ++c4)
                 {
-                    uint4 kc[2*N];
+                    uint4 kc[N][2];
 #pragma unroll
-                    for(int blk = 0; blk < 2*N; ++blk)
-                    {
-                        kc[blk] = *reinterpret_cast<const uint4 *>(st[blk >> 1]
-                                + L::offset(8*(blk & 1) + n, t + 4*c4, true));
-                    }
+                    for(int j = 0; j < N; ++j)
+#pragma unroll
+                        for(int h = 0; h < 2; ++h)
+                        {
+                            kc[j][h] = *reinterpret_cast<const uint4 *>(st[j]
+                                    + L::offset(8*h + n, t + 4*c4, true));
+                        }
 #pragma unroll
                     for(int w = 0; w < 4; ++w)
 #pragma unroll
-                        for(int blk = 0; blk < 2*N; ++blk)
+                        for(int j = 0; j < N; ++j)
                         {
-                            const uint32_t c = word4(kc[blk], w);
-                            const uint32_t b0 = e4m3x2_to_half2(c & 0xFFFFu);
-                            const uint32_t b1 = e4m3x2_to_half2(c >> 16);
+                            const uint32_t c = word4(kc[j][0], w), d = word4(kc[j][1], w);
+                            const uint32_t a0 = e4m3x2_to_half2(c & 0xFFFFu);
+                            const uint32_t a1 = e4m3x2_to_half2(d & 0xFFFFu);
+                            const uint32_t a2 = e4m3x2_to_half2(c >> 16);
+                            const uint32_t a3 = e4m3x2_to_half2(d >> 16);
 #pragma unroll
                             for(int m = 0; m < MT; ++m)
                             {
-                                mma16<M>(s[m][blk], qa[m][4*c4 + w][0], 0u, qa[m][4*c4 + w][1],
-                                        0u, b0, b1);
+                                mma16<M>(s[m][j][w & 1], a0, a1, a2, a3, qa[m][4*c4 + w][0],
+                                        qa[m][4*c4 + w][1]);
                             }
                         }
                 }
             }
-            float kscale[2*N][2], vfactor[2*N][2];
-            int vtop = vref;
+            float kscale[N][2];
+            int vbyte[N][2];
+            bool moved = false;
             if(E4M3)
             {
-                uint32_t vb[2*N];
 #pragma unroll
-                for(int blk = 0; blk < 2*N; ++blk)
-                {
-                    const uint8_t *sc = st[blk >> 1] + 2*L::KV_BYTES + 8*(blk & 1) + 2*t;
-                    const uint32_t kb = *reinterpret_cast<const uint16_t *>(sc);
-                    kscale[blk][0] = scale_value(kb & 0xFFu);
-                    kscale[blk][1] = scale_value(kb >> 8);
-                    vb[blk] = *reinterpret_cast<const uint16_t *>(sc + PD_TILE);
+                for(int j = 0; j < N; ++j)
 #pragma unroll
-                    for(int i = 0; i < 2; ++i)
-                    {
-                        const int e = 8*(blk & 1) + 2*t + i < nv[blk >> 1]
-                                ? (int)(vb[blk] >> 8*i & 0xFFu) : 0;
-                        vtop = max(vtop, e);
-                    }
-                }
-                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
-#pragma unroll
-                for(int blk = 0; blk < 2*N; ++blk)
-#pragma unroll
-                    for(int i = 0; i < 2; ++i)
+                    for(int h = 0; h < 2; ++h)
                     {
                         // the scale of a row behind the length may be anything: keep it out
-                        const int e = 8*(blk & 1) + 2*t + i < nv[blk >> 1]
-                                ? (int)(vb[blk] >> 8*i & 0xFFu) - vtop + 127 + LIFT : 0;
-                        vfactor[blk][i] = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
+                        const uint8_t *sc = st[j] + 2*L::KV_BYTES + 8*h + n;
+                        kscale[j][h] = scale_value(sc[0]);
+                        vbyte[j][h] = 8*h + n < nv[j] ? (int)sc[PD_TILE] : 0;
+                        moved = moved || vbyte[j][h] > vref;
                     }
             }
-            float ntop[MT];
-            bool moved = E4M3 && vtop != vref;
 #pragma unroll
             for(int m = 0; m < MT; ++m)
-            {
-                ntop[m] = top[m];
 #pragma unroll
-                for(int blk = 0; blk < 2*N; ++blk)
+                for(int j = 0; j < N; ++j)
 #pragma unroll
-                    for(int i = 0; i < 2; ++i)
+                    for(int r = 0; r < 4; ++r)
                     {
-                        float z = s[m][blk][i]*qscale[m];
+                        float z = (s[m][j][0][r] + s[m][j][1][r])*qscale[m][r & 1];
                         if(E4M3)
                         {
-                            z *= kscale[blk][i];
+                            z *= kscale[j][r >> 1];
                         }
-                        z = 8*(blk & 1) + 2*t + i < nv[blk >> 1] ? z : -CUDART_INF_F;
-                        s[m][blk][i] = z;
-                        ntop[m] = fmaxf(ntop[m], z);
+                        z = 8*(r >> 1) + n < nv[j] ? z : -CUDART_INF_F;
+                        s[m][j][0][r] = z;
+                        moved = moved || z > top[m][r & 1] + SLACK;
                     }
-                ntop[m] = fmaxf(ntop[m], __shfl_xor_sync(0xffffffffu, ntop[m], 1));
-                ntop[m] = fmaxf(ntop[m], __shfl_xor_sync(0xffffffffu, ntop[m], 2));
-                moved = moved || ntop[m] != top[m];
-            }
             if(__any_sync(0xffffffffu, moved))
             {
                 float back = 1.0f;
                 if(E4M3)
                 {
+                    int vtop = vref;
+#pragma unroll
+                    for(int j = 0; j < N; ++j)
+                    {
+                        vtop = max(vtop, max(vbyte[j][0], vbyte[j][1]));
+                    }
+                    vtop = __reduce_max_sync(0xffffffffu, vtop);
                     const int e = vref - vtop + 127;
                     back = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
                     vref = vtop;
@@ -912,47 +919,68 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                 for(int m = 0; m < MT; ++m)
                 {
-                    const float shrink = ntop[m] == top[m] ? 1.0f : ex2(top[m] - ntop[m]);
-                    top[m] = ntop[m];
-                    sum[m] *= shrink;
-                    const float f = shrink*back;
+                    float f[2];
 #pragma unroll
-                    for(int e = 0; e < NBLK; ++e)
-#pragma unroll
-                        for(int i = 0; i < 4; ++i)
-                            acc[m][e][i] *= f;
-                }
-            }
-            uint32_t pa[MT][N][4];
-#pragma unroll
-            for(int m = 0; m < MT; ++m)
-            {
-                // no finite score yet: every weight is exp2(-inf) = 0
-                const float ref = top[m] == -CUDART_INF_F ? 0.0f : top[m];
-#pragma unroll
-                for(int blk = 0; blk < 2*N; ++blk)
-                {
-                    float p[2];
-#pragma unroll
-                    for(int i = 0; i < 2; ++i)
+                    for(int y = 0; y < 2; ++y)
                     {
-                        p[i] = ex2(s[m][blk][i] - ref);
-                        sum[m] += p[i];
-                        if(E4M3)
+                        float ntop = top[m][y];
+#pragma unroll
+                        for(int j = 0; j < N; ++j)
                         {
-                            p[i] *= vfactor[blk][i];
+                            ntop = fmaxf(ntop, fmaxf(s[m][j][0][y], s[m][j][0][2 + y]));
                         }
-                        else if(HALF)
+#pragma unroll
+                        for(int o = 4; o < 32; o <<= 1)
                         {
-                            p[i] *= (float)(1 << LIFT);
+                            ntop = fmaxf(ntop, __shfl_xor_sync(0xffffffffu, ntop, o));
                         }
+                        const float shrink = ntop == top[m][y] ? 1.0f : ex2(top[m][y] - ntop);
+                        top[m][y] = ntop;
+                        sum[m][y] *= shrink;
+                        f[y] = shrink*back;
                     }
-                    const uint32_t up = pack2<M>(p[0], p[1]);
-                    const float2 kept = unpack2<M>(up);
-                    pa[m][blk >> 1][2*(blk & 1)] = up;
-                    pa[m][blk >> 1][2*(blk & 1) + 1] = pack2<M>(p[0] - kept.x, p[1] - kept.y);
+#pragma unroll
+                    for(int i = 0; i < MBLK; ++i)
+#pragma unroll
+                        for(int r = 0; r < 4; ++r)
+                            acc[m][i][r] *= f[r & 1];
                 }
             }
+            // ---- weights, in two 16-bit parts, as the 8-column operand of the second product
+            uint32_t pb[MT][N][2][2];                    // part, positions >= 8
+#pragma unroll
+            for(int j = 0; j < N; ++j)
+#pragma unroll
+                for(int h = 0; h < 2; ++h)
+                {
+                    float lift = (float)(1 << LIFT);
+                    if(E4M3)
+                    {
+                        const int e = vbyte[j][h] - vref + 127 + LIFT;
+                        lift = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
+                    }
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+                    {
+                        float p[2];
+#pragma unroll
+                        for(int y = 0; y < 2; ++y)
+                        {
+                            // no finite score yet: every weight is exp2(-inf) = 0
+                            const float ref = top[m][y] == -CUDART_INF_F ? 0.0f : top[m][y];
+                            p[y] = ex2(s[m][j][0][2*h + y] - ref);
+                            sum[m][y] += p[y];
+                            if(HALF)
+                            {
+                                p[y] *= lift;
+                            }
+                        }
+                        const uint32_t up = pack2<M>(p[0], p[1]);
+                        const float2 kept = unpack2<M>(up);
+                        pb[m][j][0][h] = transpose8x8(up);
+                        pb[m][j][1][h] = transpose8x8(pack2<M>(p[0] - kept.x, p[1] - kept.y));
+                    }
+                }
             // ---- O += P V
 #pragma unroll
             for(int j = 0; j < N; ++j)
@@ -960,20 +988,18 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 const uint8_t *sv = st[j] + L::KV_BYTES;
                 if(!E4M3)
                 {
-                    const int r = lane & 15, col = lane >> 4;
+                    const int r = (lane & 7) + ((lane >> 4) << 3), col = (lane >> 3) & 1;
 #pragma unroll
-                    for(int e = 0; e < NBLK; e += 2)
+                    for(int i = 0; i < MBLK; ++i)
                     {
-                        uint32_t vb[4];
-                        ldmatrix4_trans(vb, smem_addr(sv + L::offset(r, e + col, false)));
+                        uint32_t va[4];
+                        ldmatrix4_trans(va, smem_addr(sv + L::offset(r, 2*i + col, false)));
 #pragma unroll
                         for(int m = 0; m < MT; ++m)
-                        {
-                            mma16<M>(acc[m][e], pa[m][j][0], pa[m][j][1], pa[m][j][2],
-                                    pa[m][j][3], vb[0], vb[1]);
-                            mma16<M>(acc[m][e + 1], pa[m][j][0], pa[m][j][1], pa[m][j][2],
-                                    pa[m][j][3], vb[2], vb[3]);
-                        }
+#pragma unroll
+                            for(int part = 0; part < 2; ++part)
+                                mma16<M>(acc[m][i], va[0], va[1], va[2], va[3],
+                                        pb[m][j][part][0], pb[m][j][part][1]);
                     }
                 }
                 else
@@ -1009,25 +1035,21 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                             for(int pair = 0; pair < 2; ++pair)
                             {
-                                // codes 2*pair, 2*pair + 1 of the word, positions 2t and 2t + 1
+                                // codes 2*pair and 2*pair + 1 of the word, positions 2t, 2t + 1
                                 const uint32_t sel = pair ? 0x7362u : 0x5140u;
                                 const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], sel);
                                 const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], sel);
+                                const uint32_t a0 = e4m3x2_to_half2(lo & 0xFFFFu);
+                                const uint32_t a1 = e4m3x2_to_half2(lo >> 16);
+                                const uint32_t a2 = e4m3x2_to_half2(hi & 0xFFFFu);
+                                const uint32_t a3 = e4m3x2_to_half2(hi >> 16);
+                                const int i = 8*q4 + 2*w + pair;
 #pragma unroll
-                                for(int odd = 0; odd < 2; ++odd)
-                                {
-                                    const int e = 16*q4 + 4*w + 2*pair + odd;
-                                    const uint32_t b0 = e4m3x2_to_half2(odd ? lo >> 16
-                                            : lo & 0xFFFFu);
-                                    const uint32_t b1 = e4m3x2_to_half2(odd ? hi >> 16
-                                            : hi & 0xFFFFu);
+                                for(int m = 0; m < MT; ++m)
 #pragma unroll
-                                    for(int m = 0; m < MT; ++m)
-                                    {
-                                        mma16<M>(acc[m][e], pa[m][j][0], pa[m][j][1],
-                                                pa[m][j][2], pa[m][j][3], b0, b1);
-                                    }
-                                }
+                                    for(int part = 0; part < 2; ++part)
+                                        mma16<M>(acc[m][i], a0, a1, a2, a3, pb[m][j][part][0],
+                                                pb[m][j][part][1]);
                             }
                     }
                 }
@@ -1056,77 +1078,107 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
         for(int m = 0; m < MT; ++m)
         {
-            sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
-            sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
-            float o[NBLK][2];
 #pragma unroll
-            for(int e = 0; e < NBLK; ++e)
-            {
-                o[e][0] = (acc[m][e][0] + acc[m][e][2])*drop*vscale;
-                o[e][1] = (acc[m][e][1] + acc[m][e][3])*drop*vscale;
-            }
+            for(int y = 0; y < 2; ++y)
+#pragma unroll
+                for(int o = 4; o < 32; o <<= 1)
+                {
+                    sum[m][y] += __shfl_xor_sync(0xffffffffu, sum[m][y], o);
+                }
+#pragma unroll
+            for(int i = 0; i < MBLK; ++i)
+#pragma unroll
+                for(int r = 0; r < 4; ++r)
+                    acc[m][i][r] = acc[m][i][r]*drop*vscale;
             if(wpw > 1)
             {
-                if(t == 0)
+                if(n == 0)
                 {
-                    top_s[warp][n] = top[m];
-                    sum_s[warp][n] = sum[m];
+#pragma unroll
+                    for(int y = 0; y < 2; ++y)
+                    {
+                        top_s[warp][2*t + y] = top[m][y];
+                        sum_s[warp][2*t + y] = sum[m][y];
+                    }
                 }
                 float *mw = merge + warp*8*DP;
 #pragma unroll
-                for(int e = 0; e < NBLK; ++e)
-                {
-                    mw[(2*e)*32 + lane] = o[e][0];
-                    mw[(2*e + 1)*32 + lane] = o[e][1];
-                }
+                for(int i = 0; i < MBLK; ++i)
+#pragma unroll
+                    for(int r = 0; r < 4; ++r)
+                        mw[(4*i + r)*32 + lane] = acc[m][i][r];
                 __syncthreads();
-                // every warp joins NBLK/WARPS blocks of the columns, same lanes, same heads
-                float big = -CUDART_INF_F;
+                // every warp joins its share of the blocks, same lanes, same heads
+                float big[2], den[2], wgt[WARPS][2];
 #pragma unroll
-                for(int w = 0; w < WARPS; ++w)
+                for(int y = 0; y < 2; ++y)
                 {
-                    big = fmaxf(big, top_s[w][n]);
-                }
-                const float ref = big == -CUDART_INF_F ? 0.0f : big;
-                float den = 0.0f, wgt[WARPS];
-#pragma unroll
-                for(int w = 0; w < WARPS; ++w)
-                {
-                    wgt[w] = ex2(top_s[w][n] - ref);
-                    den = fmaf(wgt[w], sum_s[w][n], den);
-                }
-                constexpr int MY = NBLK/WARPS;
-#pragma unroll
-                for(int i = 0; i < MY; ++i)
-                {
-                    const int e = warp*MY + i;
-                    float z0 = 0.0f, z1 = 0.0f;
+                    big[y] = -CUDART_INF_F;
+                    den[y] = 0.0f;
 #pragma unroll
                     for(int w = 0; w < WARPS; ++w)
                     {
-                        z0 = fmaf(wgt[w], merge[w*8*DP + (2*e)*32 + lane], z0);
-                        z1 = fmaf(wgt[w], merge[w*8*DP + (2*e + 1)*32 + lane], z1);
+                        big[y] = fmaxf(big[y], top_s[w][2*t + y]);
                     }
-                    write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, e, z0, z1, den, kvh,
-                            h0, heads, b);
+                    const float ref = big[y] == -CUDART_INF_F ? 0.0f : big[y];
+#pragma unroll
+                    for(int w = 0; w < WARPS; ++w)
+                    {
+                        wgt[w][y] = ex2(top_s[w][2*t + y] - ref);
+                        den[y] = fmaf(wgt[w][y], sum_s[w][2*t + y], den[y]);
+                    }
                 }
-                if(warp == 0 && t == 0)
+                // fewer blocks than warps (64 columns): the upper warps have none
+                constexpr int MY = (MBLK + WARPS - 1)/WARPS;
+#pragma unroll
+                for(int k = 0; k < MY; ++k)
                 {
-                    write_sums<MT>(a, complete, part, m, n, big, den, kvh, h0, heads, b);
+                    const int i = warp*MY + k;
+                    if(i < MBLK)
+                    {
+                        float z[4];
+#pragma unroll
+                        for(int r = 0; r < 4; ++r)
+                        {
+                            z[r] = 0.0f;
+#pragma unroll
+                            for(int w = 0; w < WARPS; ++w)
+                            {
+                                z[r] = fmaf(wgt[w][r & 1], merge[w*8*DP + (4*i + r)*32 + lane],
+                                        z[r]);
+                            }
+                        }
+                        write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, i, z, den, kvh,
+                                h0, heads, b);
+                    }
+                }
+                if(warp == 0 && n == 0)
+                {
+#pragma unroll
+                    for(int y = 0; y < 2; ++y)
+                    {
+                        write_sums<MT>(a, complete, part, m, 2*t + y, big[y], den[y], kvh, h0,
+                                heads, b);
+                    }
                 }
                 __syncthreads();
             }
             else
             {
 #pragma unroll
-                for(int e = 0; e < NBLK; ++e)
+                for(int i = 0; i < MBLK; ++i)
                 {
-                    write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, e, o[e][0], o[e][1],
-                            sum[m], kvh, h0, heads, b);
+                    write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, i, acc[m][i], sum[m],
+                            kvh, h0, heads, b);
                 }
-                if(t == 0)
+                if(n == 0)
                 {
-                    write_sums<MT>(a, complete, part, m, n, top[m], sum[m], kvh, h0, heads, b);
+#pragma unroll
+                    for(int y = 0; y < 2; ++y)
+                    {
+                        write_sums<MT>(a, complete, part, m, 2*t + y, top[m][y], sum[m][y], kvh,
+                                h0, heads, b);
+                    }
                 }
             }
         }
@@ -1148,8 +1200,8 @@ paged_decode_kernel(const PagedDecodeArgs a)
 }
 
 // Joins the parts of the units that fell into several shares, and answers those with
-// nothing to attend to.  A piece is 128 of the 8*DP values of 8 heads, four a lane, all of
-// head lane % 8; `wpp` warps share the parts of a piece and meet in shared memory: one warp
+// nothing to attend to.  A piece is 128 of the 8*DP values of 8 heads, four neighbouring
+// columns a lane; `wpp` warps share the parts of a piece and meet in shared memory: one warp
 // while units are many and their parts few, eight when a few units have many parts each.
 constexpr int PD_JOIN_WARPS = 8;
 
@@ -1200,6 +1252,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     const int x0 = before + hu*nt;
     const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
     const int m = piece*128/(8*DP), off = piece*128 - m*8*DP + 4*lane;   // in the part's values
+    const int head = off/DP, col = off - head*DP;
     // before any return: the block's end must not come before the first kernel's
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // one worker had it all and wrote it, or (the last block) there is no such unit
@@ -1214,7 +1267,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
         for(int i = warp % wpp; i < parts; i += wpp)
         {
             const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
-            const float2 ts = a.part_sums[(p*MT + m)*8 + (lane & 7)];
+            const float2 ts = a.part_sums[(p*MT + m)*8 + head];
             const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (p*MT + m)*8*DP + off);
             join_add(s, ts.x, ts.y, o);
         }
@@ -1238,25 +1291,21 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     {
         return;
     }
-    // values off .. off + 3: accumulator register off/32, lanes off%32 .. + 3, which are the
-    // four quads of head n's two columns each
-    const int n = lane & 7, reg = off >> 5;
-    const int kvh = hu/htiles, h0 = (hu - kvh*htiles)*8*MT, g = 8*m + n;
-    if(h0 + g < a.group)
+    const int kvh = hu/htiles, g = (hu - kvh*htiles)*8*MT + 8*m + head;
+    if(g < a.group)
     {
-        const size_t qh = ((size_t)kvh*a.group + h0 + g)*a.batch + b;
+        const size_t qh = ((size_t)kvh*a.group + g)*a.batch + b;
         const float inv = s.sum == 0.0f ? 0.0f : 1.0f/s.sum;
         const float v[4] = {s.o.x, s.o.y, s.o.z, s.o.w};
 #pragma unroll
-        for(int t = 0; t < 4; ++t)
+        for(int i = 0; i < 4; ++i)
         {
-            const int col = L::column(reg >> 1, 2*t + (reg & 1));
-            if(col < a.head)
+            if(col + i < a.head)
             {
-                ((T *)a.out)[qh*a.head + col] = from_f<T>(v[t]*inv);
+                ((T *)a.out)[qh*a.head + col + i] = from_f<T>(v[i]*inv);
             }
         }
-        if(a.lse_out && reg == 0)
+        if(a.lse_out && col == 0)
         {
             a.lse_out[qh] = s.sum == 0.0f ? -CUDART_INF_F
                     : ((s.top == -CUDART_INF_F ? 0.0f : s.top) + log2f(s.sum))*PD_LN2;
