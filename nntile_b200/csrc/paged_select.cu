@@ -59,37 +59,28 @@ struct PagedSelectArgs
     uint32_t *status;
 };
 
-// The exact key of a block, by a whole warp (same value in every lane).
+// The exact key of a block for query head g, by a whole warp (same value in every lane).
 template<typename T>
 __device__ __forceinline__ unsigned long long exact_key(const PagedSelectArgs &a, int kvh, int b,
-        int page, int lane)
+        int page, int g, int lane)
 {
     const T *low = (const T *)a.bounds + ((size_t)page*a.kv_heads + kvh)*2*a.head;
     const T *high = low + a.head;
-    unsigned long long best = 0ull;
-    for(int g = 0; g < a.group; ++g)
+    const T *q = (const T *)a.q + (((size_t)kvh*a.group + g)*a.batch + b)*a.head;
+    double s = 0.0;
+#pragma unroll 4
+    for(int h = lane; h < a.head; h += 32)
     {
-        const T *q = (const T *)a.q + (((size_t)kvh*a.group + g)*a.batch + b)*a.head;
-        double s = 0.0;
-        for(int h = lane; h < a.head; h += 32)
-        {
-            const double x = (double)to_f(q[h]);
-            s += (x > 0.0 ? x : 0.0)*(double)to_f(high[h])
-                    + (x < 0.0 ? x : 0.0)*(double)to_f(low[h]);
-            if(x != x)
-            {
-                s = x;
-            }
-        }
-#pragma unroll
-        for(int o = 16; o > 0; o >>= 1)
-        {
-            s += __shfl_xor_sync(0xffffffffu, s, o);
-        }
-        const unsigned long long key = score_key(s);
-        best = key > best ? key : best;
+        const double x = (double)to_f(q[h]);
+        s += x != x ? x : (x > 0.0 ? x : 0.0)*(double)to_f(high[h])
+                + (x < 0.0 ? x : 0.0)*(double)to_f(low[h]);
     }
-    return best;
+#pragma unroll
+    for(int o = 16; o > 0; o >>= 1)
+    {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+    return score_key(s);
 }
 
 __device__ __forceinline__ int filled_blocks(const PagedSelectArgs &a, int b, uint32_t *status)
@@ -117,7 +108,12 @@ paged_score_generic_kernel(const PagedSelectArgs a)
     float s = -CUDART_INF_F, error = 0.0f;
     if(page >= 0)
     {
-        const unsigned long long key = exact_key<T>(a, kvh, b, page, lane);
+        unsigned long long key = 0ull;
+        for(int g = 0; g < a.group; ++g)
+        {
+            const unsigned long long one = exact_key<T>(a, kvh, b, page, g, lane);
+            key = one > key ? one : key;
+        }
         const double exact = __longlong_as_double((long long)((key >> 63)
                 ? key & 0x7FFFFFFFFFFFFFFFull : ~key));
         s = key == ~0ull ? CUDART_NAN_F : (float)exact;
@@ -179,22 +175,26 @@ template<> __device__ __forceinline__ uint32_t negative2<__half>(uint32_t w)
     return r;
 }
 
-// Layout of the scoring kernel: a tile is 8 blocks of a unit, whose bounds (kmin, then kmax:
+// Layout of the scoring kernel: a tile is 16 blocks of a unit, whose bounds (kmin, then kmax:
 // 4*head contiguous bytes each) a warp copies into its private ring in shared memory and
 // consumes itself; every warp of the grid takes the same number of neighbouring tiles.  The
-// order of the head elements is free in a sum, so a lane's 16-byte piece t + 4j of a row is
-// the operand of two steps of the tensor instruction as it lies in memory.
+// blocks are the 16 rows of the tensor instruction, 8 query heads its columns.  The order of
+// the head elements is free in a sum, so a lane's 16-byte piece t + 4j of a row is the operand
+// of two steps as it lies in memory.
 constexpr int SCORE_WARPS = 8;
+constexpr int SCORE_TILE = 16;
 constexpr int SCORE_SMS = 148;
 
 template<int DP>
 struct ScoreTile
 {
     static constexpr int HALF = DP/8;                    // 16-byte pieces of kmin, of kmax
-    static constexpr int STAGE = 8*2*HALF*16;
-    static constexpr int STAGES = 24576/STAGE < 8 ? 24576/STAGE : 8;
-    static constexpr int SMEM = SCORE_WARPS*STAGES*STAGE;
-    static constexpr int PASSES = 8*2*HALF/32;           // copies a lane issues a tile
+    static constexpr int STAGE = SCORE_TILE*2*HALF*16;
+    static constexpr int WARPS = DP == 256 ? 4 : SCORE_WARPS;
+    static constexpr int RING = 196608/WARPS;
+    static constexpr int STAGES = RING/STAGE < 8 ? RING/STAGE : 8;
+    static constexpr int SMEM = WARPS*STAGES*STAGE;
+    static constexpr int PASSES = SCORE_TILE*2*HALF/32;  // copies a lane issues a tile
     // the lanes that read together hold 4 pieces of 2 neighbouring rows: different banks
     static __device__ __forceinline__ int offset(int r, int c)
     {
@@ -206,15 +206,16 @@ struct ScoreTile
 __device__ __forceinline__ int score_tiles(const PagedSelectArgs &a, int b, uint32_t *status)
 {
     const int blocks = filled_blocks(a, b, status);
-    return blocks > a.num_selected ? (blocks + 7)/8 : 0;  // otherwise all of them are taken
+    // otherwise all of them are taken
+    return blocks > a.num_selected ? (blocks + SCORE_TILE - 1)/SCORE_TILE : 0;
 }
 
 template<typename T, int DP, bool WIDE>
-__global__ void __launch_bounds__(SCORE_WARPS*32, 1)
+__global__ void __launch_bounds__(ScoreTile<DP>::WARPS*32, 1)
 paged_score_kernel(const PagedSelectArgs a)
 {
     using L = ScoreTile<DP>;
-    constexpr int JN = DP/32, STAGES = L::STAGES, ROWS = WIDE ? 16 : 8, MT = WIDE ? 2 : 1;
+    constexpr int JN = DP/32, STAGES = L::STAGES, MT = WIDE ? 2 : 1;
     extern __shared__ __align__(128) uint8_t score_smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -235,7 +236,7 @@ paged_score_kernel(const PagedSelectArgs a)
                 blockIdx.x == 0 && warp == 0 ? a.status : nullptr)*a.kv_heads : 0;
     }
     total = __reduce_add_sync(0xffffffffu, total);
-    const int workers = gridDim.x*SCORE_WARPS, worker = blockIdx.x*SCORE_WARPS + warp;
+    const int workers = gridDim.x*L::WARPS, worker = blockIdx.x*L::WARPS + warp;
     const int share = (total + workers - 1)/workers;
     const int begin = (int)min((long long)total, (long long)worker*share);
     int left = min(share, total - begin);
@@ -269,8 +270,8 @@ paged_score_kernel(const PagedSelectArgs a)
     // ---- issuing side
     int ib = b, ix = begin - seq_begin, ileft = left;
     int icount = filled_blocks(a, ib, nullptr), int_ = score_tiles(a, ib, nullptr);
-    int ipos = 4;
-    long long look_row = -1;
+    int ipos = 2;
+    long long look_at = -1;
     auto issue = [&](int stage)
     {
         if(ileft > 0)
@@ -284,22 +285,23 @@ paged_score_kernel(const PagedSelectArgs a)
                     int_ = score_tiles(a, ib, nullptr);
                 }
                 icount = filled_blocks(a, ib, nullptr);
-                ipos = 4;
+                ipos = 2;
             }
-            if(ipos == 4)
+            if(ipos == 2)
             {
-                // pages of the next 32 blocks: four tiles, which may be of several units
+                // bounds of the next 32 blocks: two tiles, which may be of two units
                 ipos = 0;
-                look_row = -1;
-                const long long x = ix + (long long)(lane >> 3);
-                if(x < (long long)int_*a.kv_heads && (lane >> 3) < ileft)
+                look_at = -1;
+                const long long x = ix + (long long)(lane >> 4);
+                if(x < (long long)int_*a.kv_heads && (lane >> 4) < ileft)
                 {
-                    const int kvh = (int)x/int_, block = ((int)x - kvh*int_)*8 + (lane & 7);
+                    const int kvh = (int)x/int_;
+                    const int block = ((int)x - kvh*int_)*SCORE_TILE + (lane & 15);
                     if(block < icount)
                     {
                         const int page = checked_page(a.block_table + (size_t)ib*a.max_blocks,
                                 block, a.num_pages, a.status);
-                        look_row = page < 0 ? -1 : (long long)page*a.kv_heads + kvh;
+                        look_at = page < 0 ? -1 : ((long long)page*a.kv_heads + kvh)*4*a.head;
                     }
                 }
             }
@@ -308,11 +310,11 @@ paged_score_kernel(const PagedSelectArgs a)
             for(int i = 0; i < L::PASSES; ++i)
             {
                 const int at = i*32 + lane, r = at/(2*L::HALF), c = at % (2*L::HALF);
-                const long long row = __shfl_sync(0xffffffffu, look_row, 8*ipos + r);
+                const long long from = __shfl_sync(0xffffffffu, look_at, 16*ipos + r);
                 const int piece = c % L::HALF;
-                if(row >= 0 && piece < chunks)
+                if(from >= 0 && piece < chunks)
                 {
-                    const uint8_t *src = (const uint8_t *)a.bounds + row*4*a.head
+                    const uint8_t *src = (const uint8_t *)a.bounds + from
                             + (piece + (c < L::HALF ? 0 : chunks))*16;
                     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;"
                             :: "r"(dst + L::offset(r, c)), "l"(src) : "memory");
@@ -334,7 +336,7 @@ paged_score_kernel(const PagedSelectArgs a)
     int nt = score_tiles(a, b, nullptr), count = filled_blocks(a, b, nullptr);
     int kvh = (begin - seq_begin)/nt, tile = (begin - seq_begin) - kvh*nt;
     bool fresh = true;
-    uint32_t q[MT][JN][4];
+    uint32_t qp[MT][JN][4], qm[MT][JN][4];       // positive and negative parts of head 8m + n
     int stage = 0;
     while(left-- > 0)
     {
@@ -343,10 +345,11 @@ paged_score_kernel(const PagedSelectArgs a)
         issue(stage == 0 ? STAGES - 1 : stage - 1);
         const uint8_t *st = ring + stage*L::STAGE;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
+        // of blocks n and n + 8, over this lane's heads
         float best[2] = {-CUDART_INF_F, -CUDART_INF_F}, error[2] = {0.0f, 0.0f};
-        for(int g0 = 0; g0 < a.group; g0 += ROWS)
+        for(int g0 = 0; g0 < a.group; g0 += 8*MT)
         {
-            if(fresh || a.group > ROWS)
+            if(fresh || a.group > 8*MT)
             {
 #pragma unroll
                 for(int m = 0; m < MT; ++m)
@@ -358,76 +361,84 @@ paged_score_kernel(const PagedSelectArgs a)
                                 ? *reinterpret_cast<const uint4 *>((const T *)a.q
                                         + (((size_t)kvh*a.group + g)*a.batch + b)*a.head + h)
                                 : make_uint4(0u, 0u, 0u, 0u);
-                        q[m][j][0] = v.x;
-                        q[m][j][1] = v.y;
-                        q[m][j][2] = v.z;
-                        q[m][j][3] = v.w;
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for(int i = 0; i < 4; ++i)
+                        {
+                            qp[m][j][i] = positive2<T>(w[i]);
+                            qm[m][j][i] = negative2<T>(w[i]);
+                        }
                     }
                 fresh = false;
             }
-            // scores (s, less) and sums of magnitudes (up, down; down is negative) by the
-            // positive and the negative part of q: four chains of products
-            float s[4] = {}, less[4] = {}, up[4] = {}, down[4] = {};
+            // scores by the two parts of q (s, less) and their sums of magnitudes (up, down;
+            // down is negative): four chains of products
+            float s[MT][4] = {}, less[MT][4] = {}, up[MT][4] = {}, down[MT][4] = {};
 #pragma unroll
             for(int j = 0; j < JN; ++j)
             {
-                const uint4 lo = *reinterpret_cast<const uint4 *>(st + L::offset(n, t + 4*j));
-                const uint4 hi = *reinterpret_cast<const uint4 *>(st
-                        + L::offset(n, L::HALF + t + 4*j));
-#pragma unroll
-                for(int w = 0; w < 4; w += 2)
-                {
-                    const uint32_t l0 = w ? lo.z : lo.x, l1 = w ? lo.w : lo.y;
-                    const uint32_t h0 = w ? hi.z : hi.x, h1 = w ? hi.w : hi.y;
-                    const uint32_t p0 = positive2<T>(q[0][j][w]);
-                    const uint32_t p2 = positive2<T>(q[0][j][w + 1]);
-                    const uint32_t m0 = negative2<T>(q[0][j][w]);
-                    const uint32_t m2 = negative2<T>(q[0][j][w + 1]);
-                    const uint32_t p1 = WIDE ? positive2<T>(q[MT - 1][j][w]) : 0u;
-                    const uint32_t p3 = WIDE ? positive2<T>(q[MT - 1][j][w + 1]) : 0u;
-                    const uint32_t m1 = WIDE ? negative2<T>(q[MT - 1][j][w]) : 0u;
-                    const uint32_t m3 = WIDE ? negative2<T>(q[MT - 1][j][w + 1]) : 0u;
-                    score_mma<T>(s, p0, p1, p2, p3, h0, h1);
-                    score_mma<T>(up, p0, p1, p2, p3, h0 & 0x7FFF7FFFu, h1 & 0x7FFF7FFFu);
-                    score_mma<T>(less, m0, m1, m2, m3, l0, l1);
-                    score_mma<T>(down, m0, m1, m2, m3, l0 & 0x7FFF7FFFu, l1 & 0x7FFF7FFFu);
-                }
-            }
-#pragma unroll
-            for(int m = 0; m < MT; ++m)
+                uint4 lo[2], hi[2];
 #pragma unroll
                 for(int x = 0; x < 2; ++x)
                 {
-                    if(g0 + 8*m + n < a.group)
+                    lo[x] = *reinterpret_cast<const uint4 *>(st + L::offset(n + 8*x, t + 4*j));
+                    hi[x] = *reinterpret_cast<const uint4 *>(st
+                            + L::offset(n + 8*x, L::HALF + t + 4*j));
+                }
+#pragma unroll
+                for(int w = 0; w < 4; w += 2)
+                {
+                    const uint32_t l0 = w ? lo[0].z : lo[0].x, l2 = w ? lo[0].w : lo[0].y;
+                    const uint32_t l1 = w ? lo[1].z : lo[1].x, l3 = w ? lo[1].w : lo[1].y;
+                    const uint32_t h0 = w ? hi[0].z : hi[0].x, h2 = w ? hi[0].w : hi[0].y;
+                    const uint32_t h1 = w ? hi[1].z : hi[1].x, h3 = w ? hi[1].w : hi[1].y;
+                    constexpr uint32_t ABS = 0x7FFF7FFFu;
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
                     {
-                        best[x] = max_nan(best[x], s[2*m + x] + less[2*m + x]);
-                        error[x] = max_nan(error[x], up[2*m + x] - down[2*m + x]);
+                        score_mma<T>(s[m], h0, h1, h2, h3, qp[m][j][w], qp[m][j][w + 1]);
+                        score_mma<T>(less[m], l0, l1, l2, l3, qm[m][j][w], qm[m][j][w + 1]);
+                        score_mma<T>(up[m], h0 & ABS, h1 & ABS, h2 & ABS, h3 & ABS,
+                                qp[m][j][w], qp[m][j][w + 1]);
+                        score_mma<T>(down[m], l0 & ABS, l1 & ABS, l2 & ABS, l3 & ABS,
+                                qm[m][j][w], qm[m][j][w + 1]);
+                    }
+                }
+            }
+            // value r: block n + 8*(r >> 1), head g0 + 8m + 2t + (r & 1)
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+#pragma unroll
+                for(int r = 0; r < 4; ++r)
+                {
+                    if(g0 + 8*m + 2*t + (r & 1) < a.group)
+                    {
+                        best[r >> 1] = max_nan(best[r >> 1], s[m][r] + less[m][r]);
+                        error[r >> 1] = max_nan(error[r >> 1], up[m][r] - down[m][r]);
                     }
                 }
         }
 #pragma unroll
-        for(int o = 4; o < 32; o <<= 1)
+        for(int x = 0; x < 2; ++x)
         {
 #pragma unroll
-            for(int x = 0; x < 2; ++x)
+            for(int o = 1; o < 4; o <<= 1)
             {
                 best[x] = max_nan(best[x], __shfl_xor_sync(0xffffffffu, best[x], o));
                 error[x] = max_nan(error[x], __shfl_xor_sync(0xffffffffu, error[x], o));
             }
         }
-        const int block = tile*8 + 2*t;
-        float2 *out = a.scores + ((size_t)kvh*a.batch + b)*a.max_blocks + block;
-#pragma unroll
-        for(int x = 0; x < 2; ++x)
+        // lanes t = 0, 1 write blocks n and n + 8
+        const int block = tile*SCORE_TILE + n + 8*t;
+        if(t < 2 && block < count)
         {
             // the copying side has reported a missing page; its score is the lowest
-            if(n == 0 && block + x < count)
-            {
-                const bool gone = !page_in_pool(a.block_table[(size_t)b*a.max_blocks + block + x],
-                        a.num_pages);
-                out[x] = gone ? make_float2(-CUDART_INF_F, 0.0f)
-                        : make_float2(best[x], error[x]*SCORE_ERROR + SCORE_FLOOR);
-            }
+            const bool gone = !page_in_pool(a.block_table[(size_t)b*a.max_blocks + block],
+                    a.num_pages);
+            a.scores[((size_t)kvh*a.batch + b)*a.max_blocks + block] = gone
+                    ? make_float2(-CUDART_INF_F, 0.0f)
+                    : make_float2(t ? best[1] : best[0],
+                            (t ? error[1] : error[0])*SCORE_ERROR + SCORE_FLOOR);
         }
         if(++tile == nt)
         {
@@ -481,7 +492,9 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ float fred[PICK_WARPS];
     __shared__ int listed_s, list_s[PICK_LIST];
     __shared__ unsigned long long list_key_s[PICK_LIST], cut_s;
-    __shared__ int equal_want_s, bin_s[256], hit_s, hits_s, rank_s;
+    __shared__ int equal_want_s, bin_s[256];
+    __shared__ float list_score_s[PICK_LIST], last_s;
+    __shared__ uint2 mask_s[PICK_THREADS];
     __shared__ uint32_t low_s, high_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int unit = blockIdx.x, b = unit % a.batch, kvh = unit/a.batch;
@@ -504,6 +517,7 @@ paged_pick_kernel(const PagedSelectArgs a)
 
     auto score = [&](int i) { return CACHED ? cached_s[i] : scores[i].x; };
     float error = 0.0f, low = CUDART_INF_F, high = -CUDART_INF_F;
+#pragma unroll 4
     for(int i = begin + tid; i < end; i += PICK_THREADS)
     {
         const float2 se = scores[i];
@@ -522,6 +536,14 @@ paged_pick_kernel(const PagedSelectArgs a)
         low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
+    for(int i = tid; i < 256; i += PICK_THREADS)
+    {
+        bin_s[i] = 0;
+    }
+    if(tid == 0)
+    {
+        listed_s = 0;
+    }
     if(lane == 0)
     {
         fred[warp] = error;
@@ -529,6 +551,7 @@ paged_pick_kernel(const PagedSelectArgs a)
         red2[warp] = __float_as_int(high);
     }
     __syncthreads();
+#pragma unroll
     for(int w = 0; w < PICK_WARPS; ++w)
     {
         error = max_nan(error, fred[w]);
@@ -540,28 +563,19 @@ paged_pick_kernel(const PagedSelectArgs a)
     float sure_in = CUDART_INF_F, sure_out = -CUDART_INF_F;
     if(want > 0 && !unsure)
     {
-        // The want-th highest score: count the scores in 256 equal bins of the range that holds
-        // it, go on with the bin it lies in; two or three rounds leave a single score, or a
-        // threshold that exactly the wanted number reaches.  Missing pages (-inf) go into the
-        // lowest bin.
+        // The want-th highest score: count the scores in 256 equal bins of their range; the bin
+        // it lies in holds a few, which are ranked against one another - or, when they are
+        // more than the list, are the range of another round.  Missing pages (-inf) go into
+        // the lowest bin.
         int rank = want;                         // from the top of [low, high]
         low = fmaxf(low, -FLT_MAX);
         high = fmaxf(high, -FLT_MAX);
         while(low < high)
         {
-            for(int i = tid; i < 256; i += PICK_THREADS)
-            {
-                bin_s[i] = 0;
-            }
-            if(tid == 0)
-            {
-                low_s = ~0u;
-                high_s = 0u;
-            }
-            __syncthreads();
             // halves: the range of finite numbers may itself not be one
             const float origin = 0.5f*low, scale = 256.0f/(0.5f*high - origin);
             auto bin = [&](float s) { return min(255, (int)((0.5f*s - origin)*scale)); };
+#pragma unroll 4
             for(int i = begin + tid; i < end; i += PICK_THREADS)
             {
                 const float s = fmaxf(score(i), -FLT_MAX);
@@ -571,43 +585,79 @@ paged_pick_kernel(const PagedSelectArgs a)
                 }
             }
             __syncthreads();
-            if(warp == 0)
+            // every warp finds the bin: lane 0 has the top eight
+            int c[8], sum = 0;
+#pragma unroll
+            for(int k = 0; k < 8; ++k)
             {
-                // lane 0 has the top eight bins
-                int c[8], sum = 0;
+                c[k] = bin_s[255 - 8*lane - k];
+                sum += c[k];
+            }
+            int scan = sum;
 #pragma unroll
-                for(int k = 0; k < 8; ++k)
+            for(int o = 1; o < 32; o <<= 1)
+            {
+                const int up = __shfl_up_sync(0xffffffffu, scan, o);
+                scan += lane >= o ? up : 0;
+            }
+            int above = scan - sum, hit = 0, hits = 0, left = 0;
+            const bool here = above < rank && scan >= rank;
+#pragma unroll
+            for(int k = 0; k < 8; ++k)
+            {
+                if(above < rank && above + c[k] >= rank)
                 {
-                    c[k] = bin_s[255 - 8*lane - k];
-                    sum += c[k];
+                    hit = 255 - 8*lane - k;
+                    left = rank - above;
+                    hits = c[k];
                 }
-                int scan = sum;
-#pragma unroll
-                for(int o = 1; o < 32; o <<= 1)
+                above += c[k];
+            }
+            const int from = __ffs((int)__ballot_sync(0xffffffffu, here)) - 1;
+            hit = __shfl_sync(0xffffffffu, hit, from);
+            hits = __shfl_sync(0xffffffffu, hits, from);
+            rank = __shfl_sync(0xffffffffu, left, from);
+            if(hits <= PICK_LIST)
+            {
+#pragma unroll 4
+                for(int i = begin + tid; i < end; i += PICK_THREADS)
                 {
-                    const int up = __shfl_up_sync(0xffffffffu, scan, o);
-                    scan += lane >= o ? up : 0;
-                }
-                int above = scan - sum;
-                if(above < rank && scan >= rank)
-                {
-#pragma unroll
-                    for(int k = 0; k < 8; ++k)
+                    const float s = fmaxf(score(i), -FLT_MAX);
+                    if(s >= low && s <= high && bin(s) == hit)
                     {
-                        if(above < rank && above + c[k] >= rank)
-                        {
-                            hit_s = 255 - 8*lane - k;
-                            rank_s = rank - above;
-                            hits_s = c[k];
-                        }
-                        above += c[k];
+                        list_score_s[atomicAdd(&listed_s, 1)] = s;
                     }
                 }
+                __syncthreads();
+                for(int k = tid; k < hits; k += PICK_THREADS)
+                {
+                    const float s = list_score_s[k];
+                    int over = 0, same = 0;
+                    for(int j = 0; j < hits; ++j)
+                    {
+                        over += list_score_s[j] > s ? 1 : 0;
+                        same += list_score_s[j] == s ? 1 : 0;
+                    }
+                    if(over < rank && over + same >= rank)
+                    {
+                        last_s = s;              // the same value from every equal
+                    }
+                }
+                __syncthreads();
+                low = high = last_s;
+                break;
+            }
+            // the range of the scores in that bin
+            if(tid == 0)
+            {
+                low_s = ~0u;
+                high_s = 0u;
             }
             __syncthreads();
-            const int hit = hit_s, hits = hits_s;
-            rank = rank_s;
-            // the scores in that bin
+            for(int i = tid; i < 256; i += PICK_THREADS)
+            {
+                bin_s[i] = 0;
+            }
             uint32_t least = ~0u, most = 0u;
             for(int i = begin + tid; i < end; i += PICK_THREADS)
             {
@@ -651,6 +701,7 @@ paged_pick_kernel(const PagedSelectArgs a)
         }
         __syncthreads();
         int in = 0, near = 0;
+#pragma unroll 4
         for(int i = begin + tid; i < end; i += PICK_THREADS)
         {
             const float s = score(i);
@@ -662,33 +713,53 @@ paged_pick_kernel(const PagedSelectArgs a)
                 if(at < PICK_LIST)
                 {
                     list_s[at] = i;
+                    list_key_s[at] = 0ull;
                 }
             }
         }
-        in = block_sum(in, red);
-        near = block_sum(near, red);
+        in = __reduce_add_sync(0xffffffffu, in);
+        if(lane == 0)
+        {
+            red[warp] = in;
+        }
+        __syncthreads();
+        near = listed_s;
+        in = 0;
+#pragma unroll
+        for(int w = 0; w < PICK_WARPS; ++w)
+        {
+            in += red[w];
+        }
         const int need = want - in;              // of the near ones
         take_near = need >= near;
         if(!take_near)
         {
+            // a warp per block and query head
             const bool listed = near <= PICK_LIST;
-            const int todo = listed ? near : end - begin;
-            for(int k = warp; k < todo; k += PICK_WARPS)
+            const long long todo = (long long)(listed ? near : end - begin)*a.group;
+            if(!listed)
             {
-                const int i = listed ? list_s[k] : begin + k;
+                for(int i = begin + tid; i < end; i += PICK_THREADS)
+                {
+                    keys[i] = 0ull;
+                }
+                __syncthreads();
+            }
+            for(long long k = warp; k < todo; k += PICK_WARPS)
+            {
+                const int c = (int)(k/a.group), g = (int)(k - (long long)c*a.group);
+                const int i = listed ? list_s[c] : begin + c;
                 if(!listed && !is_near(score(i)))
                 {
                     continue;
                 }
                 const int page = a.block_table[(size_t)b*a.max_blocks + i];
-                const unsigned long long key = page_in_pool(page, a.num_pages)
-                        ? exact_key<T>(a, kvh, b, page, lane) : 0ull;
-                if(lane == 0)
+                if(page_in_pool(page, a.num_pages))
                 {
-                    keys[i] = key;
-                    if(listed)
+                    const unsigned long long key = exact_key<T>(a, kvh, b, page, g, lane);
+                    if(lane == 0)
                     {
-                        list_key_s[k] = key;
+                        atomicMax(listed ? &list_key_s[c] : &keys[i], key);
                     }
                 }
             }
@@ -714,6 +785,10 @@ paged_pick_kernel(const PagedSelectArgs a)
                 __syncthreads();
                 cut = cut_s;
                 equal_want = equal_want_s;
+                for(int k = tid; k < near; k += PICK_THREADS)
+                {
+                    keys[list_s[k]] = list_key_s[k];
+                }
             }
             else
             {
@@ -742,9 +817,6 @@ paged_pick_kernel(const PagedSelectArgs a)
         }
         __syncthreads();
     }
-    // write in index order: a run of neighbours a thread, one scan over the threads
-    const int per = (n + PICK_THREADS - 1)/PICK_THREADS;
-    const int i0 = min(n, tid*per), i1 = min(n, i0 + per);
     auto state = [&](int i)                      // 2 taken, 1 equal to the cut, 0 left out
     {
         if(i < begin || i >= end) return 2;
@@ -756,46 +828,66 @@ paged_pick_kernel(const PagedSelectArgs a)
         const unsigned long long key = keys[i];
         return key > cut ? 2 : key == cut ? 1 : 0;
     };
-    int taken = 0, equal = 0;
-    for(int i = i0; i < i1; ++i)
+    // write in index order: 32 neighbours a warp as two masks, a thread per mask for the rest
+    int taken = 0, equals = 0;                   // of the runs before
+    for(int base = 0; base < n; base += 32*PICK_THREADS)
     {
-        const int st = state(i);
-        taken += st == 2 ? 1 : 0;
-        equal += st == 1 ? 1 : 0;
-    }
-    int scan_t = taken, scan_e = equal;
-#pragma unroll
-    for(int o = 1; o < 32; o <<= 1)
-    {
-        const int ut = __shfl_up_sync(0xffffffffu, scan_t, o);
-        const int ue = __shfl_up_sync(0xffffffffu, scan_e, o);
-        scan_t += lane >= o ? ut : 0;
-        scan_e += lane >= o ? ue : 0;
-    }
-    __syncthreads();
-    if(lane == 31)
-    {
-        red[warp] = scan_t;
-        red2[warp] = scan_e;
-    }
-    __syncthreads();
-    int before_t = scan_t - taken, before_e = scan_e - equal;
-    for(int w = 0; w < warp; ++w)
-    {
-        before_t += red[w];
-        before_e += red2[w];
-    }
-    for(int i = i0; i < i1; ++i)
-    {
-        const int st = state(i);
-        const bool take = st == 2 || (st == 1 && before_e < equal_want);
-        const int at = before_t + min(before_e, equal_want);
-        if(take && at < S)
+        __syncthreads();
+#pragma unroll 2
+        for(int k = warp; k < PICK_THREADS && base + 32*k < n; k += PICK_WARPS)
         {
-            out[at] = i;
+            const int i = base + 32*k + lane;
+            const int st = i < n ? state(i) : 0;
+            const unsigned take = __ballot_sync(0xffffffffu, st == 2);
+            const unsigned equal = __ballot_sync(0xffffffffu, st == 1);
+            if(lane == 0)
+            {
+                mask_s[k] = make_uint2(take, equal);
+            }
         }
-        before_t += st == 2 ? 1 : 0;
-        before_e += st == 1 ? 1 : 0;
+        __syncthreads();
+        uint2 mine = make_uint2(0u, 0u);
+        if(base + 32*tid < n)
+        {
+            mine = mask_s[tid];
+        }
+        const int ct = __popc(mine.x), ce = __popc(mine.y);
+        int scan_t = ct, scan_e = ce;
+#pragma unroll
+        for(int o = 1; o < 32; o <<= 1)
+        {
+            const int ut = __shfl_up_sync(0xffffffffu, scan_t, o);
+            const int ue = __shfl_up_sync(0xffffffffu, scan_e, o);
+            scan_t += lane >= o ? ut : 0;
+            scan_e += lane >= o ? ue : 0;
+        }
+        if(lane == 31)
+        {
+            red[warp] = scan_t;
+            red2[warp] = scan_e;
+        }
+        __syncthreads();
+        int before_t = taken + scan_t - ct, before_e = equals + scan_e - ce;
+#pragma unroll
+        for(int w = 0; w < PICK_WARPS; ++w)
+        {
+            before_t += w < warp ? red[w] : 0;
+            before_e += w < warp ? red2[w] : 0;
+            taken += red[w];
+            equals += red2[w];
+        }
+        for(unsigned any = mine.x | mine.y; any != 0u; any &= any - 1u)
+        {
+            const int k = __ffs((int)any) - 1;
+            const bool equal = (mine.y >> k & 1u) != 0u;
+            const int at = before_t + min(before_e, equal_want);
+            if((!equal || before_e < equal_want) && at < S)
+            {
+                out[at] = base + 32*tid + k;
+            }
+            before_t += equal ? 0 : 1;
+            before_e += equal ? 1 : 0;
+        }
     }
 }
 
@@ -817,16 +909,17 @@ static int launch_score_as(cudaStream_t s, const PagedSelectArgs &a, unsigned gr
     {
         return NNTILE_B200_E_LAUNCH;
     }
-    paged_score_kernel<T, DP, WIDE><<<grid, SCORE_WARPS*32, ScoreTile<DP>::SMEM, s>>>(a);
+    paged_score_kernel<T, DP, WIDE><<<grid, ScoreTile<DP>::WARPS*32, ScoreTile<DP>::SMEM, s>>>(a);
     return launch_status();
 }
 
 template<typename T, int DP>
 static int launch_score(cudaStream_t s, const PagedSelectArgs &a)
 {
-    const int64_t tiles = (int64_t)a.batch*a.kv_heads*((a.max_blocks + 7)/8);
-    const unsigned grid = (unsigned)std::min<int64_t>(SCORE_SMS,
-            (tiles + SCORE_WARPS - 1)/SCORE_WARPS);
+    constexpr int WARPS = ScoreTile<DP>::WARPS;
+    const int64_t tiles = (int64_t)a.batch*a.kv_heads
+            *((a.max_blocks + SCORE_TILE - 1)/SCORE_TILE);
+    const unsigned grid = (unsigned)std::min<int64_t>(SCORE_SMS, (tiles + WARPS - 1)/WARPS);
     return a.group > 8 ? launch_score_as<T, DP, true>(s, a, grid)
             : launch_score_as<T, DP, false>(s, a, grid);
 }
@@ -920,7 +1013,7 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.status = status;
     // 16-byte rows, and tiles that 30 bits can count
     const bool vec = head % 8 == 0 && aligned16(q) && aligned16(bounds)
-            && units*((max_blocks + 7)/8) < (int64_t)1 << 30;
+            && units*((max_blocks + SCORE_TILE - 1)/SCORE_TILE) < (int64_t)1 << 30;
     cudaStream_t s = as_stream(stream);
     int st2 = NNTILE_B200_OK;
     if(max_blocks > num_selected)                // otherwise everything is taken
