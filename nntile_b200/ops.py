@@ -10,6 +10,7 @@ dtype float32 selects the fp32 kernels, bfloat16 the bf16 ones.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -205,38 +206,50 @@ def decode_sdpa(head, max_seq, length, batch, group, kv_heads, q, Kcache, Vcache
 
 # ---- paged key/value cache --------------------------------------------------------
 # Unlike the rest of this module these calls run on the stream of the device that their
-# tensors are on, whichever device is current.
+# tensors are on, whichever device is current.  A decode step makes a few of them and its
+# kernels take microseconds, so they are written to cost the host little: entry points and
+# workspace sizes are looked up once.
 
-def _paged_call(name, dev, args):
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _call(name, torch.cuda.current_stream(dev).cuda_stream, *args)
+_paged_entries = {}
+
+
+def _paged_entry(name, dtype):
+    """(entry point, its name) for rows of `dtype`."""
+    found = _paged_entries.get((name, dtype))
+    if found is None:
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"paged caches take bfloat16 or float16 rows, not {dtype}")
+        full = f"nntile_b200_paged_{name}_{'bf16' if dtype == torch.bfloat16 else 'fp16'}"
+        found = _paged_entries[name, dtype] = getattr(_lib.load(), full), full
+    return found
+
+
+def _paged_call(entry, dev, args):
+    fn, name = entry
+    if dev == torch._C._cuda_getDevice():
+        st = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
     else:
-        _call(name, torch.cuda.current_stream(dev).cuda_stream, *args)
+        with torch.cuda.device(dev):
+            st = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    if st:
+        _lib.check(name, st)
 
 
 def _paged_ptrs(dev, *tensors):
     """Device addresses (None stays None) of contiguous tensors, all on device `dev`."""
     if dev < 0:
         raise ValueError("nntile_b200 ops need CUDA tensors (there is no CPU path)")
-    ptrs = []
     for t in tensors:
-        if t is None:
-            ptrs.append(None)
-            continue
-        if t.get_device() != dev:
-            raise ValueError("paged cache operations need CUDA tensors on one device")
-        if not t.is_contiguous():
-            raise ValueError("nntile_b200 ops need contiguous buffers")
-        ptrs.append(t.data_ptr())
-    return ptrs
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+            raise ValueError("paged cache operations need contiguous CUDA tensors on one device")
+    return [None if t is None else t.data_ptr() for t in tensors]
 
 
 def paged_kv_append(head, page_size, num_pages, max_blocks, batch, kv_heads, new_seq, page_format,
                     lengths, new_lens, block_table, k, v, k_pages, v_pages, k_scales, v_scales,
                     bounds, status):
     dev = k.get_device()
-    _paged_call(f"nntile_b200_paged_kv_append_{_sfx16(k)}", dev,
+    _paged_call(_paged_entry("kv_append", k.dtype), dev,
                 (head, page_size, num_pages, max_blocks, batch, kv_heads, new_seq, page_format,
                  *_paged_ptrs(dev, lengths, new_lens, block_table, k, v, k_pages, v_pages,
                               k_scales, v_scales, bounds, status)))
@@ -245,12 +258,13 @@ def paged_kv_append(head, page_size, num_pages, max_blocks, batch, kv_heads, new
 def paged_kv_gather(head, page_size, num_pages, max_blocks, batch, kv_heads, max_seq, page_format,
                     lengths, block_table, k_pages, v_pages, k_scales, v_scales, k, v, status):
     dev = k.get_device()
-    _paged_call(f"nntile_b200_paged_kv_gather_{_sfx16(k)}", dev,
+    _paged_call(_paged_entry("kv_gather", k.dtype), dev,
                 (head, page_size, num_pages, max_blocks, batch, kv_heads, max_seq, page_format,
                  *_paged_ptrs(dev, lengths, block_table, k_pages, v_pages, k_scales, v_scales,
                               k, v, status)))
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_decode_workspace_bytes(head, page_size, max_blocks, batch, group, kv_heads,
                                  num_selected=0) -> int:
     return int(_lib.load().nntile_b200_paged_decode_sdpa_workspace_bytes(
@@ -263,11 +277,12 @@ def paged_decode_sdpa(head, page_size, num_pages, max_blocks, batch, group, kv_h
     dev = q.get_device()
     ptrs = _paged_ptrs(dev, lengths, block_table, selected, q, k_pages, v_pages, k_scales,
                        v_scales, out, lse_out, workspace, status)
-    _paged_call(f"nntile_b200_paged_decode_sdpa_{_sfx16(q)}", dev,
+    _paged_call(_paged_entry("decode_sdpa", q.dtype), dev,
                 (head, page_size, num_pages, max_blocks, batch, group, kv_heads, num_selected,
-                 page_format, *ptrs[:-1], workspace.numel()*workspace.element_size(), ptrs[-1]))
+                 page_format, *ptrs[:-1], workspace.nbytes, ptrs[-1]))
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_select_workspace_bytes(max_blocks, batch, kv_heads) -> int:
     return int(_lib.load().nntile_b200_paged_select_workspace_bytes(max_blocks, batch, kv_heads))
 
@@ -277,7 +292,6 @@ def paged_select(head, page_size, num_pages, max_blocks, batch, group, kv_heads,
                  status):
     dev = q.get_device()
     ptrs = _paged_ptrs(dev, lengths, block_table, q, bounds, selected, workspace, status)
-    _paged_call(f"nntile_b200_paged_select_{_sfx16(q)}", dev,
+    _paged_call(_paged_entry("select", q.dtype), dev,
                 (head, page_size, num_pages, max_blocks, batch, group, kv_heads, num_selected,
-                 first_blocks, last_blocks, *ptrs[:-1],
-                 workspace.numel()*workspace.element_size(), ptrs[-1]))
+                 first_blocks, last_blocks, *ptrs[:-1], workspace.nbytes, ptrs[-1]))

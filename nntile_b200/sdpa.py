@@ -437,6 +437,9 @@ class KVCache:
         return self.k_cache_size
 
 
+_ROWS = (torch.bfloat16, torch.float16)
+
+
 class KVPages:
     """Buffers of a paged cache: what the paged_* functions read and write.
 
@@ -448,21 +451,22 @@ class KVPages:
     __slots__ = ("k", "v", "k_scales", "v_scales", "bounds", "e4m3")
 
     def __init__(self, k, v, k_scales=None, v_scales=None, bounds=None):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or shape != v.shape or dtype != v.dtype:
             raise ValueError("k and v pages must be two equal (num_pages, kv_heads, page_size, "
                              "head) buffers")
-        self.e4m3 = k.dtype not in (torch.bfloat16, torch.float16)
+        self.e4m3 = dtype not in _ROWS
         if self.e4m3:
-            if k.dtype not in (torch.uint8, torch.float8_e4m3fn):
-                raise TypeError(f"pages hold bfloat16, float16 or 8-bit codes, not {k.dtype}")
+            if dtype not in (torch.uint8, torch.float8_e4m3fn):
+                raise TypeError(f"pages hold bfloat16, float16 or 8-bit codes, not {dtype}")
             for s in (k_scales, v_scales):
-                if s is None or s.shape != k.shape[:3] or s.dtype != torch.uint8:
+                if s is None or s.shape != shape[:3] or s.dtype != torch.uint8:
                     raise ValueError("8-bit pages need uint8 scales (num_pages, kv_heads, "
                                      "page_size) for k and v")
         elif k_scales is not None or v_scales is not None:
             raise ValueError("only 8-bit pages have scales")
-        if bounds is not None and (bounds.shape != (k.shape[0], k.shape[1], 2, k.shape[3])
-                                   or (not self.e4m3 and bounds.dtype != k.dtype)):
+        if bounds is not None and (bounds.shape != (shape[0], shape[1], 2, shape[3])
+                                   or (not self.e4m3 and bounds.dtype != dtype)):
             raise ValueError("bounds must be (num_pages, kv_heads, 2, head) in the type of the rows")
         self.k, self.v, self.k_scales, self.v_scales, self.bounds = k, v, k_scales, v_scales, bounds
 
@@ -479,16 +483,19 @@ class KVPages:
         return cls(k, v, ks, vs, bd)
 
     def _check_rows(self, t, what):
-        if t.dtype not in (torch.bfloat16, torch.float16) \
-                or (not self.e4m3 and t.dtype != self.k.dtype):
-            raise TypeError(f"{what} is {t.dtype}, the pages hold {self.k.dtype}")
+        dtype = t.dtype
+        if dtype not in _ROWS or (not self.e4m3 and dtype != self.k.dtype):
+            raise TypeError(f"{what} is {dtype}, the pages hold {self.k.dtype}")
 
 
-def _check_table(pages, lengths, block_table, batch):
+def _check_table(lengths, block_table, batch):
+    """max_blocks of a table that fits."""
     if lengths.dtype != torch.int32 or block_table.dtype != torch.int32:
         raise TypeError("lengths and block_table must be int32")
-    if lengths.shape != (batch,) or block_table.dim() != 2 or block_table.shape[0] != batch:
+    shape = block_table.shape
+    if lengths.shape != (batch,) or len(shape) != 2 or shape[0] != batch:
         raise ValueError("lengths must be (batch,) and block_table (batch, max_blocks)")
+    return shape[1]
 
 
 def _check_status(status):
@@ -503,17 +510,18 @@ def paged_append(pages, lengths, block_table, k, v, new_lens=None, status=None):
     scales and bounds, not `lengths` and `block_table`.  `status`: optional 32-bit word that
     receives NNTILE_B200_PAGED_BAD_* bits."""
     N, H, P, D = pages.k.shape
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != H or k.shape[3] != D:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[0] != H or shape[3] != D:
         raise ValueError("k and v must be (kv_heads, batch, new_seq, head) rows for these pages")
     pages._check_rows(k, "k")
     if v.dtype != k.dtype or (pages.bounds is not None and pages.bounds.dtype != k.dtype):
         raise TypeError("k, v and the bounds must have one type")
-    B, n = k.shape[1], k.shape[2]
-    _check_table(pages, lengths, block_table, B)
+    B, n = shape[1], shape[2]
+    M = _check_table(lengths, block_table, B)
     if new_lens is not None and (new_lens.dtype != torch.int32 or new_lens.shape != (B,)):
         raise ValueError("new_lens must be int32 (batch,)")
     _check_status(status)
-    ops.paged_kv_append(D, P, N, block_table.shape[1], B, H, n, int(pages.e4m3), lengths, new_lens,
+    ops.paged_kv_append(D, P, N, M, B, H, n, int(pages.e4m3), lengths, new_lens,
                         block_table, k, v, pages.k, pages.v, pages.k_scales, pages.v_scales,
                         pages.bounds, status)
 
@@ -522,24 +530,28 @@ def paged_gather(pages, lengths, block_table, k, v, status=None):
     """Read the cache into k, v (kv_heads, batch, max_seq, head): rows 0 .. lengths[b] - 1 of
     every sequence; rows behind them are left as they are."""
     N, H, P, D = pages.k.shape
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != H or k.shape[3] != D:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[0] != H or shape[3] != D:
         raise ValueError("k and v must be (kv_heads, batch, max_seq, head) buffers for these pages")
     pages._check_rows(k, "k")
     if v.dtype != k.dtype:
         raise TypeError("k and v must have one type")
-    B = k.shape[1]
-    _check_table(pages, lengths, block_table, B)
+    B = shape[1]
+    M = _check_table(lengths, block_table, B)
     _check_status(status)
-    ops.paged_kv_gather(D, P, N, block_table.shape[1], B, H, k.shape[2], int(pages.e4m3), lengths,
+    ops.paged_kv_gather(D, P, N, M, B, H, shape[2], int(pages.e4m3), lengths,
                         block_table, pages.k, pages.v, pages.k_scales, pages.v_scales, k, v,
                         status)
 
 
 def _check_query(q, pages):
+    """(num_pages, kv_heads, page_size, head, group, batch) of a query that fits."""
     N, H, P, D = pages.k.shape
-    if q.dim() != 5 or q.shape[0] != H or q.shape[3] != 1 or q.shape[4] != D:
+    shape = q.shape
+    if len(shape) != 5 or shape[0] != H or shape[3] != 1 or shape[4] != D:
         raise ValueError("q must be (kv_heads, group, batch, 1, head) for these pages")
     pages._check_rows(q, "q")
+    return N, H, P, D, shape[1], shape[2]
 
 
 def paged_select(q, pages, lengths, block_table, num_selected, first_blocks=1, last_blocks=1,
@@ -547,16 +559,13 @@ def paged_select(q, pages, lengths, block_table, num_selected, first_blocks=1, l
     """Blocks that the new token of every sequence attends to, per kv head: the first and the
     last ones and those whose bounds allow the highest score.  Returns int32 (kv_heads,
     batch, num_selected), ascending block numbers, then -1."""
-    _check_query(q, pages)
+    N, H, P, D, G, B = _check_query(q, pages)
     if pages.bounds is None:
         raise ValueError("these pages keep no bounds")
     if pages.bounds.dtype != q.dtype:
         raise TypeError("q and the bounds must have one type")
-    H, G, B, one, D = q.shape
-    N, P = pages.k.shape[0], pages.k.shape[2]
-    _check_table(pages, lengths, block_table, B)
+    M = _check_table(lengths, block_table, B)
     _check_status(status)
-    M = block_table.shape[1]
     if out is None:
         out = torch.empty((H, B, num_selected), dtype=torch.int32, device=q.device)
     elif out.shape != (H, B, num_selected) or out.dtype != torch.int32:
@@ -575,17 +584,14 @@ def paged_decode(q, pages, lengths, block_table, selected=None, out=None, lse_ou
     sequence against its first lengths[b] positions, or against those of them in the blocks
     of `selected` (int32 (kv_heads, batch, num_selected), as paged_select returns).  Returns
     out shaped like q; lse_out: optional float32 (kv_heads, group, batch)."""
-    _check_query(q, pages)
-    H, G, B, one, D = q.shape
-    N, P = pages.k.shape[0], pages.k.shape[2]
-    _check_table(pages, lengths, block_table, B)
+    N, H, P, D, G, B = _check_query(q, pages)
+    M, S = _check_table(lengths, block_table, B), 0
     _check_status(status)
-    M, S = block_table.shape[1], 0
     if selected is not None:
-        if selected.dtype != torch.int32 or selected.dim() != 3 or selected.shape[:2] != (H, B) \
-                or selected.shape[2] == 0:
+        shape = selected.shape
+        if selected.dtype != torch.int32 or len(shape) != 3 or shape[:2] != (H, B) or shape[2] == 0:
             raise ValueError("selected must be int32 (kv_heads, batch, num_selected)")
-        S = selected.shape[2]
+        S = shape[2]
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype:
