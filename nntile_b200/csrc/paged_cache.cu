@@ -9,6 +9,8 @@
 namespace nb200 {
 
 constexpr int ROW_THREADS = 128;
+constexpr int ROWS_AHEAD = 4;
+constexpr int PART_ROWS = 32;
 
 // Elements a lane owns of a row.  VEC: eight neighbouring ones, one 16-byte access, LPR
 // lanes a row (LPR = 8, 16, 32 for heads up to 64, 128, 256).  Otherwise (a head that is
@@ -19,58 +21,77 @@ __device__ __forceinline__ int element(int lane, int i)
     return VEC ? 8*(lane & (LPR - 1)) + i : lane + 32*i;
 }
 
+// The eight elements as they lie in memory: fetched for several rows before the first is
+// used, so that a thread has that many loads in flight.
 template<typename T, bool VEC, int LPR>
-__device__ __forceinline__ void load_row(const T *row, int head, int lane, float (&x)[8])
+__device__ __forceinline__ uint4 fetch_row(const T *row, int head, int lane, bool live)
 {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
     if(VEC)
     {
         const int h = element<VEC, LPR>(lane, 0);
-        const uint4 v = h < head ? *reinterpret_cast<const uint4 *>(row + h)
+        return live && h < head ? __ldg(reinterpret_cast<const uint4 *>(row + h))
                 : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for(int i = 0; i < 4; ++i)
-        {
-            const float2 f = unpack2<T>(w[i]);
-            x[2*i] = f.x;
-            x[2*i + 1] = f.y;
-        }
     }
-    else
-    {
 #pragma unroll
-        for(int i = 0; i < 8; ++i)
+    for(int i = 0; i < 8; ++i)
+    {
+        const int h = element<VEC, LPR>(lane, i);
+        unsigned short v = 0;
+        if(live && h < head)
         {
-            const int h = element<VEC, LPR>(lane, i);
-            x[i] = h < head ? to_f(row[h]) : 0.0f;
+            v = __ldg(reinterpret_cast<const unsigned short *>(row) + h);
         }
+        w[i >> 1] |= (uint32_t)v << 16*(i & 1);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template<typename T>
+__device__ __forceinline__ void widen(const uint4 &v, float (&x)[8])
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+    {
+        const float2 f = unpack2<T>(w[i]);
+        x[2*i] = f.x;
+        x[2*i + 1] = f.y;
     }
 }
 
 template<typename T, bool VEC, int LPR>
-__device__ __forceinline__ void store_row(T *row, int head, int lane, const float (&x)[8])
+__device__ __forceinline__ void store_row(T *row, int head, int lane, const uint4 &v)
 {
     if(VEC)
     {
         const int h = element<VEC, LPR>(lane, 0);
         if(h < head)
         {
-            *reinterpret_cast<uint4 *>(row + h) = make_uint4(pack2<T>(x[0], x[1]),
-                    pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+            *reinterpret_cast<uint4 *>(row + h) = v;
         }
     }
     else
     {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for(int i = 0; i < 8; ++i)
         {
             const int h = element<VEC, LPR>(lane, i);
             if(h < head)
             {
-                row[h] = from_f<T>(x[i]);
+                reinterpret_cast<unsigned short *>(row)[h] = (unsigned short)(w[i >> 1]
+                        >> 16*(i & 1));
             }
         }
     }
+}
+
+template<typename T>
+__device__ __forceinline__ uint4 narrow(const float (&x)[8])
+{
+    return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+            pack2<T>(x[6], x[7]));
 }
 
 template<bool VEC, int LPR>
@@ -100,27 +121,25 @@ __device__ __forceinline__ void store_codes(uint8_t *row, int head, int lane,
 }
 
 template<bool VEC, int LPR>
-__device__ __forceinline__ void load_codes(const uint8_t *row, int head, int lane,
-        uint32_t (&c)[4])
+__device__ __forceinline__ uint2 fetch_codes(const uint8_t *row, int head, int lane, bool live)
 {
     if(VEC)
     {
         const int h = element<VEC, LPR>(lane, 0);
-        const uint2 v = h < head ? *reinterpret_cast<const uint2 *>(row + h) : make_uint2(0u, 0u);
-        c[0] = v.x & 0xFFFFu;
-        c[1] = v.x >> 16;
-        c[2] = v.y & 0xFFFFu;
-        c[3] = v.y >> 16;
+        return live && h < head ? __ldg(reinterpret_cast<const uint2 *>(row + h))
+                : make_uint2(0u, 0u);
     }
-    else
-    {
+    uint32_t w[2] = {0u, 0u};
 #pragma unroll
-        for(int i = 0; i < 4; ++i)
+    for(int i = 0; i < 8; ++i)
+    {
+        const int h = element<VEC, LPR>(lane, i);
+        if(live && h < head)
         {
-            const int lo = element<VEC, LPR>(lane, 2*i), hi = element<VEC, LPR>(lane, 2*i + 1);
-            c[i] = (lo < head ? (uint32_t)row[lo] : 0u) | (hi < head ? (uint32_t)row[hi] << 8 : 0u);
+            w[i >> 2] |= (uint32_t)__ldg(row + h) << 8*(i & 3);
         }
     }
+    return make_uint2(w[0], w[1]);
 }
 
 // Quantise the eight elements a lane owns (its row shared by the LPR lanes around it):
@@ -159,8 +178,11 @@ __device__ __forceinline__ uint32_t quantise_row(float (&x)[8], uint32_t (&c)[4]
     return byte;
 }
 
-// One CTA owns one (sequence, kv head, touched block): the block's new rows of K and V,
-// and, because no other CTA writes this (page, kv head), its key bounds without atomics.
+// A CTA writes up to PART_ROWS new rows of one (sequence, kv head, touched block): of K for an
+// even blockIdx.y, of V for an odd one.  With bounds the first K part takes all rows of the
+// block instead: because no other CTA writes this (page, kv head), it needs no atomics.  Four
+// rows a thread are fetched before the first is stored, the first ones before the page is
+// known: a step of one token is a chain of memory latencies and nothing else.
 // A block's bounds are those of its stored (for 8-bit pages: quantised) keys, rounded to T;
 // rows that were in the page before are merged in unless the block starts with this call.
 template<typename T, bool E4M3, bool VEC, int LPR>
@@ -188,18 +210,45 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     const int block = start/page_size + j;
     int first, last;
     rows_in_block(start, count, block, page_size, first, last);
-    if(first >= last)
+    const bool is_k = (blockIdx.y & 1) == 0;
+    const bool bounded = is_k && bounds != nullptr;
+    const int part = blockIdx.y >> 1;
+    if(!bounded)
+    {
+        first += part*PART_ROWS;
+        last = min(last, first + PART_ROWS);
+    }
+    if(first >= last || (bounded && part > 0))
     {
         return;
+    }
+    const int rows = last - first;
+    const T *src = (is_k ? k : v) + ((size_t)unit*new_seq + ((size_t)block*page_size + first
+            - start))*head;
+    uint4 raw[ROWS_AHEAD];
+#pragma unroll
+    for(int u = 0; u < ROWS_AHEAD; ++u)
+    {
+        const int row = u*SLOTS + slot;
+        raw[u] = fetch_row<T, VEC, LPR>(src + (size_t)row*head, head, lane, row < rows);
     }
     const int page = checked_page(block_table + (size_t)b*max_blocks, block, num_pages, status);
     if(page < 0)
     {
         return;
     }
-    const size_t dst0 = ((size_t)page*kv_heads + kvh)*page_size;
-    const int rows = last - first;
-    const size_t src0 = ((size_t)unit*new_seq + ((size_t)block*page_size + first - start));
+    const size_t dst0 = ((size_t)page*kv_heads + kvh)*page_size + first;
+    // what the bounds were: head <= 256 elements on 128 threads
+    T *low_g = bounds + ((size_t)page*kv_heads + kvh)*2*head, *high_g = low_g + head;
+    float low_was[2], high_was[2];
+#pragma unroll
+    for(int i = 0; i < 2; ++i)
+    {
+        const int h = threadIdx.x + i*ROW_THREADS;
+        const bool old = bounded && first > 0 && h < head;
+        low_was[i] = old ? to_f(low_g[h]) : CUDART_INF_F;
+        high_was[i] = old ? to_f(high_g[h]) : -CUDART_INF_F;
+    }
     float low[8], high[8];
 #pragma unroll
     for(int i = 0; i < 8; ++i)
@@ -208,55 +257,61 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
         high[i] = -CUDART_INF_F;
     }
     // warps stay converged: the quantiser shuffles within a row's lanes
-    for(int r0 = 0; r0 < 2*rows; r0 += SLOTS)
+    void *pages = is_k ? k_pages : v_pages;
+    uint8_t *scales = is_k ? k_scales : v_scales;
+    for(int r0 = 0; r0 < rows; r0 += ROWS_AHEAD*SLOTS)
     {
-        const int r = r0 + slot;
-        const bool live = r < 2*rows;
-        const bool is_k = r < rows;
-        const int row = is_k ? r : r - rows;
-        float x[8];
-        if(live)
-        {
-            load_row<T, VEC, LPR>((is_k ? k : v) + (src0 + row)*head, head, lane, x);
-        }
-        else
-        {
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                x[i] = 0.0f;
-            }
-        }
-        const size_t dst = dst0 + first + row;
-        if(E4M3)
+        for(int u = 0; u < ROWS_AHEAD; ++u)
         {
-            uint32_t c[4];
-            const uint32_t byte = quantise_row<LPR>(x, c);
-            if(live)
+            const int row = r0 + u*SLOTS + slot;
+            const bool live = row < rows;
+            const size_t dst = dst0 + row;
+            float x[8];
+            if(E4M3)
             {
-                store_codes<VEC, LPR>((uint8_t *)(is_k ? k_pages : v_pages) + dst*head, head,
-                        lane, c);
-                if((lane & (LPR - 1)) == 0)
+                if(r0 + u*SLOTS >= rows)
                 {
-                    (is_k ? k_scales : v_scales)[dst] = (uint8_t)byte;
+                    break;                       // the whole CTA
+                }
+                widen<T>(raw[u], x);
+                uint32_t c[4];
+                const uint32_t byte = quantise_row<LPR>(x, c);
+                if(live)
+                {
+                    store_codes<VEC, LPR>((uint8_t *)pages + dst*head, head, lane, c);
+                    if((lane & (LPR - 1)) == 0)
+                    {
+                        scales[dst] = (uint8_t)byte;
+                    }
+                }
+            }
+            else if(live)
+            {
+                store_row<T, VEC, LPR>((T *)pages + dst*head, head, lane, raw[u]);
+            }
+            if(bounded && live)
+            {
+                if(!E4M3)
+                {
+                    widen<T>(raw[u], x);
+                }
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                {
+                    low[i] = min_nan(low[i], x[i]);
+                    high[i] = max_nan(high[i], x[i]);
                 }
             }
         }
-        else if(live)
-        {
-            store_row<T, VEC, LPR>((T *)(is_k ? k_pages : v_pages) + dst*head, head, lane, x);
-        }
-        if(bounds && live && is_k)
-        {
 #pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                low[i] = min_nan(low[i], x[i]);
-                high[i] = max_nan(high[i], x[i]);
-            }
+        for(int u = 0; u < ROWS_AHEAD; ++u)
+        {
+            const int row = r0 + (u + ROWS_AHEAD)*SLOTS + slot;
+            raw[u] = fetch_row<T, VEC, LPR>(src + (size_t)row*head, head, lane, row < rows);
         }
     }
-    if(!bounds)
+    if(!bounded)
     {
         return;
     }
@@ -268,23 +323,22 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
         high_s[slot][element<VEC, LPR>(lane, i)] = high[i];
     }
     __syncthreads();
-    T *low_g = bounds + ((size_t)page*kv_heads + kvh)*2*head, *high_g = low_g + head;
-    for(int h = threadIdx.x; h < head; h += ROW_THREADS)
-    {
-        float a = low_s[0][h], z = high_s[0][h];
 #pragma unroll
-        for(int s = 1; s < SLOTS; ++s)
+    for(int i = 0; i < 2; ++i)
+    {
+        const int h = threadIdx.x + i*ROW_THREADS;
+        if(h < head)
         {
-            a = min_nan(a, low_s[s][h]);
-            z = max_nan(z, high_s[s][h]);
+            float a = low_was[i], z = high_was[i];
+#pragma unroll
+            for(int s = 0; s < SLOTS; ++s)
+            {
+                a = min_nan(a, low_s[s][h]);
+                z = max_nan(z, high_s[s][h]);
+            }
+            low_g[h] = from_f<T>(a);
+            high_g[h] = from_f<T>(z);
         }
-        if(first > 0)
-        {
-            a = min_nan(a, to_f(low_g[h]));
-            z = max_nan(z, to_f(high_g[h]));
-        }
-        low_g[h] = from_f<T>(a);
-        high_g[h] = from_f<T>(z);
     }
 }
 
@@ -293,7 +347,7 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
 template<typename T, bool E4M3, bool VEC, int LPR>
 __global__ void __launch_bounds__(ROW_THREADS)
 paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
-        int kv_heads, int max_seq, int rows_per_cta, int chunks,
+        int kv_heads, int max_seq, int rows_per_cta, int chunks, int page_shift,
         const int32_t *__restrict__ lengths, const int32_t *__restrict__ block_table,
         const void *__restrict__ k_pages, const void *__restrict__ v_pages,
         const uint8_t *__restrict__ k_scales, const uint8_t *__restrict__ v_scales,
@@ -316,35 +370,68 @@ paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     T *out = (is_k ? k : v) + (size_t)unit*max_seq*head;
     const int64_t begin = (int64_t)chunk*rows_per_cta;
     const int end = (int)min((int64_t)len, begin + rows_per_cta);
-    for(int64_t r = begin + slot; r < end; r += SLOTS)
+    // four rows at a time: their pages are looked up together, then fetched together
+    for(int64_t r0 = begin; r0 < end; r0 += ROWS_AHEAD*SLOTS)
     {
-        const int block = (int)r/page_size;
-        const int page = checked_page(block_table + (size_t)b*max_blocks, block, num_pages,
-                status);
-        if(page < 0)
-        {
-            continue;
-        }
-        const size_t src = ((size_t)page*kv_heads + kvh)*page_size + ((int)r - block*page_size);
-        float x[8];
-        if(E4M3)
-        {
-            uint32_t c[4];
-            load_codes<VEC, LPR>((const uint8_t *)pages + src*head, head, lane, c);
-            const float scale = scale_value(scales[src]);
+        size_t src[ROWS_AHEAD];
+        bool live[ROWS_AHEAD];
 #pragma unroll
-            for(int i = 0; i < 4; ++i)
+        for(int u = 0; u < ROWS_AHEAD; ++u)
+        {
+            const int64_t r = r0 + u*SLOTS + slot;
+            live[u] = r < end;
+            src[u] = 0;
+            if(live[u])
             {
-                const float2 f = e4m3x2_to_f2(c[i]);
-                x[2*i] = f.x*scale;
-                x[2*i + 1] = f.y*scale;
+                const int block = page_shift >= 0 ? (int)r >> page_shift : (int)r/page_size;
+                const int page = checked_page(block_table + (size_t)b*max_blocks, block,
+                        num_pages, status);
+                live[u] = page >= 0;
+                src[u] = ((size_t)max(page, 0)*kv_heads + kvh)*page_size
+                        + ((int)r - block*page_size);
             }
         }
-        else
+        uint4 raw[ROWS_AHEAD];
+        uint32_t byte[ROWS_AHEAD];
+#pragma unroll
+        for(int u = 0; u < ROWS_AHEAD; ++u)
         {
-            load_row<T, VEC, LPR>((const T *)pages + src*head, head, lane, x);
+            if(E4M3)
+            {
+                const uint2 c = fetch_codes<VEC, LPR>((const uint8_t *)pages + src[u]*head, head,
+                        lane, live[u]);
+                raw[u] = make_uint4(c.x, c.y, 0u, 0u);
+                byte[u] = live[u] ? scales[src[u]] : 0u;
+            }
+            else
+            {
+                raw[u] = fetch_row<T, VEC, LPR>((const T *)pages + src[u]*head, head, lane,
+                        live[u]);
+            }
         }
-        store_row<T, VEC, LPR>(out + (size_t)r*head, head, lane, x);
+#pragma unroll
+        for(int u = 0; u < ROWS_AHEAD; ++u)
+        {
+            if(E4M3)
+            {
+                const float scale = scale_value(byte[u]);
+                float x[8];
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+                {
+                    const uint32_t two = (i < 2 ? raw[u].x : raw[u].y) >> 16*(i & 1) & 0xFFFFu;
+                    const float2 f = e4m3x2_to_f2(two);
+                    x[2*i] = f.x*scale;
+                    x[2*i + 1] = f.y*scale;
+                }
+                raw[u] = narrow<T>(x);
+            }
+            if(live[u])
+            {
+                store_row<T, VEC, LPR>(out + (size_t)(r0 + u*SLOTS + slot)*head, head, lane,
+                        raw[u]);
+            }
+        }
     }
 }
 
@@ -385,7 +472,10 @@ static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     }
     const int64_t touched = std::min(most_touched(new_seq, page_size), max_blocks);
     if(touched*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
-    const unsigned grid = (unsigned)(touched*batch*kv_heads);
+    // parts of a block that this call may fill
+    const int64_t most = std::min(new_seq, page_size);
+    const dim3 grid((unsigned)(touched*batch*kv_heads),
+            (unsigned)(2*((most + PART_ROWS - 1)/PART_ROWS)));
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
 #define NB200_APPEND(E, V, L) paged_append_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
@@ -436,11 +526,16 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     const int64_t chunks = (reach + rows_per_cta - 1)/rows_per_cta;
     if(chunks*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
     const dim3 grid((unsigned)(chunks*batch*kv_heads), 2);
+    int shift = -1;                              // of a power of two, the usual page size
+    for(int i = 0; i <= 16; ++i)
+    {
+        shift = page_size == (int64_t)1 << i ? i : shift;
+    }
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
 #define NB200_GATHER(E, V, L) paged_gather_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
         (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
-        (int)max_seq, (int)rows_per_cta, (int)chunks, lengths, block_table, k_pages, v_pages, \
+        (int)max_seq, (int)rows_per_cta, (int)chunks, shift, lengths, block_table, k_pages, v_pages, \
         k_scales, v_scales, (T *)k, (T *)v, status)
 #define NB200_GATHER_L(E) \
     do { \

@@ -56,27 +56,64 @@ struct PagedSelectArgs
     int32_t *selected;
     float2 *scores;                              // [unit][block]: score, bound of its error
     unsigned long long *keys;                    // [unit][block]: exact, where it was needed
+    bool vec;                                    // q and bounds allow 16-byte accesses
     uint32_t *status;
 };
 
-// The exact key of a block for query head g, by a whole warp (same value in every lane).
+// One element's part of a score in 64 bits.  The product of two 16-bit factors is exact in 32
+// bits while it is a normal number; the rest goes the long way, which also gives infinite and
+// NaN bounds the value of the formula.
+__device__ __forceinline__ double exact_term(float q, float low, float high)
+{
+    const float p = q*(q > 0.0f ? high : low), size = fabsf(p);
+    const bool plain = size < 1e38f && (size > 1e-30f || q == 0.0f)
+            && fabsf(low) < CUDART_INF_F && fabsf(high) < CUDART_INF_F;
+    if(plain)
+    {
+        return (double)p;
+    }
+    return q != q ? (double)q : (double)fmaxf(q, 0.0f)*(double)high
+            + (double)fminf(q, 0.0f)*(double)low;
+}
+
+// The exact key of a block for query head g, by 16 lanes (the same value in each of them;
+// the whole warp takes part in the shuffles).
 template<typename T>
 __device__ __forceinline__ unsigned long long exact_key(const PagedSelectArgs &a, int kvh, int b,
-        int page, int g, int lane)
+        int page, int g)
 {
+    const int l16 = threadIdx.x & 15;
     const T *low = (const T *)a.bounds + ((size_t)page*a.kv_heads + kvh)*2*a.head;
     const T *high = low + a.head;
     const T *q = (const T *)a.q + (((size_t)kvh*a.group + g)*a.batch + b)*a.head;
     double s = 0.0;
-#pragma unroll 4
-    for(int h = lane; h < a.head; h += 32)
+    if(a.vec)
     {
-        const double x = (double)to_f(q[h]);
-        s += x != x ? x : (x > 0.0 ? x : 0.0)*(double)to_f(high[h])
-                + (x < 0.0 ? x : 0.0)*(double)to_f(low[h]);
+        for(int h = 8*l16; h < a.head; h += 128)
+        {
+            const uint4 qv = *reinterpret_cast<const uint4 *>(q + h);
+            const uint4 lv = *reinterpret_cast<const uint4 *>(low + h);
+            const uint4 hv = *reinterpret_cast<const uint4 *>(high + h);
+            const uint32_t qw[4] = {qv.x, qv.y, qv.z, qv.w};
+            const uint32_t lw[4] = {lv.x, lv.y, lv.z, lv.w};
+            const uint32_t hw[4] = {hv.x, hv.y, hv.z, hv.w};
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                const float2 x = unpack2<T>(qw[i]), y = unpack2<T>(lw[i]), z = unpack2<T>(hw[i]);
+                s += exact_term(x.x, y.x, z.x) + exact_term(x.y, y.y, z.y);
+            }
+        }
+    }
+    else
+    {
+        for(int h = l16; h < a.head; h += 16)
+        {
+            s += exact_term(to_f(q[h]), to_f(low[h]), to_f(high[h]));
+        }
     }
 #pragma unroll
-    for(int o = 16; o > 0; o >>= 1)
+    for(int o = 8; o > 0; o >>= 1)
     {
         s += __shfl_xor_sync(0xffffffffu, s, o);
     }
@@ -88,39 +125,39 @@ __device__ __forceinline__ int filled_blocks(const PagedSelectArgs &a, int b, ui
     return blocks_of(checked_length(a.lengths, b, a.max_blocks*a.page_size, status), a.page_size);
 }
 
-// Any head: a warp per block, sums in 64 bits, rounded once.
+// Any head: 16 lanes per block, sums in 64 bits, rounded once.
 template<typename T>
 __global__ void __launch_bounds__(128)
 paged_score_generic_kernel(const PagedSelectArgs a)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int chunks = (a.max_blocks + 3)/4;
+    const int chunks = (a.max_blocks + 7)/8;
     const int unit = blockIdx.x/chunks;
-    const int block = (blockIdx.x - unit*chunks)*4 + warp;
+    const int block = (blockIdx.x - unit*chunks)*8 + (threadIdx.x >> 4);
     const int b = unit % a.batch, kvh = unit/a.batch;
-    if(block >= filled_blocks(a, b, a.status))
+    const bool live = block < filled_blocks(a, b, a.status);
+    const int page = live ? checked_page(a.block_table + (size_t)b*a.max_blocks, block,
+            a.num_pages, a.status) : -1;
+    if(a.num_pages == 0)
     {
-        return;
+        return;                                  // no bounds to read; the whole grid
     }
-    const int page = checked_page(a.block_table + (size_t)b*a.max_blocks, block, a.num_pages,
-            a.status);
-    float s = -CUDART_INF_F, error = 0.0f;
-    if(page >= 0)
+    unsigned long long key = 0ull;
+    for(int g = 0; g < a.group; ++g)
     {
-        unsigned long long key = 0ull;
-        for(int g = 0; g < a.group; ++g)
+        const unsigned long long one = exact_key<T>(a, kvh, b, max(page, 0), g);
+        key = one > key ? one : key;
+    }
+    if(live && (threadIdx.x & 15) == 0)
+    {
+        float s = -CUDART_INF_F, error = 0.0f;
+        if(page >= 0)
         {
-            const unsigned long long one = exact_key<T>(a, kvh, b, page, g, lane);
-            key = one > key ? one : key;
+            const double exact = __longlong_as_double((long long)((key >> 63)
+                    ? key & 0x7FFFFFFFFFFFFFFFull : ~key));
+            s = key == ~0ull ? CUDART_NAN_F : (float)exact;
+            error = fabsf(s)*1.2e-7f + SCORE_FLOOR;      // infinite and NaN ones stay so
         }
-        const double exact = __longlong_as_double((long long)((key >> 63)
-                ? key & 0x7FFFFFFFFFFFFFFFull : ~key));
-        s = key == ~0ull ? CUDART_NAN_F : (float)exact;
-        error = fabsf(s)*1.2e-7f + SCORE_FLOOR;          // infinite and NaN ones stay so
-    }
-    if(lane == 0)
-    {
         a.scores[(size_t)unit*a.max_blocks + block] = make_float2(s, error);
     }
 }
@@ -492,7 +529,9 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ float fred[PICK_WARPS];
     __shared__ int listed_s, list_s[PICK_LIST];
     __shared__ unsigned long long list_key_s[PICK_LIST], cut_s;
-    __shared__ int equal_want_s, bin_s[256];
+    __shared__ int equal_want_s;
+    __shared__ __align__(16) int bin_s[256];
+    __shared__ int4 hit_s;
     __shared__ float list_score_s[PICK_LIST], last_s;
     __shared__ uint2 mask_s[PICK_THREADS];
     __shared__ uint32_t low_s, high_s;
@@ -585,38 +624,37 @@ paged_pick_kernel(const PagedSelectArgs a)
                 }
             }
             __syncthreads();
-            // every warp finds the bin: lane 0 has the top eight
-            int c[8], sum = 0;
-#pragma unroll
-            for(int k = 0; k < 8; ++k)
+            // the first warp finds the bin: lane 31 - l has the eight from 8l on
+            if(warp == 0)
             {
-                c[k] = bin_s[255 - 8*lane - k];
-                sum += c[k];
-            }
-            int scan = sum;
+                const int4 c0 = *reinterpret_cast<const int4 *>(bin_s + 8*(31 - lane));
+                const int4 c1 = *reinterpret_cast<const int4 *>(bin_s + 8*(31 - lane) + 4);
+                const int c[8] = {c1.w, c1.z, c1.y, c1.x, c0.w, c0.z, c0.y, c0.x};
+                const int sum = c[0] + c[1] + c[2] + c[3] + c[4] + c[5] + c[6] + c[7];
+                int scan = sum;
 #pragma unroll
-            for(int o = 1; o < 32; o <<= 1)
-            {
-                const int up = __shfl_up_sync(0xffffffffu, scan, o);
-                scan += lane >= o ? up : 0;
-            }
-            int above = scan - sum, hit = 0, hits = 0, left = 0;
-            const bool here = above < rank && scan >= rank;
-#pragma unroll
-            for(int k = 0; k < 8; ++k)
-            {
-                if(above < rank && above + c[k] >= rank)
+                for(int o = 1; o < 32; o <<= 1)
                 {
-                    hit = 255 - 8*lane - k;
-                    left = rank - above;
-                    hits = c[k];
+                    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+                    scan += lane >= o ? up : 0;
                 }
-                above += c[k];
+                int above = scan - sum;
+                if(above < rank && scan >= rank)
+                {
+#pragma unroll
+                    for(int k = 0; k < 8; ++k)
+                    {
+                        if(above < rank && above + c[k] >= rank)
+                        {
+                            hit_s = make_int4(8*(31 - lane) + 7 - k, c[k], rank - above, 0);
+                        }
+                        above += c[k];
+                    }
+                }
             }
-            const int from = __ffs((int)__ballot_sync(0xffffffffu, here)) - 1;
-            hit = __shfl_sync(0xffffffffu, hit, from);
-            hits = __shfl_sync(0xffffffffu, hits, from);
-            rank = __shfl_sync(0xffffffffu, left, from);
+            __syncthreads();
+            const int hit = hit_s.x, hits = hit_s.y;
+            rank = hit_s.z;
             if(hits <= PICK_LIST)
             {
 #pragma unroll 4
@@ -734,9 +772,8 @@ paged_pick_kernel(const PagedSelectArgs a)
         take_near = need >= near;
         if(!take_near)
         {
-            // a warp per block and query head
+            // 16 lanes per block and query head
             const bool listed = near <= PICK_LIST;
-            const long long todo = (long long)(listed ? near : end - begin)*a.group;
             if(!listed)
             {
                 for(int i = begin + tid; i < end; i += PICK_THREADS)
@@ -745,22 +782,32 @@ paged_pick_kernel(const PagedSelectArgs a)
                 }
                 __syncthreads();
             }
-            for(long long k = warp; k < todo; k += PICK_WARPS)
+            const int most = listed ? near : end - begin;
+            int c = (tid >> 4)/a.group, g = (tid >> 4) - c*a.group;
+            const int dc = (PICK_THREADS/16)/a.group, dg = PICK_THREADS/16 - dc*a.group;
+            while(__any_sync(0xffffffffu, c < most))
             {
-                const int c = (int)(k/a.group), g = (int)(k - (long long)c*a.group);
-                const int i = listed ? list_s[c] : begin + c;
-                if(!listed && !is_near(score(i)))
+                const int i = c >= most ? -1 : listed ? list_s[c] : begin + c;
+                int page = -1;
+                if(i >= 0 && (listed || is_near(score(i))))
                 {
-                    continue;
+                    page = a.block_table[(size_t)b*a.max_blocks + i];
+                    page = page_in_pool(page, a.num_pages) ? page : -1;
                 }
-                const int page = a.block_table[(size_t)b*a.max_blocks + i];
-                if(page_in_pool(page, a.num_pages))
+                if(__any_sync(0xffffffffu, page >= 0))
                 {
-                    const unsigned long long key = exact_key<T>(a, kvh, b, page, g, lane);
-                    if(lane == 0)
+                    const unsigned long long key = exact_key<T>(a, kvh, b, max(page, 0), g);
+                    if(page >= 0 && (tid & 15) == 0)
                     {
                         atomicMax(listed ? &list_key_s[c] : &keys[i], key);
                     }
+                }
+                c += dc;
+                g += dg;
+                if(g >= a.group)
+                {
+                    g -= a.group;
+                    ++c;
                 }
             }
             __syncthreads();
@@ -1011,9 +1058,9 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.scores = static_cast<float2 *>(workspace);
     a.keys = reinterpret_cast<unsigned long long *>(a.scores + (size_t)units*max_blocks);
     a.status = status;
-    // 16-byte rows, and tiles that 30 bits can count
-    const bool vec = head % 8 == 0 && aligned16(q) && aligned16(bounds)
-            && units*((max_blocks + SCORE_TILE - 1)/SCORE_TILE) < (int64_t)1 << 30;
+    // 16-byte rows; for the tensor instruction also tiles that 30 bits can count
+    a.vec = head % 8 == 0 && aligned16(q) && aligned16(bounds);
+    const bool vec = a.vec && units*((max_blocks + SCORE_TILE - 1)/SCORE_TILE) < (int64_t)1 << 30;
     cudaStream_t s = as_stream(stream);
     int st2 = NNTILE_B200_OK;
     if(max_blocks > num_selected)                // otherwise everything is taken
@@ -1023,7 +1070,7 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
         else if(vec) st2 = launch_score<T, 256>(s, a);
         else
         {
-            const int64_t ctas = units*((max_blocks + 3)/4);
+            const int64_t ctas = units*((max_blocks + 7)/8);
             if(ctas > INT32_MAX) return NNTILE_B200_E_SHAPE;
             paged_score_generic_kernel<T><<<(unsigned)ctas, 128, 0, s>>>(a);
             st2 = launch_status();
