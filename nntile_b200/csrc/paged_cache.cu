@@ -142,38 +142,61 @@ __device__ __forceinline__ uint2 fetch_codes(const uint8_t *row, int head, int l
     return make_uint2(w[0], w[1]);
 }
 
-// Quantise the eight elements a lane owns (its row shared by the LPR lanes around it):
-// returns the exponent byte, leaves the codes in `c` and the stored values in `x`.
-template<int LPR>
-__device__ __forceinline__ uint32_t quantise_row(float (&x)[8], uint32_t (&c)[4])
+// The larger of two packed pairs of magnitudes; a NaN loses.
+template<typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template<> __device__ __forceinline__ uint32_t max2<bf16>(uint32_t a, uint32_t b)
 {
-    float amax = 0.0f;
-#pragma unroll
-    for(int i = 0; i < 8; ++i)
-    {
-        const float a = fabsf(x[i]);
-        amax = a < CUDART_INF_F ? fmaxf(amax, a) : amax;     // infinities and NaN do not count
-    }
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Quantise the eight elements a lane owns (its row shared by the LPR lanes around it):
+// returns the exponent byte, leaves the codes in `c`.  The largest magnitude is found on
+// packed pairs; only a row that holds an infinity goes through the elements one by one.
+// The format has no infinity: what is not finite is kept as NaN.
+template<typename T, int LPR>
+__device__ __forceinline__ uint32_t quantise_row(const uint4 &raw, uint32_t (&c)[4])
+{
+    constexpr uint32_t ABS = 0x7FFF7FFFu;
+    uint32_t top = max2<T>(max2<T>(raw.x & ABS, raw.y & ABS), max2<T>(raw.z & ABS, raw.w & ABS));
 #pragma unroll
     for(int o = LPR/2; o > 0; o >>= 1)
     {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        top = max2<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    const float2 two = unpack2<T>(top);
+    float amax = fmaxf(fmaxf(two.x, two.y), 0.0f);           // all NaN: 0
+    float x[8];
+    widen<T>(raw, x);
+    if(__any_sync(0xffffffffu, amax == CUDART_INF_F))
+    {
+        amax = 0.0f;
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            const float a = fabsf(x[i]);
+            amax = a < CUDART_INF_F ? fmaxf(amax, a) : amax;
+            x[i] = a < CUDART_INF_F ? x[i] : CUDART_NAN_F;
+        }
+#pragma unroll
+        for(int o = LPR/2; o > 0; o >>= 1)
+        {
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        }
     }
     const uint32_t byte = scale_byte(amax);
-    const float inv = inverse_scale(byte), scale = scale_value(byte);
-#pragma unroll
-    for(int i = 0; i < 8; ++i)
-    {
-        // the format has no infinity: what is not finite is kept as NaN
-        x[i] = fabsf(x[i]) < CUDART_INF_F ? x[i]*inv : CUDART_NAN_F;
-    }
+    const float inv = inverse_scale(byte);
 #pragma unroll
     for(int i = 0; i < 4; ++i)
     {
-        c[i] = f2_to_e4m3x2(x[2*i], x[2*i + 1]);
-        const float2 back = e4m3x2_to_f2(c[i]);
-        x[2*i] = back.x*scale;
-        x[2*i + 1] = back.y*scale;
+        c[i] = f2_to_e4m3x2(x[2*i]*inv, x[2*i + 1]*inv);
     }
     return byte;
 }
@@ -274,9 +297,19 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
                 {
                     break;                       // the whole CTA
                 }
-                widen<T>(raw[u], x);
                 uint32_t c[4];
-                const uint32_t byte = quantise_row<LPR>(x, c);
+                const uint32_t byte = quantise_row<T, LPR>(raw[u], c);
+                if(bounded)
+                {
+                    const float scale = scale_value(byte);
+#pragma unroll
+                    for(int i = 0; i < 4; ++i)
+                    {
+                        const float2 back = e4m3x2_to_f2(c[i]);
+                        x[2*i] = back.x*scale;
+                        x[2*i + 1] = back.y*scale;
+                    }
+                }
                 if(live)
                 {
                     store_codes<VEC, LPR>((uint8_t *)pages + dst*head, head, lane, c);

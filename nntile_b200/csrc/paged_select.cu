@@ -534,6 +534,7 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ int4 hit_s;
     __shared__ float list_score_s[PICK_LIST], last_s;
     __shared__ uint2 mask_s[PICK_THREADS];
+    __shared__ int2 before_s[PICK_THREADS];
     __shared__ uint32_t low_s, high_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int unit = blockIdx.x, b = unit % a.batch, kvh = unit/a.batch;
@@ -875,7 +876,7 @@ paged_pick_kernel(const PagedSelectArgs a)
         const unsigned long long key = keys[i];
         return key > cut ? 2 : key == cut ? 1 : 0;
     };
-    // write in index order: 32 neighbours a warp as two masks, a thread per mask for the rest
+    // write in index order: 32 neighbours a warp as two masks, a thread per mask for the sums
     int taken = 0, equals = 0;                   // of the runs before
     for(int base = 0; base < n; base += 32*PICK_THREADS)
     {
@@ -923,17 +924,20 @@ paged_pick_kernel(const PagedSelectArgs a)
             taken += red[w];
             equals += red2[w];
         }
-        for(unsigned any = mine.x | mine.y; any != 0u; any &= any - 1u)
+        before_s[tid] = make_int2(before_t, before_e);
+        __syncthreads();
+        for(int k = warp; k < PICK_THREADS && base + 32*k < n; k += PICK_WARPS)
         {
-            const int k = __ffs((int)any) - 1;
-            const bool equal = (mine.y >> k & 1u) != 0u;
-            const int at = before_t + min(before_e, equal_want);
-            if((!equal || before_e < equal_want) && at < S)
+            const uint2 mask = mask_s[k];
+            const int2 before = before_s[k];
+            const unsigned below = (1u << lane) - 1u;
+            const bool equal = (mask.y >> lane & 1u) != 0u;
+            const int e = before.y + __popc(mask.y & below);
+            const int at = before.x + __popc(mask.x & below) + min(e, equal_want);
+            if((((mask.x >> lane & 1u) != 0u) || (equal && e < equal_want)) && at < S)
             {
-                out[at] = base + 32*tid + k;
+                out[at] = base + 32*k + lane;
             }
-            before_t += equal ? 0 : 1;
-            before_e += equal ? 1 : 0;
         }
     }
 }
