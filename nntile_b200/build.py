@@ -2,6 +2,9 @@
 
     python -m nntile_b200.build [--force]
 
+The calls of the paged cache on torch tensors are a Python extension module beside the
+library, ``_paged_torch.so`` (``csrc/paged_torch.cpp``, g++ against torch's headers).
+
 One nvcc invocation per source (object files are cached under csrc/build/), then
 one link step into ``csrc/libnntile_b200.so``.  nvcc cross-compiles without a
 GPU.  The library has no link-time dependency beyond the CUDA runtime (linked
@@ -20,6 +23,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libnntile_b200.so")
+TORCH_MODULE = os.path.join(HERE, "_paged_torch.so")
 SOURCES = [
     "vanilla_ops.cu", "flash_generic.cu", "flash_api.cu", "decode.cu",
     "flash_fwd_sm100.cu", "flash_bwd_sm100.cu", "host_tensor.cu", "gemm_cublas.cu",
@@ -70,6 +74,29 @@ def _compile(job, force: bool) -> str:
     return obj
 
 
+def _build_torch_module(force: bool) -> str:
+    """The extension module; it finds the library beside it and torch's in the process."""
+    src = os.path.join(CSRC, "paged_torch.cpp")
+    header = os.path.join(os.path.dirname(HERE), "include", "nntile_b200.h")
+    if force or _stale(TORCH_MODULE, [src, header]):
+        import sysconfig
+
+        import torch
+        base = os.path.dirname(torch.__file__)
+        cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(base, "include"),
+               "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               "-I" + os.path.join(cuda, "include"), src, "-o", TORCH_MODULE,
+               "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+               "-lc10_cuda", "-L" + CSRC, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN/csrc"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed on paged_torch.cpp:\n{res.stdout}{res.stderr}")
+    return TORCH_MODULE
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     jobs = [(s, False) for s in SOURCES] + [(s, True) for s in FP16_SOURCES]
@@ -79,6 +106,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [_nvcc(), "-shared", "-o", LIB] + objs + ["-gencode",
                "arch=compute_100a,code=sm_100a", "-ldl"]
         subprocess.run(cmd, check=True)
+    _build_torch_module(force)
     if verbose:
         for o in objs:
             with open(o + ".log") as f:

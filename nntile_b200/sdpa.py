@@ -22,6 +22,12 @@ import numpy as np
 import torch
 
 from . import _lib, ops
+try:
+    # the paged calls without the interpreter between the tensors and the library; what it
+    # does not take (and every mistake) goes the way through ops
+    from . import _paged_torch
+except ImportError:
+    _paged_torch = None
 
 
 def from_fortran(arr: np.ndarray, device="cuda") -> torch.Tensor:
@@ -509,6 +515,10 @@ def paged_append(pages, lengths, block_table, k, v, new_lens=None, status=None):
     of every sequence (the first new_lens[b] of them; default all).  Changes the pages, their
     scales and bounds, not `lengths` and `block_table`.  `status`: optional 32-bit word that
     receives NNTILE_B200_PAGED_BAD_* bits."""
+    if _paged_torch is not None:
+        done = _paged_torch.append(pages, lengths, block_table, k, v, new_lens, status)
+        if done is True:
+            return
     N, H, P, D = pages.k.shape
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[0] != H or shape[3] != D:
@@ -529,6 +539,10 @@ def paged_append(pages, lengths, block_table, k, v, new_lens=None, status=None):
 def paged_gather(pages, lengths, block_table, k, v, status=None):
     """Read the cache into k, v (kv_heads, batch, max_seq, head): rows 0 .. lengths[b] - 1 of
     every sequence; rows behind them are left as they are."""
+    if _paged_torch is not None:
+        done = _paged_torch.gather(pages, lengths, block_table, k, v, status)
+        if done is True:
+            return
     N, H, P, D = pages.k.shape
     shape = k.shape
     if len(shape) != 4 or shape != v.shape or shape[0] != H or shape[3] != D:
@@ -559,6 +573,11 @@ def paged_select(q, pages, lengths, block_table, num_selected, first_blocks=1, l
     """Blocks that the new token of every sequence attends to, per kv head: the first and the
     last ones and those whose bounds allow the highest score.  Returns int32 (kv_heads,
     batch, num_selected), ascending block numbers, then -1."""
+    if _paged_torch is not None:
+        done = _paged_torch.select(q, pages, lengths, block_table, num_selected, first_blocks,
+                                   last_blocks, out, workspace, status)
+        if isinstance(done, torch.Tensor):
+            return done
     N, H, P, D, G, B = _check_query(q, pages)
     if pages.bounds is None:
         raise ValueError("these pages keep no bounds")
@@ -584,6 +603,11 @@ def paged_decode(q, pages, lengths, block_table, selected=None, out=None, lse_ou
     sequence against its first lengths[b] positions, or against those of them in the blocks
     of `selected` (int32 (kv_heads, batch, num_selected), as paged_select returns).  Returns
     out shaped like q; lse_out: optional float32 (kv_heads, group, batch)."""
+    if _paged_torch is not None:
+        done = _paged_torch.decode(q, pages, lengths, block_table, selected, out, lse_out,
+                                   workspace, status)
+        if isinstance(done, torch.Tensor):
+            return done
     N, H, P, D, G, B = _check_query(q, pages)
     M, S = _check_table(lengths, block_table, B), 0
     _check_status(status)
