@@ -147,6 +147,41 @@ __device__ __forceinline__ int checked_page(const int32_t *table, int n, int num
     return page;
 }
 
+// Chained launches.  A kernel of this family may be set up while the one before it in the
+// stream still runs; it touches memory only after chain_wait(), which returns when everything
+// before it is complete and visible, and only then lets the next one be set up.  So whatever
+// starts early starts after all but the last kernel before it are complete: what that one
+// does not write (for the second kernel of a call: lengths and tables) may be read before the
+// wait, the rest only after it.  Every kernel waits, also in blocks with nothing to do: a
+// grid must not end before the one it is chained to.
+__device__ __forceinline__ void chain_wait()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template<typename... P, typename... A>
+inline int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+        cudaStream_t s, A... args)
+{
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) != cudaSuccess)
+    {
+        cudaGetLastError();
+        return NNTILE_B200_E_LAUNCH;
+    }
+    return launch_status();
+}
+
 // Sizes every paged entry point shares.  max_blocks*page_size positions are addressed
 // with 32-bit integers; byte offsets into the pool are 64-bit everywhere.
 inline int check_paged(int64_t head, int64_t page_size, int64_t num_pages, int64_t max_blocks,

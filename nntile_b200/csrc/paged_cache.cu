@@ -223,6 +223,7 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     const int unit = blockIdx.x/touched, j = blockIdx.x - unit*touched;
     const int b = unit % batch, kvh = unit/batch;
     const int capacity = max_blocks*page_size;
+    chain_wait();
     const int start = checked_length(lengths, b, capacity, status);
     bool bad = false;
     const int count = held_count(new_lens ? new_lens[b] : new_seq, new_seq, start, capacity, bad);
@@ -391,6 +392,7 @@ paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     const int slot = threadIdx.x/LPR;
     const int unit = blockIdx.x/chunks, chunk = blockIdx.x - unit*chunks;
     const int b = unit % batch, kvh = unit/batch;
+    chain_wait();
     int len = checked_length(lengths, b, max_blocks*page_size, status);
     if(len > max_seq)
     {
@@ -511,8 +513,8 @@ static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
             (unsigned)(2*((most + PART_ROWS - 1)/PART_ROWS)));
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
-#define NB200_APPEND(E, V, L) paged_append_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
-        (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
+#define NB200_APPEND(E, V, L) return launch_chained(paged_append_kernel<T, E, V, L>, grid, \
+        ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
         (int)new_seq, (int)touched, lengths, new_lens, block_table, (const T *)k, (const T *)v, \
         k_pages, v_pages, k_scales, v_scales, (T *)bounds, status)
 #define NB200_APPEND_L(E) \
@@ -526,7 +528,6 @@ static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     else NB200_APPEND_L(false);
 #undef NB200_APPEND_L
 #undef NB200_APPEND
-    return launch_status();
 }
 
 template<typename T>
@@ -566,8 +567,8 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     }
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
-#define NB200_GATHER(E, V, L) paged_gather_kernel<T, E, V, L><<<grid, ROW_THREADS, 0, s>>>( \
-        (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
+#define NB200_GATHER(E, V, L) return launch_chained(paged_gather_kernel<T, E, V, L>, grid, \
+        ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
         (int)max_seq, (int)rows_per_cta, (int)chunks, shift, lengths, block_table, k_pages, v_pages, \
         k_scales, v_scales, (T *)k, (T *)v, status)
 #define NB200_GATHER_L(E) \
@@ -581,7 +582,6 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     else NB200_GATHER_L(false);
 #undef NB200_GATHER_L
 #undef NB200_GATHER
-    return launch_status();
 }
 
 } // namespace nb200

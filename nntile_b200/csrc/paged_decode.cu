@@ -509,9 +509,6 @@ paged_decode_kernel(const PagedDecodeArgs a)
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
     const int tpb = P/PD_TILE;
 
-    // lets the joining kernel start its own preparations
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
     // columns behind the head are never copied: zero for good
     if(D < DP)
     {
@@ -522,6 +519,8 @@ paged_decode_kernel(const PagedDecodeArgs a)
         }
         __syncwarp();
     }
+
+    chain_wait();
 
     // ---- this worker's share: tiles [begin, end) of the row of all tiles
     int *prefix = reinterpret_cast<int *>(merge);
@@ -1253,8 +1252,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
     const int m = piece*128/(8*DP), off = piece*128 - m*8*DP + 4*lane;   // in the part's values
     const int head = off/DP, col = off - head*DP;
-    // before any return: the block's end must not come before the first kernel's
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    chain_wait();
     // one worker had it all and wrote it, or (the last block) there is no such unit
     const bool none = first == last || unit >= a.batch*HU;
     JoinState s = {-CUDART_INF_F, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
@@ -1404,28 +1402,16 @@ static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDeco
     {
         return NNTILE_B200_E_LAUNCH;
     }
-    paged_decode_kernel<T, E4M3, DP, MT><<<plan.grid, L::WARPS*32, L::SMEM, s>>>(a);
-    if(launch_status() != NNTILE_B200_OK) return NNTILE_B200_E_LAUNCH;
-    if(a.whole) return NNTILE_B200_OK;
+    const int st = launch_chained(paged_decode_kernel<T, E4M3, DP, MT>, dim3(plan.grid),
+            L::WARPS*32, L::SMEM, s, a);
+    if(st != NNTILE_B200_OK || a.whole) return st;
     // starts while the first kernel still runs and waits for its results on the device
     const int htiles = (a.group + 8*MT - 1)/(8*MT);
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
     const int wpp = a.wpw == 1 ? 1 : PD_JOIN_WARPS;
     const unsigned warps = (unsigned)a.batch*a.kv_heads*htiles*(MT*8*DP/128)*wpp;
-    cfg.gridDim = dim3((warps + PD_JOIN_WARPS - 1)/PD_JOIN_WARPS);
-    cfg.blockDim = dim3(PD_JOIN_WARPS*32);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, E4M3, DP, MT>, a, plan.grid, wpp) != cudaSuccess)
-    {
-        cudaGetLastError();
-        return NNTILE_B200_E_LAUNCH;
-    }
-    return launch_status();
+    return launch_chained(paged_join_kernel<T, E4M3, DP, MT>,
+            dim3((warps + PD_JOIN_WARPS - 1)/PD_JOIN_WARPS), PD_JOIN_WARPS*32, 0, s, a, plan.grid,
+            wpp);
 }
 
 template<typename T>

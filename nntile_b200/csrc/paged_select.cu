@@ -130,7 +130,7 @@ template<typename T>
 __global__ void __launch_bounds__(128)
 paged_score_generic_kernel(const PagedSelectArgs a)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    chain_wait();
     const int chunks = (a.max_blocks + 7)/8;
     const int unit = blockIdx.x/chunks;
     const int block = (blockIdx.x - unit*chunks)*8 + (threadIdx.x >> 4);
@@ -254,7 +254,6 @@ paged_score_kernel(const PagedSelectArgs a)
     using L = ScoreTile<DP>;
     constexpr int JN = DP/32, STAGES = L::STAGES, MT = WIDE ? 2 : 1;
     extern __shared__ __align__(128) uint8_t score_smem[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = lane >> 2, t = lane & 3;
     uint8_t *ring = score_smem + warp*STAGES*L::STAGE;
@@ -264,6 +263,7 @@ paged_score_kernel(const PagedSelectArgs a)
         reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     __syncwarp();
+    chain_wait();
 
     // ---- this warp's share of all tiles, and the sequence it begins in
     int total = 0;
@@ -538,9 +538,19 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ uint32_t low_s, high_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int unit = blockIdx.x, b = unit % a.batch, kvh = unit/a.batch;
+    // behind the scoring kernel the lengths are settled; as the first kernel of a call (a table
+    // that short is taken whole) this one has to wait for them
+    const bool scored = a.max_blocks > a.num_selected;
+    if(!scored)
+    {
+        chain_wait();
+    }
     const int n = filled_blocks(a, b, a.status), S = a.num_selected;
     int32_t *out = a.selected + (size_t)unit*S;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if(scored)
+    {
+        chain_wait();
+    }
     if(n <= S)
     {
         for(int i = tid; i < S; i += PICK_THREADS)
@@ -960,8 +970,8 @@ static int launch_score_as(cudaStream_t s, const PagedSelectArgs &a, unsigned gr
     {
         return NNTILE_B200_E_LAUNCH;
     }
-    paged_score_kernel<T, DP, WIDE><<<grid, ScoreTile<DP>::WARPS*32, ScoreTile<DP>::SMEM, s>>>(a);
-    return launch_status();
+    return launch_chained(paged_score_kernel<T, DP, WIDE>, dim3(grid), ScoreTile<DP>::WARPS*32,
+            ScoreTile<DP>::SMEM, s, a);
 }
 
 template<typename T, int DP>
@@ -991,25 +1001,11 @@ static int launch_pick(cudaStream_t s, const PagedSelectArgs &a)
     {
         return NNTILE_B200_E_LAUNCH;
     }
-    // starts while the scores are still being written and waits for them on the device
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = a.max_blocks > a.num_selected ? 1 : 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.batch*a.kv_heads);
-    cfg.blockDim = dim3(PICK_THREADS);
-    cfg.dynamicSmemBytes = cached ? (size_t)a.max_blocks*4 : 0;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t err = cached ? cudaLaunchKernelEx(&cfg, paged_pick_kernel<T, true>, a)
-            : cudaLaunchKernelEx(&cfg, paged_pick_kernel<T, false>, a);
-    if(err != cudaSuccess)
-    {
-        cudaGetLastError();
-        return NNTILE_B200_E_LAUNCH;
-    }
-    return launch_status();
+    // set up while the scores are still being written, and waits for them on the device
+    const dim3 grid((unsigned)a.batch*a.kv_heads);
+    return cached ? launch_chained(paged_pick_kernel<T, true>, grid, PICK_THREADS,
+                    (size_t)a.max_blocks*4, s, a)
+            : launch_chained(paged_pick_kernel<T, false>, grid, PICK_THREADS, 0, s, a);
 }
 
 template<typename T>
@@ -1076,8 +1072,8 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
         {
             const int64_t ctas = units*((max_blocks + 7)/8);
             if(ctas > INT32_MAX) return NNTILE_B200_E_SHAPE;
-            paged_score_generic_kernel<T><<<(unsigned)ctas, 128, 0, s>>>(a);
-            st2 = launch_status();
+            st2 = launch_chained(paged_score_generic_kernel<T>, dim3((unsigned)ctas), 128, 0, s,
+                    a);
         }
         if(st2 != NNTILE_B200_OK) return st2;
     }

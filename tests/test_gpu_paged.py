@@ -693,6 +693,69 @@ def test_captured_step_with_other_lengths_and_pages():
         assert torch.equal(dense, check_attention(q, pages, after, table)[0])
 
 
+def test_lengths_and_tables_written_just_before_each_call():
+    """Every call of a step reads what the kernel right before it in the stream has written
+    (lengths by an addition, table, rows and queries by copies), eagerly and in a graph whose
+    steps also fork to another stream."""
+    g = gen(25)
+    H, B, D, G, P, M = 2, 5, 64, 4, 16, 41                   # room for 656 positions
+    pages = make_pool(g, B*M, P, H, D, torch.bfloat16, False, bounds=True)
+    table = torch.randperm(B*M, generator=g, device="cuda", dtype=torch.int32).reshape(B, M)
+    zero = torch.zeros((), dtype=torch.int32, device="cuda")
+    real, lens, after, work = ints(300, 17, 620, 0, 95), ints(0, 0, 0, 0, 0), ints(0, 0, 0, 0, 0), \
+        torch.zeros_like(table)
+    k = randn(g, H, B, 1, D).bfloat16()
+    src = randn(g, H, G, B, 1, D).bfloat16()
+    q = torch.zeros_like(src)
+    out = [torch.zeros_like(src) for _ in range(3)]
+    sel = [torch.zeros((H, B, n), dtype=torch.int32, device="cuda") for n in (5, M)]
+    side = torch.cuda.Stream()
+
+    def step():
+        lens.copy_(real)
+        work.copy_(table)
+        paged_append(pages, lens, work, k, k)
+        torch.add(lens, zero + 1, out=after)
+        paged_decode(q, pages, after, work, out=out[0])         # of the queries before
+        q.copy_(src)
+        paged_select(q, pages, after, work, 5, 1, 1, out=sel[0])
+        paged_decode(q, pages, after, work, sel[0], out=out[1])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            paged_decode(q, pages, after, work, out=out[2])
+        after.add_(0)
+        paged_select(q, pages, after, work, M, 0, 0, out=sel[1])
+        torch.cuda.current_stream().wait_stream(side)
+        lens.zero_()
+        work.fill_(-1)
+        after.zero_()
+
+    def check():
+        ends = real + 1
+        assert torch.equal(sel[0], chosen(q, pages.bounds, ends, table, P, 5, 1, 1))
+        assert torch.equal(sel[1], chosen(q, pages.bounds, ends, table, P, M, 0, 0))
+        assert torch.equal(out[1], check_attention(src, pages, ends, table, sel[0])[0])
+        assert torch.equal(out[2], check_attention(src, pages, ends, table)[0])
+
+    for _ in range(3):
+        step()
+    torch.cuda.synchronize()
+    check()
+    assert torch.equal(out[0], out[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+        step()
+    for _ in range(3):
+        real += 7
+        real[3] = 0
+        src.copy_(randn(g, *src.shape))
+        graph.replay()
+        graph.replay()
+        check()
+        assert torch.equal(out[0], out[2])
+
+
 def test_offsets_past_32_bits():
     """Pages behind 4 GB of codes, 2^32 elements into the pool."""
     H, P, D = 8, 64, 128
