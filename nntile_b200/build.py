@@ -29,10 +29,11 @@ SOURCES = [
     "flash_fwd_sm100.cu", "flash_bwd_sm100.cu", "host_tensor.cu", "gemm_cublas.cu",
     "sdpa_prologue.cu", "paged_cache.cu", "paged_decode.cu", "paged_select.cu",
 ]
-# the fused-attention sources are compiled a second time for IEEE half (elem.cuh)
+# the fused-attention sources are compiled a second time for IEEE half (elem.cuh), and
+# paged_decode.cu, whose two row types take about 40 s each
 FP16_SOURCES = [
     "flash_generic.cu", "flash_api.cu", "flash_fwd_sm100.cu", "flash_bwd_sm100.cu",
-    "host_tensor.cu",
+    "host_tensor.cu", "paged_decode.cu",
 ]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -241,12 +241,19 @@ paged_decode_join_kernel(const PagedDecodeArgs a, int heads)
 constexpr int PD_SMS = 148;
 constexpr int PD_TILE = 16;                  // positions of a tile
 
+// Warps of a block, one block per SM: with four, 16-bit rows of 256 columns still have three
+// tiles (48 KB) a warp in the ring.
+__host__ __device__ constexpr int paged_warps(bool e4m3, int dp)
+{
+    return dp == 256 && !e4m3 ? 4 : 8;
+}
+
 // Layout of one kernel variant.  DP: head size rounded up to 64, 128 or 256 (columns behind
 // the head stay zero in the ring); MT: tiles of 8 query heads that share a pass.
 template<bool E4M3, int DP>
 struct PagedTile
 {
-    static constexpr int WARPS = DP == 256 ? 4 : 8;
+    static constexpr int WARPS = paged_warps(E4M3, DP);
     static constexpr int ROW_BYTES = DP*(E4M3 ? 1 : 2);
     static constexpr int CHUNKS = ROW_BYTES/16;          // 16-byte pieces of a row
     static constexpr int KV_BYTES = PD_TILE*ROW_BYTES;   // one of K, V
@@ -260,7 +267,9 @@ struct PagedTile
     static constexpr int AHEAD = STAGES - ABREAST;       // tiles in flight or waiting
     static_assert(AHEAD >= ABREAST, "the ring must hold what is consumed and what is coming");
     static constexpr int MBLK = DP/16;                   // 16-column blocks of the output
-    static constexpr int MERGE = WARPS*8*DP*4;           // one tile of 8 heads of every warp
+    // One tile of 8 heads of every warp, in two rounds where that is more than 32 KB.
+    static constexpr int ROUNDS = WARPS*8*DP*4 > 32768 ? 2 : 1;
+    static constexpr int MERGE = WARPS*8*DP*4/ROUNDS;
     static constexpr int SMEM = WARPS*STAGES*STAGE + MERGE;
 
     // Offset of piece c of row r.  A 128-byte line holds 8 pieces; which of them is piece c
@@ -425,13 +434,17 @@ __device__ __forceinline__ void write_part(const PagedDecodeArgs &a, bool comple
     for(int y = 0; y < 2; ++y)
     {
         const int g = 8*m + 2*t + y;
+        if(g >= heads)
+        {
+            continue;
+        }
         if(!complete)
         {
             float *o = a.part_o + (((size_t)part*MT + m)*8 + 2*t + y)*DP;
             o[L::column(i, 0, n)] = z[y];
             o[L::column(i, 1, n)] = z[2 + y];
         }
-        else if(g < heads)
+        else
         {
             const float inv = den[y] == 0.0f ? 0.0f : 1.0f/den[y];
             T *out = (T *)a.out + (((size_t)kvh*a.group + h0 + g)*a.batch + b)*a.head;
@@ -454,11 +467,15 @@ __device__ __forceinline__ void write_sums(const PagedDecodeArgs &a, bool comple
         int m, int head, float top, float sum, int kvh, int h0, int heads, int b)
 {
     const int g = 8*m + head;
+    if(g >= heads)
+    {
+        return;
+    }
     if(!complete)
     {
         a.part_sums[((size_t)part*MT + m)*8 + head] = make_float2(top, sum);
     }
-    else if(g < heads && a.lse_out)
+    else if(a.lse_out)
     {
         a.lse_out[((size_t)kvh*a.group + h0 + g)*a.batch + b] = sum == 0.0f ? -CUDART_INF_F
                 : ((top == -CUDART_INF_F ? 0.0f : top) + log2f(sum))*PD_LN2;
@@ -483,19 +500,20 @@ __host__ __device__ inline PagedShares paged_shares(int total, int blocks, int w
     return s;
 }
 
-template<typename T, bool E4M3, int DP, int MT>
+// EXACT: the head size is DP.
+template<typename T, bool E4M3, int DP, int MT, bool EXACT>
 __global__ void __launch_bounds__(PagedTile<E4M3, DP>::WARPS*32, 1)
 paged_decode_kernel(const PagedDecodeArgs a)
 {
     using L = PagedTile<E4M3, DP>;
     using M = typename std::conditional<E4M3, __half, T>::type;      // operand format
     constexpr bool HALF = std::is_same<M, __half>::value;
-    // A weight is exp2(score - reference), and the reference only moves when a score passes it
-    // by more than SLACK: weights stay below 2^SLACK and most tiles do without a maximum.
-    // fp16 weights are lifted by 2^LIFT, which keeps those down to 2^-34 of the reference;
-    // bf16 has fp32's range.
-    constexpr int LIFT = HALF ? 10 : 0;
-    constexpr float SLACK = 4.0f;
+    // A weight is exp2(score - reference).  The reference moves to LIFT below the largest score,
+    // and only when a score passes that by more than SLACK: weights stay below
+    // 2^(LIFT + SLACK) and most tiles do without a maximum.  fp16 weights are lifted to keep
+    // those down to 2^-34 of the largest; bf16 has fp32's range.
+    constexpr float LIFT = HALF ? 10.0f : 0.0f, SLACK = 4.0f;
+    constexpr float LOWEST = -3.0e38f;                   // no score yet
     constexpr int KSTEPS = DP/16, MBLK = L::MBLK, WARPS = L::WARPS, STAGES = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int nv_s[WARPS][STAGES];
@@ -505,7 +523,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
     const int n = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + warp*STAGES*L::STAGE;
     float *merge = reinterpret_cast<float *>(smem + WARPS*STAGES*L::STAGE);
-    const int D = a.head, P = a.page_size;
+    const int D = EXACT ? DP : a.head, P = a.page_size;
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
     const int tpb = P/PD_TILE;
 
@@ -600,12 +618,13 @@ paged_decode_kernel(const PagedDecodeArgs a)
     int ileft = end - begin > slot0 ? (end - begin - slot0 + step - 1)/step : 0;
     int ilen = held_len(a, ib), int_ = unit_tiles(a, ilen);
     int ipos = 32;                                       // used up: look up at once
-    int look_nv = 0;
-    long long look_row = 0;
-    const int elt = E4M3 ? 1 : (int)sizeof(T);
-    const int row_bytes = D*elt, chunks = row_bytes/16;
+    uint32_t look = 0;                                   // first row/16 << 5 | rows filled
+    const int row_bytes = EXACT ? L::ROW_BYTES : D*(E4M3 ? 1 : (int)sizeof(T));
+    const int chunks = row_bytes/16;
     constexpr int RPP = 32/L::CHUNKS > 0 ? 32/L::CHUNKS : 1;     // rows a warp copies at once
     const int crow = lane/L::CHUNKS, cchunk = lane % L::CHUNKS;
+    const uint8_t *k_lane = (const uint8_t *)a.k_pages + crow*row_bytes + cchunk*16;
+    const uint8_t *v_lane = (const uint8_t *)a.v_pages + crow*row_bytes + cchunk*16;
 
     auto issue = [&](int stage)
     {
@@ -626,8 +645,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
             {
                 // pages of this warp's next 32 tiles in the sequence
                 ipos = 0;
-                look_nv = 0;
-                look_row = 0;
+                look = 0;
                 const long long x = ix + (long long)lane*step;
                 if(x < (long long)int_*HU && lane < ileft)
                 {
@@ -651,33 +669,48 @@ paged_decode_kernel(const PagedDecodeArgs a)
                                 + (size_t)ib*a.max_blocks, block, a.num_pages, a.status) : -1;
                         if(page >= 0)
                         {
-                            look_nv = min(left, PD_TILE);
-                            look_row = ((long long)page*a.kv_heads + kvh)*P + sub;
+                            const uint32_t row = ((uint32_t)page*(uint32_t)a.kv_heads + kvh)
+                                    *(uint32_t)P + sub;
+                            look = row/PD_TILE << 5 | (uint32_t)min(left, PD_TILE);
                         }
                     }
                 }
             }
-            const int nv = __shfl_sync(0xffffffffu, look_nv, ipos);
-            const long long row = __shfl_sync(0xffffffffu, look_row, ipos);
+            const uint32_t here = __shfl_sync(0xffffffffu, look, ipos);
+            const int nv = (int)(here & 31u);
+            const uint32_t row = (here >> 5)*PD_TILE;
             if(lane == 0)
             {
                 nv_s[warp][stage] = nv;
             }
-            // rows behind the length, and all of a tile without a page, are filled with zeros
             const uint32_t dst = smem_addr(ring + stage*L::STAGE);
-            const long long at = row*row_bytes + crow*row_bytes + cchunk*16;
-            const uint8_t *ks = (const uint8_t *)a.k_pages + at;
-            const uint8_t *vs = (const uint8_t *)a.v_pages + at;
-            if(cchunk < chunks)
+            const uint8_t *ks = k_lane + (size_t)row*row_bytes;
+            const uint8_t *vs = v_lane + (size_t)row*row_bytes;
+            if(nv == PD_TILE)
             {
+                if(EXACT || cchunk < chunks)
+                {
+#pragma unroll
+                    for(int i = 0; i < PD_TILE/RPP; ++i)
+                    {
+                        copy16(dst + L::offset(crow + i*RPP, cchunk, E4M3),
+                                ks + i*RPP*row_bytes, 16);
+                        copy16(dst + L::KV_BYTES + L::offset(crow + i*RPP, cchunk, false),
+                                vs + i*RPP*row_bytes, 16);
+                    }
+                }
+            }
+            else if(EXACT || cchunk < chunks)
+            {
+                // rows behind the length, and all of a tile without a page: zeros
 #pragma unroll
                 for(int i = 0; i < PD_TILE/RPP; ++i)
                 {
-                    const int r = crow + i*RPP;
-                    const int bytes = r < nv ? 16 : 0;
-                    copy16(dst + L::offset(r, cchunk, E4M3), ks + (size_t)i*RPP*row_bytes, bytes);
-                    copy16(dst + L::KV_BYTES + L::offset(r, cchunk, false),
-                            vs + (size_t)i*RPP*row_bytes, bytes);
+                    const int bytes = crow + i*RPP < nv ? 16 : 0;
+                    copy16(dst + L::offset(crow + i*RPP, cchunk, E4M3), ks + i*RPP*row_bytes,
+                            bytes);
+                    copy16(dst + L::KV_BYTES + L::offset(crow + i*RPP, cchunk, false),
+                            vs + i*RPP*row_bytes, bytes);
                 }
             }
             if(E4M3 && lane < 2)
@@ -691,10 +724,10 @@ paged_decode_kernel(const PagedDecodeArgs a)
         }
         copy_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for(int s = 0; s < L::AHEAD; ++s)
     {
-        issue(s);
+        issue(s);                                        // once in the code: it is long
     }
 
     // ---- consuming side, unit by unit
@@ -768,7 +801,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
         for(int m = 0; m < MT; ++m)
         {
-            top[m][0] = top[m][1] = -CUDART_INF_F;
+            top[m][0] = top[m][1] = LOWEST;
             sum[m][0] = sum[m][1] = 0.0f;
 #pragma unroll
             for(int i = 0; i < MBLK; ++i)
@@ -782,29 +815,32 @@ paged_decode_kernel(const PagedDecodeArgs a)
 
         // N tiles at once.  Keys and values are the 16-row operand, the query heads the 8
         // columns: this lane holds the scores of positions n and n + 8 of a tile for heads 2t
-        // and 2t + 1, in the order [2*(position >= 8) + (head odd)].
-        auto process = [&](auto tiles)
+        // and 2t + 1, in the order [2*(position >= 8) + (head odd)].  FULL: all 16 rows of every
+        // tile are filled.
+        auto process = [&](auto tiles, auto filled)
         {
             constexpr int N = decltype(tiles)::value;
-            copy_wait<L::AHEAD - L::ABREAST>();
-            __syncwarp();
-            // what was consumed last is free for every lane now
+            constexpr bool FULL = decltype(filled)::value;
             const uint8_t *st[N];
-            int nv[N], some = 0;
+            int nv[N];
+            int to = stage + L::AHEAD;
+            to -= to >= STAGES ? STAGES : 0;
+#pragma unroll 1
+            for(int j = 0; j < N; ++j)
+            {
+                issue(to);
+                to = to + 1 == STAGES ? 0 : to + 1;
+            }
 #pragma unroll
             for(int j = 0; j < N; ++j)
             {
-                int to = stage + L::AHEAD;
-                to -= to >= STAGES ? STAGES : 0;
-                issue(to);
                 st[j] = ring + stage*L::STAGE;
-                nv[j] = nv_s[warp][stage];
-                some |= nv[j];
+                nv[j] = FULL ? PD_TILE : nv_s[warp][stage];
                 stage = stage + 1 == STAGES ? 0 : stage + 1;
             }
-            if(some == 0)
+            if(!FULL && nv[0] == 0)
             {
-                return;
+                return;                                  // N = 1
             }
             // ---- scores, in two sums of every other step: half as long a chain
             float s[MT][N][2][4];
@@ -866,23 +902,31 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         }
                 }
             }
-            float kscale[N][2];
+            // factors of the scores, by position and head
+            float factor[MT][N][2][2];
             int vbyte[N][2];
             bool moved = false;
-            if(E4M3)
-            {
 #pragma unroll
-                for(int j = 0; j < N; ++j)
+            for(int j = 0; j < N; ++j)
 #pragma unroll
-                    for(int h = 0; h < 2; ++h)
+                for(int h = 0; h < 2; ++h)
+                {
+                    float kscale = 1.0f;
+                    if(E4M3)
                     {
-                        // the scale of a row behind the length may be anything: keep it out
                         const uint8_t *sc = st[j] + 2*L::KV_BYTES + 8*h + n;
-                        kscale[j][h] = scale_value(sc[0]);
-                        vbyte[j][h] = 8*h + n < nv[j] ? (int)sc[PD_TILE] : 0;
+                        kscale = __uint_as_float((uint32_t)sc[0] << 23);
+                        // the scale of a row behind the length may be anything: keep it out
+                        vbyte[j][h] = FULL || 8*h + n < nv[j] ? (int)sc[PD_TILE] : 0;
                         moved = moved || vbyte[j][h] > vref;
                     }
-            }
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+#pragma unroll
+                        for(int y = 0; y < 2; ++y)
+                            factor[m][j][h][y] = E4M3 ? qscale[m][y]*kscale : qscale[m][y];
+                }
+            // d = score - reference, in the place of the first sum
 #pragma unroll
             for(int m = 0; m < MT; ++m)
 #pragma unroll
@@ -890,14 +934,15 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                     for(int r = 0; r < 4; ++r)
                     {
-                        float z = (s[m][j][0][r] + s[m][j][1][r])*qscale[m][r & 1];
-                        if(E4M3)
+                        s[m][j][1][r] += s[m][j][0][r];
+                        float d = fmaf(s[m][j][1][r], factor[m][j][r >> 1][r & 1],
+                                -top[m][r & 1]);
+                        if(!FULL)
                         {
-                            z *= kscale[j][r >> 1];
+                            d = 8*(r >> 1) + n < nv[j] ? d : -CUDART_INF_F;
                         }
-                        z = 8*(r >> 1) + n < nv[j] ? z : -CUDART_INF_F;
-                        s[m][j][0][r] = z;
-                        moved = moved || z > top[m][r & 1] + SLACK;
+                        s[m][j][0][r] = d;
+                        moved = moved || d > LIFT + SLACK;
                     }
             if(__any_sync(0xffffffffu, moved))
             {
@@ -912,7 +957,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
                     }
                     vtop = __reduce_max_sync(0xffffffffu, vtop);
                     const int e = vref - vtop + 127;
-                    back = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
+                    back = __uint_as_float((uint32_t)max(e, 0) << 23);
                     vref = vtop;
                 }
 #pragma unroll
@@ -922,21 +967,34 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                     for(int y = 0; y < 2; ++y)
                     {
-                        float ntop = top[m][y];
+                        float ntop = -CUDART_INF_F;
 #pragma unroll
                         for(int j = 0; j < N; ++j)
-                        {
-                            ntop = fmaxf(ntop, fmaxf(s[m][j][0][y], s[m][j][0][2 + y]));
-                        }
+#pragma unroll
+                            for(int h = 0; h < 2; ++h)
+                                if(FULL || 8*h + n < nv[j])
+                                {
+                                    ntop = fmaxf(ntop, s[m][j][1][2*h + y]*factor[m][j][h][y]);
+                                }
 #pragma unroll
                         for(int o = 4; o < 32; o <<= 1)
                         {
                             ntop = fmaxf(ntop, __shfl_xor_sync(0xffffffffu, ntop, o));
                         }
+                        ntop = fmaxf(top[m][y], ntop - LIFT);
                         const float shrink = ntop == top[m][y] ? 1.0f : ex2(top[m][y] - ntop);
                         top[m][y] = ntop;
                         sum[m][y] *= shrink;
                         f[y] = shrink*back;
+#pragma unroll
+                        for(int j = 0; j < N; ++j)
+#pragma unroll
+                            for(int h = 0; h < 2; ++h)
+                                if(FULL || 8*h + n < nv[j])
+                                {
+                                    s[m][j][0][2*h + y] = fmaf(s[m][j][1][2*h + y],
+                                            factor[m][j][h][y], -ntop);
+                                }
                     }
 #pragma unroll
                     for(int i = 0; i < MBLK; ++i)
@@ -952,12 +1010,9 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                 for(int h = 0; h < 2; ++h)
                 {
-                    float lift = (float)(1 << LIFT);
-                    if(E4M3)
-                    {
-                        const int e = vbyte[j][h] - vref + 127 + LIFT;
-                        lift = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.0f;
-                    }
+                    // 2^(scale of the row - scale of the accumulators), 0 when far below
+                    const float rel = E4M3 ? __uint_as_float((uint32_t)max(vbyte[j][h] - vref + 127,
+                            0) << 23) : 1.0f;
 #pragma unroll
                     for(int m = 0; m < MT; ++m)
                     {
@@ -965,13 +1020,11 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                         for(int y = 0; y < 2; ++y)
                         {
-                            // no finite score yet: every weight is exp2(-inf) = 0
-                            const float ref = top[m][y] == -CUDART_INF_F ? 0.0f : top[m][y];
-                            p[y] = ex2(s[m][j][0][2*h + y] - ref);
+                            p[y] = ex2(s[m][j][0][2*h + y]);
                             sum[m][y] += p[y];
-                            if(HALF)
+                            if(E4M3)
                             {
-                                p[y] *= lift;
+                                p[y] *= rel;
                             }
                         }
                         const uint32_t up = pack2<M>(p[0], p[1]);
@@ -1056,15 +1109,30 @@ paged_decode_kernel(const PagedDecodeArgs a)
         };
         while(mine < seg_end)
         {
-            if(L::ABREAST > 1 && mine + (L::ABREAST - 1)*step < seg_end)
+            copy_wait<L::AHEAD - L::ABREAST>();
+            // every lane's copies are there, and what was consumed last is free
+            __syncwarp();
+            bool full = L::ABREAST > 1 && mine + (L::ABREAST - 1)*step < seg_end;
+            int at = stage;
+#pragma unroll
+            for(int j = 0; j < L::ABREAST; ++j)
+            {
+                full = full && nv_s[warp][at] == PD_TILE;
+                at = at + 1 == STAGES ? 0 : at + 1;
+            }
+            if(L::ABREAST == 1)
+            {
+                full = nv_s[warp][stage] == PD_TILE;
+            }
+            if(full)
             {
                 mine += L::ABREAST*step;
-                process(std::integral_constant<int, L::ABREAST>());
+                process(std::integral_constant<int, L::ABREAST>(), std::true_type());
             }
             else
             {
                 mine += step;
-                process(std::integral_constant<int, 1>());
+                process(std::integral_constant<int, 1>(), std::false_type());
             }
         }
 
@@ -1072,7 +1140,6 @@ paged_decode_kernel(const PagedDecodeArgs a)
         // this share's part of it
         const bool complete = x == unit_begin && seg_end == unit_end;
         const int part = 2*worker + (x == unit_begin ? 1 : 0);
-        const float drop = HALF ? 1.0f/(float)(1 << LIFT) : 1.0f;
         const float vscale = E4M3 ? scale_value((uint32_t)vref) : 1.0f;
 #pragma unroll
         for(int m = 0; m < MT; ++m)
@@ -1088,7 +1155,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
             for(int i = 0; i < MBLK; ++i)
 #pragma unroll
                 for(int r = 0; r < 4; ++r)
-                    acc[m][i][r] = acc[m][i][r]*drop*vscale;
+                    acc[m][i][r] *= vscale;
             if(wpw > 1)
             {
                 if(n == 0)
@@ -1100,55 +1167,67 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         sum_s[warp][2*t + y] = sum[m][y];
                     }
                 }
-                float *mw = merge + warp*8*DP;
-#pragma unroll
-                for(int i = 0; i < MBLK; ++i)
-#pragma unroll
-                    for(int r = 0; r < 4; ++r)
-                        mw[(4*i + r)*32 + lane] = acc[m][i][r];
-                __syncthreads();
-                // every warp joins its share of the blocks, same lanes, same heads
                 float big[2], den[2], wgt[WARPS][2];
+                constexpr int ROUND = MBLK/L::ROUNDS;        // blocks a round
+                float *mw = merge + warp*ROUND*128;
 #pragma unroll
-                for(int y = 0; y < 2; ++y)
+                for(int q = 0; q < L::ROUNDS; ++q)
                 {
-                    big[y] = -CUDART_INF_F;
-                    den[y] = 0.0f;
 #pragma unroll
-                    for(int w = 0; w < WARPS; ++w)
-                    {
-                        big[y] = fmaxf(big[y], top_s[w][2*t + y]);
-                    }
-                    const float ref = big[y] == -CUDART_INF_F ? 0.0f : big[y];
-#pragma unroll
-                    for(int w = 0; w < WARPS; ++w)
-                    {
-                        wgt[w][y] = ex2(top_s[w][2*t + y] - ref);
-                        den[y] = fmaf(wgt[w][y], sum_s[w][2*t + y], den[y]);
-                    }
-                }
-                // fewer blocks than warps (64 columns): the upper warps have none
-                constexpr int MY = (MBLK + WARPS - 1)/WARPS;
-#pragma unroll
-                for(int k = 0; k < MY; ++k)
-                {
-                    const int i = warp*MY + k;
-                    if(i < MBLK)
-                    {
-                        float z[4];
+                    for(int i = 0; i < ROUND; ++i)
 #pragma unroll
                         for(int r = 0; r < 4; ++r)
+                            mw[(4*i + r)*32 + lane] = acc[m][q*ROUND + i][r];
+                    __syncthreads();
+                    if(q == 0)
+                    {
+#pragma unroll
+                        for(int y = 0; y < 2; ++y)
                         {
-                            z[r] = 0.0f;
+                            big[y] = -CUDART_INF_F;
+                            den[y] = 0.0f;
 #pragma unroll
                             for(int w = 0; w < WARPS; ++w)
                             {
-                                z[r] = fmaf(wgt[w][r & 1], merge[w*8*DP + (4*i + r)*32 + lane],
-                                        z[r]);
+                                big[y] = fmaxf(big[y], top_s[w][2*t + y]);
+                            }
+                            const float ref = big[y] == -CUDART_INF_F ? 0.0f : big[y];
+#pragma unroll
+                            for(int w = 0; w < WARPS; ++w)
+                            {
+                                wgt[w][y] = ex2(top_s[w][2*t + y] - ref);
+                                den[y] = fmaf(wgt[w][y], sum_s[w][2*t + y], den[y]);
                             }
                         }
-                        write_part<T, E4M3, DP, MT>(a, complete, part, m, lane, i, z, den, kvh,
-                                h0, heads, b);
+                    }
+                    // every warp joins its share of the blocks, same lanes, same heads; with
+                    // fewer blocks than warps the upper ones have none
+                    constexpr int MY = (ROUND + WARPS - 1)/WARPS;
+#pragma unroll
+                    for(int k = 0; k < MY; ++k)
+                    {
+                        const int i = warp*MY + k;
+                        if(i < ROUND)
+                        {
+                            float z[4];
+#pragma unroll
+                            for(int r = 0; r < 4; ++r)
+                            {
+                                z[r] = 0.0f;
+#pragma unroll
+                                for(int w = 0; w < WARPS; ++w)
+                                {
+                                    z[r] = fmaf(wgt[w][r & 1],
+                                            merge[(w*ROUND*4 + 4*i + r)*32 + lane], z[r]);
+                                }
+                            }
+                            write_part<T, E4M3, DP, MT>(a, complete, part, m, lane,
+                                    q*ROUND + i, z, den, kvh, h0, heads, b);
+                        }
+                    }
+                    if(q + 1 < L::ROUNDS)
+                    {
+                        __syncthreads();
                     }
                 }
                 if(warp == 0 && n == 0)
@@ -1199,10 +1278,15 @@ paged_decode_kernel(const PagedDecodeArgs a)
 }
 
 // Joins the parts of the units that fell into several shares, and answers those with
-// nothing to attend to.  A piece is 128 of the 8*DP values of 8 heads, four neighbouring
-// columns a lane; `wpp` warps share the parts of a piece and meet in shared memory: one warp
-// while units are many and their parts few, eight when a few units have many parts each.
+// nothing to attend to.  A piece is 128 columns of a unit's heads, four neighbouring ones a
+// lane; `wpp` warps share the parts of a piece and meet in shared memory: one warp while
+// units are many and their parts few, up to eight when a few units have many parts each.
 constexpr int PD_JOIN_WARPS = 8;
+
+__host__ __device__ inline int join_pieces(int heads, int dp)
+{
+    return (heads*dp + 127)/128;
+}
 
 struct JoinState                         // four values of a head, not yet divided by the sum
 {
@@ -1228,13 +1312,13 @@ __global__ void __launch_bounds__(PD_JOIN_WARPS*32)
 paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
 {
     using L = PagedTile<E4M3, DP>;
-    constexpr int PIECES = MT*8*DP/128;
+    const int pieces = join_pieces(min(8*MT, a.group), DP);
     __shared__ float2 sums_s[PD_JOIN_WARPS][32];
     __shared__ float4 o_s[PD_JOIN_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
     const int id = (blockIdx.x*PD_JOIN_WARPS + warp)/wpp;
-    const int unit = id/PIECES, piece = id - unit*PIECES;
+    const int unit = id/pieces, piece = id - unit*pieces;
     const int b = min(unit/HU, a.batch - 1), hu = unit - b*HU;
     // tiles of all sequences, and of those before this one
     int total = 0, before = 0;
@@ -1252,22 +1336,36 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
     const int m = piece*128/(8*DP), off = piece*128 - m*8*DP + 4*lane;   // in the part's values
     const int head = off/DP, col = off - head*DP;
+    const int kvh = hu/htiles, g = (hu - kvh*htiles)*8*MT + 8*m + head;
     chain_wait();
-    // one worker had it all and wrote it, or (the last block) there is no such unit
-    const bool none = first == last || unit >= a.batch*HU;
+    // one worker had it all and wrote it, or there is no such head, or (the last block) unit
+    const bool none = first == last || g >= a.group || unit >= a.batch*HU;
     JoinState s = {-CUDART_INF_F, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
     if(!none)
     {
         // the first share holds the unit's beginning in its second part, the others in their
         // first
         const int parts = last - first + 1;
-#pragma unroll 4
-        for(int i = warp % wpp; i < parts; i += wpp)
+        for(int i0 = warp % wpp; i0 < parts; i0 += 4*wpp)
         {
-            const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
-            const float2 ts = a.part_sums[(p*MT + m)*8 + head];
-            const float4 o = *reinterpret_cast<const float4 *>(a.part_o + (p*MT + m)*8*DP + off);
-            join_add(s, ts.x, ts.y, o);
+            // four at a time: the loads' latency is what this costs
+            float2 ts[4];
+            float4 o[4];
+#pragma unroll
+            for(int u = 0; u < 4; ++u)
+            {
+                const int i = i0 + u*wpp;
+                const size_t p = 2*(size_t)(first + i) + (i == 0 ? 1 : 0);
+                const bool on = i < parts;
+                ts[u] = on ? a.part_sums[(p*MT + m)*8 + head] : make_float2(-CUDART_INF_F, 0.0f);
+                o[u] = on ? *reinterpret_cast<const float4 *>(a.part_o + (p*MT + m)*8*DP + off)
+                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for(int u = 0; u < 4; ++u)
+            {
+                join_add(s, ts[u].x, ts[u].y, o[u]);
+            }
         }
     }
     if(wpp > 1)
@@ -1289,25 +1387,21 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     {
         return;
     }
-    const int kvh = hu/htiles, g = (hu - kvh*htiles)*8*MT + 8*m + head;
-    if(g < a.group)
-    {
-        const size_t qh = ((size_t)kvh*a.group + g)*a.batch + b;
-        const float inv = s.sum == 0.0f ? 0.0f : 1.0f/s.sum;
-        const float v[4] = {s.o.x, s.o.y, s.o.z, s.o.w};
+    const size_t qh = ((size_t)kvh*a.group + g)*a.batch + b;
+    const float inv = s.sum == 0.0f ? 0.0f : 1.0f/s.sum;
+    const float v[4] = {s.o.x, s.o.y, s.o.z, s.o.w};
 #pragma unroll
-        for(int i = 0; i < 4; ++i)
+    for(int i = 0; i < 4; ++i)
+    {
+        if(col + i < a.head)
         {
-            if(col + i < a.head)
-            {
-                ((T *)a.out)[qh*a.head + col + i] = from_f<T>(v[i]*inv);
-            }
+            ((T *)a.out)[qh*a.head + col + i] = from_f<T>(v[i]*inv);
         }
-        if(a.lse_out && col == 0)
-        {
-            a.lse_out[qh] = s.sum == 0.0f ? -CUDART_INF_F
-                    : ((s.top == -CUDART_INF_F ? 0.0f : s.top) + log2f(s.sum))*PD_LN2;
-        }
+    }
+    if(a.lse_out && col == 0)
+    {
+        a.lse_out[qh] = s.sum == 0.0f ? -CUDART_INF_F
+                : ((s.top == -CUDART_INF_F ? 0.0f : s.top) + log2f(s.sum))*PD_LN2;
     }
 }
 
@@ -1337,10 +1431,11 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
     const int64_t unit_tiles = listed*(page_size/PD_TILE);
     const int64_t units = batch*kv_heads*htiles;
     p.fast = page_size % PD_TILE == 0 && head % (e4m3 ? 16 : 8) == 0 && batch < 4096
-            && unit_tiles*units < (int64_t)1 << 30 && units < (int64_t)1 << 24 && num_pages > 0;
+            && unit_tiles*units < (int64_t)1 << 30 && units < (int64_t)1 << 24
+            && num_pages > 0 && num_pages*kv_heads*page_size < (int64_t)1 << 31;
     if(p.fast)
     {
-        const int warps = p.dp == 256 ? 4 : 8;
+        const int warps = paged_warps(e4m3, p.dp);
         const int64_t total = unit_tiles*units;
         // Workers are warps when there are units enough for most of a warp's share to be of
         // one or two of them; with fewer units the warps of a block work together, which
@@ -1388,27 +1483,37 @@ static size_t paged_decode_bytes(int64_t head, int64_t page_size, int64_t max_bl
     return most;
 }
 
-template<typename T, bool E4M3, int DP, int MT>
-static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDecodePlan &plan)
+template<typename T, bool E4M3, int DP, int MT, bool EXACT>
+static int launch_main(cudaStream_t s, const PagedDecodeArgs &a, const PagedDecodePlan &plan)
 {
     using L = PagedTile<E4M3, DP>;
     static PerDeviceOnce once;
     int dev = -1;
     if(cudaGetDevice(&dev) != cudaSuccess || !once.ensure(dev, []
     {
-        return cudaFuncSetAttribute(paged_decode_kernel<T, E4M3, DP, MT>,
+        return cudaFuncSetAttribute(paged_decode_kernel<T, E4M3, DP, MT, EXACT>,
                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) == cudaSuccess;
     }))
     {
         return NNTILE_B200_E_LAUNCH;
     }
-    const int st = launch_chained(paged_decode_kernel<T, E4M3, DP, MT>, dim3(plan.grid),
+    return launch_chained(paged_decode_kernel<T, E4M3, DP, MT, EXACT>, dim3(plan.grid),
             L::WARPS*32, L::SMEM, s, a);
+}
+
+template<typename T, bool E4M3, int DP, int MT>
+static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDecodePlan &plan)
+{
+    const int st = a.head == DP ? launch_main<T, E4M3, DP, MT, true>(s, a, plan)
+            : launch_main<T, E4M3, DP, MT, false>(s, a, plan);
     if(st != NNTILE_B200_OK || a.whole) return st;
     // starts while the first kernel still runs and waits for its results on the device
     const int htiles = (a.group + 8*MT - 1)/(8*MT);
-    const int wpp = a.wpw == 1 ? 1 : PD_JOIN_WARPS;
-    const unsigned warps = (unsigned)a.batch*a.kv_heads*htiles*(MT*8*DP/128)*wpp;
+    // warps a piece: about as many as it has parts by fours, were the lengths even; with
+    // uneven ones a unit may have more, so never one alone when blocks are the workers
+    const int wpp = a.wpw == 1 ? 1 : plan.grid <= 3*a.batch*a.kv_heads*htiles ? 4 : PD_JOIN_WARPS;
+    const unsigned warps = (unsigned)a.batch*a.kv_heads*htiles
+            *join_pieces(std::min(8*MT, a.group), DP)*wpp;
     return launch_chained(paged_join_kernel<T, E4M3, DP, MT>,
             dim3((warps + PD_JOIN_WARPS - 1)/PD_JOIN_WARPS), PD_JOIN_WARPS*32, 0, s, a, plan.grid,
             wpp);
@@ -1481,7 +1586,7 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.part_o = static_cast<float *>(workspace);
     a.part_lse = a.part_o + (size_t)heads*plan.nsplit*(size_t)head;      // generic kernel
     a.part_sums = reinterpret_cast<float2 *>(a.part_o + (plan.fast
-            ? (size_t)2*plan.grid*(plan.dp == 256 ? 4 : 8)*plan.mt*8*plan.dp : 0));
+            ? (size_t)2*plan.grid*paged_warps(e4m3, plan.dp)*plan.mt*8*plan.dp : 0));
     a.wpw = plan.wpw;
     a.whole = plan.whole;
     a.status = status;
@@ -1521,6 +1626,8 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
 
 using namespace nb200;
 
+// Compiled twice, once per row type (-DNB200_FP16), to keep the build short.
+#ifndef NB200_FP16
 extern "C" size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, int64_t page_size,
         int64_t max_blocks, int64_t batch, int64_t group, int64_t kv_heads, int64_t num_selected)
 {
@@ -1532,6 +1639,8 @@ extern "C" size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, in
     }
     return paged_decode_bytes(head, page_size, max_blocks, batch, group, kv_heads, num_selected);
 }
+
+#endif // NB200_FP16
 
 #define NB200_PAGED_DECODE_ENTRY(SFX, T) \
 extern "C" int nntile_b200_paged_decode_sdpa_##SFX(nntile_b200_stream_t stream, int64_t head, \
@@ -1547,5 +1656,8 @@ extern "C" int nntile_b200_paged_decode_sdpa_##SFX(nntile_b200_stream_t stream, 
             v_pages, k_scales, v_scales, out, lse_out, workspace, workspace_bytes, status); \
 }
 
-NB200_PAGED_DECODE_ENTRY(bf16, bf16)
+#ifdef NB200_FP16
 NB200_PAGED_DECODE_ENTRY(fp16, __half)
+#else
+NB200_PAGED_DECODE_ENTRY(bf16, bf16)
+#endif
