@@ -138,12 +138,9 @@ paged_score_generic_kernel(const PagedSelectArgs a)
     const bool live = block < filled_blocks(a, b, a.status);
     const int page = live ? checked_page(a.block_table + (size_t)b*a.max_blocks, block,
             a.num_pages, a.status) : -1;
-    if(a.num_pages == 0)
-    {
-        return;                                  // no bounds to read; the whole grid
-    }
     unsigned long long key = 0ull;
-    for(int g = 0; g < a.group; ++g)
+    // without a pool there are no bounds to read, not even by lanes that only keep step
+    for(int g = 0; g < (a.num_pages > 0 ? a.group : 0); ++g)
     {
         const unsigned long long one = exact_key<T>(a, kvh, b, max(page, 0), g);
         key = one > key ? one : key;

@@ -325,9 +325,9 @@ class Sdpa:
         lengths agree; otherwise the unfused chain.  ``mask`` is what the
         constructor takes for the chosen path.
 
-        Beyond the reference: with ``kv_cache`` (a KVCache holding the un-replicated
-        keys and values) and a single query position, the split-KV decode kernel
-        reads the filled part of the cache in place; k and v are then ignored."""
+        Beyond the reference: with ``kv_cache`` (a KVCache or PagedKVCache holding the
+        un-replicated keys and values) and a single query position, the split-KV decode
+        kernel reads the filled part of the cache in place; k and v are then ignored."""
         H, G, B, Sq, D = q.shape
         if kv_cache is not None and Sq == 1 and len(kv_cache) > 0:
             return kv_cache.decode(q)
@@ -684,18 +684,22 @@ class PagedKVCache:
         if sum(more) > len(self._free):
             raise ValueError(f"the pool has {len(self._free)} free pages, {sum(more)} are needed")
         device = self.lengths.device
-        entries = []
+        left = len(self._free) - sum(more)
+        pages, entries = iter(self._free[:left - 1 if left else None:-1]), []
         for b, m in enumerate(more):
-            for _ in range(m):
-                entries.append((b, len(self._tables[b]), self._free[-1]))
-                self._tables[b].append(self._free.pop())
+            entries += [(b, len(self._tables[b]) + i, next(pages)) for i in range(m)]
         if entries:
             rows = torch.tensor(entries, dtype=torch.int64).to(device)
             self.block_table[rows[:, 0], rows[:, 1]] = rows[:, 2].to(torch.int32)
         lens = None if new_lens is None else torch.tensor(new, dtype=torch.int32).to(device)
         paged_append(self.pages, self.lengths, self.block_table, k_partial.contiguous(),
                      v_partial.contiguous(), lens)
+        # the rows are on their way: from here on the pages are taken (until then only table
+        # entries behind the lengths have changed, which nothing reads)
         self.lengths += n if lens is None else lens
+        del self._free[left:]
+        for b, _, page in entries:
+            self._tables[b].append(page)
         self._filled = [f + x for f, x in zip(self._filled, new)]
 
     def decode(self, q, out=None, lse_out=None, num_selected=None, first_blocks=1, last_blocks=1):

@@ -329,6 +329,12 @@ def poison_tails(pages, lengths, table):
     (1, 1, 1, 1, [4]),
     (128, 16, 8, 4, [2048]),
     (128, 128, 1, 1, [5000, 2, 1200]),
+    (256, 16, 2, 9, [300, 50]),              # two tiles of heads, each with a pass of its own
+    (64, 16, 1, 1, [60001]),                 # one unit over every SM
+    (64, 32, 8, 2, [(37*i) % 401 for i in range(40)]),       # many units, a warp takes several
+    (64, 16, 8, 3, [(29*i) % 251 for i in range(40)]),       # and none is long enough to split
+    (128, 32, 4, 3, [(211*i) % 977 for i in range(20)]),
+    (128, 16, 4, 1, [1]*19 + [9000]),        # one long among short ones
 ])
 def test_decode_against_64_bits(D, P, H, G, lengths, e4m3, dtype):
     dt, g = DT[dtype], gen(D*P + G)
@@ -540,6 +546,22 @@ def test_select_with_nan_infinite_and_missing_pages():
     assert int(status) == BAD_PAGE
     # behind every block that has a page
     assert sorted(set(range(count)) - set(got[0, 0].tolist())) == [3]
+
+
+def test_select_without_a_pool():
+    """Every page is missing: the lowest blocks, reported, nothing read."""
+    for D in (64, 20):
+        pages = KVPages.empty(0, 16, 1, D, bounds=True)
+        q = torch.ones((1, 2, 1, 1, D), dtype=torch.bfloat16, device="cuda")
+        status = ints(0)
+        table = torch.arange(9, dtype=torch.int32, device="cuda").reshape(1, 9)
+        got = paged_select(q, pages, ints(9*16), table, 3, 0, 1, status=status)
+        assert got.tolist() == [[[0, 1, 8]]] and int(status) == BAD_PAGE
+        status.zero_()
+        lse = torch.zeros((1, 2, 1), device="cuda")
+        out = paged_decode(q, pages, ints(9*16), table, got, lse_out=lse, status=status)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+        assert int(status) == BAD_PAGE
 
 
 def test_bounds_hold_every_score():

@@ -205,6 +205,14 @@ def test_cache_bookkeeping_refuses_before_it_changes_anything(monkeypatch):
     with pytest.raises(TypeError):
         c.append(rows(2, torch.float16), rows(2, torch.float16))
     assert len(calls) == 1
+
+    def fails(*a, **k):
+        raise ValueError("rows on another device")
+    with monkeypatch.context() as m:                        # the call itself is refused
+        m.setattr(sdpa, "paged_append", fails)
+        with pytest.raises(ValueError):
+            c.append(rows(30), rows(30), [10, 30])
+    assert c.free_pages == 2 and c.sequence_lengths() == [20, 3] and c.lengths.tolist() == [20, 3]
     used = set(c.block_table[0, :2].tolist())
     c.release(0)
     assert c.free_pages == 4 and c.sequence_lengths() == [0, 3] and c.lengths.tolist() == [0, 3]
