@@ -1441,7 +1441,15 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
         // one or two of them; with fewer units the warps of a block work together, which
         // makes a part of a unit eight times as long and the parts to join eight times fewer.
         p.wpw = units >= 2*PD_SMS ? 1 : warps;
-        if(unit_tiles <= 2*warps)
+        // Whole units, nothing to join: short ones always; longer ones when they about fill
+        // the SMs once, where a block streams a unit in the time that splitting and joining
+        // add.  Measured (bf16, head 128, group 4, whole against split): 512 positions 9.2
+        // against 11.2 us at 64 units and 9.4 against 11.7 at 144, 1024 positions 12.1 against
+        // 12.6 and 12.3 against 14.3; 2048 positions 17.0 against 15.7 and 28.3 against 29.2.
+        // Selections are equally long for all units, so that there more of them may be whole.
+        const bool fills = units >= PD_SMS/3 && units <= PD_SMS;
+        const bool even = num_selected > 0 && units >= 2*PD_SMS/3;
+        if(unit_tiles <= 2*warps || (fills && unit_tiles <= (even ? 20 : 8)*warps))
         {
             p.whole = 1;
             const int64_t per = warps/p.wpw;
