@@ -515,6 +515,71 @@ __device__ __forceinline__ int block_sum(int v, int *red)
     return all;
 }
 
+// The bin, counted from the highest, in which the rank-th score lies: (bin, scores in it, rank
+// inside it); by a warp, lane 31 - l having the eight from 8l on.
+__device__ __forceinline__ void find_bin(const int *bins, int rank, int4 &found)
+{
+    const int lane = threadIdx.x & 31;
+    const int4 c0 = *reinterpret_cast<const int4 *>(bins + 8*(31 - lane));
+    const int4 c1 = *reinterpret_cast<const int4 *>(bins + 8*(31 - lane) + 4);
+    const int c[8] = {c1.w, c1.z, c1.y, c1.x, c0.w, c0.z, c0.y, c0.x};
+    const int sum = c[0] + c[1] + c[2] + c[3] + c[4] + c[5] + c[6] + c[7];
+    int scan = sum;
+#pragma unroll
+    for(int o = 1; o < 32; o <<= 1)
+    {
+        const int up = __shfl_up_sync(0xffffffffu, scan, o);
+        scan += lane >= o ? up : 0;
+    }
+    int above = scan - sum;
+    if(above < rank && scan >= rank)
+    {
+#pragma unroll
+        for(int k = 0; k < 8; ++k)
+        {
+            if(above < rank && above + c[k] >= rank)
+            {
+                found = make_int4(8*(31 - lane) + 7 - k, c[k], rank - above, 0);
+            }
+            above += c[k];
+        }
+    }
+}
+
+// Exact keys of listed blocks, the largest over the group; 16 lanes per block and query head,
+// all threads of the block.  keys[] starts at zero, where a block without a page stays.
+template<typename T, int THREADS>
+__device__ void rank_near(const PagedSelectArgs &a, int kvh, int b, const int *list,
+        unsigned long long *keys, int count)
+{
+    int c = (threadIdx.x >> 4)/a.group, g = (threadIdx.x >> 4) - c*a.group;
+    const int dc = (THREADS/16)/a.group, dg = THREADS/16 - dc*a.group;
+    while(__any_sync(0xffffffffu, c < count))
+    {
+        int page = -1;
+        if(c < count)
+        {
+            page = a.block_table[(size_t)b*a.max_blocks + list[c]];
+            page = page_in_pool(page, a.num_pages) ? page : -1;
+        }
+        if(__any_sync(0xffffffffu, page >= 0))
+        {
+            const unsigned long long key = exact_key<T>(a, kvh, b, max(page, 0), g);
+            if(page >= 0 && (threadIdx.x & 15) == 0)
+            {
+                atomicMax(&keys[c], key);
+            }
+        }
+        c += dc;
+        g += dg;
+        if(g >= a.group)
+        {
+            g -= a.group;
+            ++c;
+        }
+    }
+}
+
 // The num_selected best blocks of a unit, a CTA each.  CACHED: the scores are kept in
 // shared memory (as many as the launch reserved), otherwise read from L2 again.
 template<typename T, bool CACHED>
@@ -524,7 +589,7 @@ paged_pick_kernel(const PagedSelectArgs a)
     extern __shared__ float cached_s[];
     __shared__ int red[PICK_WARPS], red2[PICK_WARPS];
     __shared__ float fred[PICK_WARPS];
-    __shared__ int listed_s, list_s[PICK_LIST];
+    __shared__ int listed_s, near_s, list_s[PICK_LIST];
     __shared__ unsigned long long list_key_s[PICK_LIST], cut_s;
     __shared__ int equal_want_s;
     __shared__ __align__(16) int bin_s[256];
@@ -564,17 +629,31 @@ paged_pick_kernel(const PagedSelectArgs a)
 
     auto score = [&](int i) { return CACHED ? cached_s[i] : scores[i].x; };
     float error = 0.0f, low = CUDART_INF_F, high = -CUDART_INF_F;
-#pragma unroll 4
-    for(int i = begin + tid; i < end; i += PICK_THREADS)
+    // eight at a time: the first pass is one latency of the L2 cache for up to 4096 blocks
+    for(int i0 = begin + tid; i0 < end; i0 += 8*PICK_THREADS)
     {
-        const float2 se = scores[i];
-        if(CACHED)
+        float2 se[8];
+#pragma unroll
+        for(int u = 0; u < 8; ++u)
         {
-            cached_s[i] = se.x;
+            const int i = i0 + u*PICK_THREADS;
+            se[u] = i < end ? scores[i] : make_float2(0.0f, -1.0f);
         }
-        error = max_nan(error, se.y);
-        low = fminf(low, se.x);
-        high = fmaxf(high, se.x);
+#pragma unroll
+        for(int u = 0; u < 8; ++u)
+        {
+            const int i = i0 + u*PICK_THREADS;
+            if(i < end)
+            {
+                if(CACHED)
+                {
+                    cached_s[i] = se[u].x;
+                }
+                error = max_nan(error, se[u].y);
+                low = fminf(low, se[u].x);
+                high = fmaxf(high, se[u].x);
+            }
+        }
     }
 #pragma unroll
     for(int o = 16; o > 0; o >>= 1)
@@ -608,7 +687,117 @@ paged_pick_kernel(const PagedSelectArgs a)
     // no bound (NaN or infinite sums): every block is ranked exactly
     const bool unsure = !(error < CUDART_INF_F);
     float sure_in = CUDART_INF_F, sure_out = -CUDART_INF_F;
-    if(want > 0 && !unsure)
+    // The usual case in few passes: 256 equal bins of the range; the want-th score lies in one
+    // of them, and what may be exchanged with it in that one and its neighbours, a hundred
+    // blocks or so.  They are ranked in shared memory, the near-ties among them exactly, and
+    // the outcome replaces their scores.
+    bool decided = false;
+    if(CACHED && want > 0 && !unsure && low < high && low > -FLT_MAX)
+    {
+        const float origin = 0.5f*low, scale = 256.0f/(0.5f*high - origin);
+        auto bin = [&](float s) { return min(255, (int)((0.5f*s - origin)*scale)); };
+#pragma unroll 4
+        for(int i = begin + tid; i < end; i += PICK_THREADS)
+        {
+            atomicAdd(&bin_s[bin(cached_s[i])], 1);
+        }
+        __syncthreads();
+        if(warp == 0)
+        {
+            find_bin(bin_s, want, hit_s);
+        }
+        __syncthreads();
+        const int hit = hit_s.x, above = want - hit_s.z;         // scores in higher bins
+        const int over = hit < 255 ? bin_s[hit + 1] : 0;
+        const int many = hit_s.y + over + (hit > 0 ? bin_s[hit - 1] : 0);
+        const float widest = 2.0f*error + fmaxf(fabsf(low), fabsf(high))*4e-7f;
+        // the neighbours hold all that is near: half of the band's width is in the scale
+        decided = many <= PICK_LIST && 0.5f*widest*scale < 0.9f;
+        if(decided)
+        {
+#pragma unroll 4
+            for(int i = begin + tid; i < end; i += PICK_THREADS)
+            {
+                const float s = cached_s[i];
+                const int d = bin(s) - hit;
+                if(d >= -1 && d <= 1)
+                {
+                    const int at = atomicAdd(&listed_s, 1);
+                    list_s[at] = i;
+                    list_score_s[at] = s;
+                }
+            }
+            __syncthreads();
+            // PICK_LIST <= PICK_THREADS: an entry a thread
+            const int rank = want - above + over;                // among the listed ones
+            const float mine = tid < many ? list_score_s[tid] : 0.0f;
+            int higher = 0, same = 0;
+            for(int j = 0; tid < many && j < many; ++j)
+            {
+                higher += list_score_s[j] > mine ? 1 : 0;
+                same += list_score_s[j] == mine ? 1 : 0;
+            }
+            if(tid < many && higher < rank && higher + same >= rank)
+            {
+                last_s = mine;                                   // the same from every equal
+            }
+            if(tid == 0)
+            {
+                near_s = 0;
+            }
+            __syncthreads();
+            const float last = last_s, band = 2.0f*error + fabsf(last)*4e-7f;
+            sure_in = last + band;
+            const bool near = tid < many && mine <= sure_in && mine >= last - band;
+            int slot = 0;
+            if(near)
+            {
+                slot = atomicAdd(&near_s, 1);
+            }
+            const int block = tid < many ? list_s[tid] : 0;
+            // what is above the band in the list is taken; the rest of `rank` are near ones
+            const int need = rank - __syncthreads_count(tid < many && mine > sure_in);
+            const int nears = near_s;
+            if(near)
+            {
+                list_s[slot] = block;
+                list_key_s[slot] = 0ull;
+                // all of them, unless they are ranked
+                cached_s[block] = CUDART_INF_F;
+            }
+            __syncthreads();
+            if(need < nears)
+            {
+                rank_near<T, PICK_THREADS>(a, kvh, b, list_s, list_key_s, nears);
+                __syncthreads();
+                for(int k = tid; k < nears; k += PICK_THREADS)
+                {
+                    const unsigned long long key = list_key_s[k];
+                    int better = 0;
+                    for(int j = 0; j < nears; ++j)
+                    {
+                        better += list_key_s[j] > key || (list_key_s[j] == key
+                                && list_s[j] < list_s[k]) ? 1 : 0;
+                    }
+                    if(better >= need)
+                    {
+                        cached_s[list_s[k]] = -CUDART_INF_F;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        else
+        {
+            __syncthreads();
+            for(int i = tid; i < 256; i += PICK_THREADS)
+            {
+                bin_s[i] = 0;
+            }
+            __syncthreads();
+        }
+    }
+    if(want > 0 && !unsure && !decided)
     {
         // The want-th highest score: count the scores in 256 equal bins of their range; the bin
         // it lies in holds a few, which are ranked against one another - or, when they are
@@ -632,33 +821,9 @@ paged_pick_kernel(const PagedSelectArgs a)
                 }
             }
             __syncthreads();
-            // the first warp finds the bin: lane 31 - l has the eight from 8l on
             if(warp == 0)
             {
-                const int4 c0 = *reinterpret_cast<const int4 *>(bin_s + 8*(31 - lane));
-                const int4 c1 = *reinterpret_cast<const int4 *>(bin_s + 8*(31 - lane) + 4);
-                const int c[8] = {c1.w, c1.z, c1.y, c1.x, c0.w, c0.z, c0.y, c0.x};
-                const int sum = c[0] + c[1] + c[2] + c[3] + c[4] + c[5] + c[6] + c[7];
-                int scan = sum;
-#pragma unroll
-                for(int o = 1; o < 32; o <<= 1)
-                {
-                    const int up = __shfl_up_sync(0xffffffffu, scan, o);
-                    scan += lane >= o ? up : 0;
-                }
-                int above = scan - sum;
-                if(above < rank && scan >= rank)
-                {
-#pragma unroll
-                    for(int k = 0; k < 8; ++k)
-                    {
-                        if(above < rank && above + c[k] >= rank)
-                        {
-                            hit_s = make_int4(8*(31 - lane) + 7 - k, c[k], rank - above, 0);
-                        }
-                        above += c[k];
-                    }
-                }
+                find_bin(bin_s, rank, hit_s);
             }
             __syncthreads();
             const int hit = hit_s.x, hits = hit_s.y;
@@ -739,7 +904,7 @@ paged_pick_kernel(const PagedSelectArgs a)
     bool take_near = false;                      // all near ones are taken; otherwise
     unsigned long long cut = 0ull;               // those above this key,
     int equal_want = 0;                          // and of those equal to it this many
-    if(want > 0)
+    if(want > 0 && !decided)
     {
         if(tid == 0)
         {
@@ -780,42 +945,30 @@ paged_pick_kernel(const PagedSelectArgs a)
         take_near = need >= near;
         if(!take_near)
         {
-            // 16 lanes per block and query head
             const bool listed = near <= PICK_LIST;
-            if(!listed)
+            if(listed)
             {
-                for(int i = begin + tid; i < end; i += PICK_THREADS)
-                {
-                    keys[i] = 0ull;
-                }
-                __syncthreads();
+                rank_near<T, PICK_THREADS>(a, kvh, b, list_s, list_key_s, near);
             }
-            const int most = listed ? near : end - begin;
-            int c = (tid >> 4)/a.group, g = (tid >> 4) - c*a.group;
-            const int dc = (PICK_THREADS/16)/a.group, dg = PICK_THREADS/16 - dc*a.group;
-            while(__any_sync(0xffffffffu, c < most))
+            else
             {
-                const int i = c >= most ? -1 : listed ? list_s[c] : begin + c;
-                int page = -1;
-                if(i >= 0 && (listed || is_near(score(i))))
+                // one by one, near or not: this is for rows of NaN and infinities
+                for(int i0 = begin; i0 < end; i0 += PICK_LIST)
                 {
-                    page = a.block_table[(size_t)b*a.max_blocks + i];
-                    page = page_in_pool(page, a.num_pages) ? page : -1;
-                }
-                if(__any_sync(0xffffffffu, page >= 0))
-                {
-                    const unsigned long long key = exact_key<T>(a, kvh, b, max(page, 0), g);
-                    if(page >= 0 && (tid & 15) == 0)
+                    const int count = min(PICK_LIST, end - i0);
+                    __syncthreads();
+                    for(int k = tid; k < count; k += PICK_THREADS)
                     {
-                        atomicMax(listed ? &list_key_s[c] : &keys[i], key);
+                        list_s[k] = i0 + k;
+                        list_key_s[k] = 0ull;
                     }
-                }
-                c += dc;
-                g += dg;
-                if(g >= a.group)
-                {
-                    g -= a.group;
-                    ++c;
+                    __syncthreads();
+                    rank_near<T, PICK_THREADS>(a, kvh, b, list_s, list_key_s, count);
+                    __syncthreads();
+                    for(int k = tid; k < count; k += PICK_THREADS)
+                    {
+                        keys[i0 + k] = list_key_s[k];
+                    }
                 }
             }
             __syncthreads();
@@ -878,7 +1031,7 @@ paged_pick_kernel(const PagedSelectArgs a)
         if(want <= 0) return 0;
         const float s = score(i);
         if(is_in(s)) return 2;
-        if(!is_near(s)) return 0;
+        if(decided || !is_near(s)) return 0;
         if(take_near) return 2;
         const unsigned long long key = keys[i];
         return key > cut ? 2 : key == cut ? 1 : 0;
