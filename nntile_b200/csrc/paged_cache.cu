@@ -208,7 +208,7 @@ __device__ __forceinline__ uint32_t quantise_row(const uint4 &raw, uint32_t (&c)
 // known: a step of one token is a chain of memory latencies and nothing else.
 // A block's bounds are those of its stored (for 8-bit pages: quantised) keys, rounded to T;
 // rows that were in the page before are merged in unless the block starts with this call.
-template<typename T, bool E4M3, bool VEC, int LPR>
+template<typename T, bool E4M3, bool VEC, int LPR, bool BOUNDS>
 __global__ void __launch_bounds__(ROW_THREADS)
 paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
         int kv_heads, int new_seq, int touched, const int32_t *__restrict__ lengths,
@@ -235,7 +235,7 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     int first, last;
     rows_in_block(start, count, block, page_size, first, last);
     const bool is_k = (blockIdx.y & 1) == 0;
-    const bool bounded = is_k && bounds != nullptr;
+    const bool bounded = BOUNDS && is_k && bounds != nullptr;
     const int part = blockIdx.y >> 1;
     if(!bounded)
     {
@@ -513,8 +513,8 @@ static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
             (unsigned)(2*((most + PART_ROWS - 1)/PART_ROWS)));
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
-#define NB200_APPEND(E, V, L) return launch_chained(paged_append_kernel<T, E, V, L>, grid, \
-        ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
+#define NB200_APPEND(E, V, L) return launch_chained(bounds ? paged_append_kernel<T, E, V, L, true> \
+        : paged_append_kernel<T, E, V, L, false>, grid, ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
         (int)new_seq, (int)touched, lengths, new_lens, block_table, (const T *)k, (const T *)v, \
         k_pages, v_pages, k_scales, v_scales, (T *)bounds, status)
 #define NB200_APPEND_L(E) \
