@@ -11,6 +11,7 @@ namespace nb200 {
 constexpr int ROW_THREADS = 128;
 constexpr int ROWS_AHEAD = 4;
 constexpr int PART_ROWS = 32;
+constexpr int GATHER_ROWS = 64;
 
 // Elements a lane owns of a row.  VEC: eight neighbouring ones, one 16-byte access, LPR
 // lanes a row (LPR = 8, 16, 32 for heads up to 64, 128, 256).  Otherwise (a head that is
@@ -381,7 +382,7 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
 template<typename T, bool E4M3, bool VEC, int LPR>
 __global__ void __launch_bounds__(ROW_THREADS)
 paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
-        int kv_heads, int max_seq, int rows_per_cta, int chunks, int page_shift,
+        int kv_heads, int max_seq, int chunks, int page_shift,
         const int32_t *__restrict__ lengths, const int32_t *__restrict__ block_table,
         const void *__restrict__ k_pages, const void *__restrict__ v_pages,
         const uint8_t *__restrict__ k_scales, const uint8_t *__restrict__ v_scales,
@@ -403,28 +404,35 @@ paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     const void *pages = is_k ? k_pages : v_pages;
     const uint8_t *scales = is_k ? k_scales : v_scales;
     T *out = (is_k ? k : v) + (size_t)unit*max_seq*head;
-    const int64_t begin = (int64_t)chunk*rows_per_cta;
-    const int end = (int)min((int64_t)len, begin + rows_per_cta);
-    // four rows at a time: their pages are looked up together, then fetched together
-    for(int64_t r0 = begin; r0 < end; r0 += ROWS_AHEAD*SLOTS)
+    const int64_t begin = (int64_t)chunk*GATHER_ROWS;
+    const int rows = (int)min((int64_t)GATHER_ROWS, len - begin);
+    if(rows <= 0)
+    {
+        return;
+    }
+    // where the rows are, once per row: the lanes that share a row would all work it out
+    __shared__ int64_t from_s[GATHER_ROWS];
+    if(threadIdx.x < rows)
+    {
+        const int r = (int)begin + threadIdx.x;
+        const int block = page_shift >= 0 ? r >> page_shift : r/page_size;
+        const int page = checked_page(block_table + (size_t)b*max_blocks, block, num_pages, status);
+        from_s[threadIdx.x] = page < 0 ? -1
+                : ((int64_t)page*kv_heads + kvh)*page_size + (r - block*page_size);
+    }
+    __syncthreads();
+    // four rows at a time are fetched together
+    for(int r0 = 0; r0 < rows; r0 += ROWS_AHEAD*SLOTS)
     {
         size_t src[ROWS_AHEAD];
         bool live[ROWS_AHEAD];
 #pragma unroll
         for(int u = 0; u < ROWS_AHEAD; ++u)
         {
-            const int64_t r = r0 + u*SLOTS + slot;
-            live[u] = r < end;
-            src[u] = 0;
-            if(live[u])
-            {
-                const int block = page_shift >= 0 ? (int)r >> page_shift : (int)r/page_size;
-                const int page = checked_page(block_table + (size_t)b*max_blocks, block,
-                        num_pages, status);
-                live[u] = page >= 0;
-                src[u] = ((size_t)max(page, 0)*kv_heads + kvh)*page_size
-                        + ((int)r - block*page_size);
-            }
+            const int r = r0 + u*SLOTS + slot;
+            const int64_t from = r < rows ? from_s[r] : -1;
+            live[u] = from >= 0;
+            src[u] = (size_t)max(from, (int64_t)0);
         }
         uint4 raw[ROWS_AHEAD];
         uint32_t byte[ROWS_AHEAD];
@@ -463,7 +471,7 @@ paged_gather_kernel(int head, int page_size, int num_pages, int max_blocks, int 
             }
             if(live[u])
             {
-                store_row<T, VEC, LPR>(out + (size_t)(r0 + u*SLOTS + slot)*head, head, lane,
+                store_row<T, VEC, LPR>(out + (size_t)(begin + r0 + u*SLOTS + slot)*head, head, lane,
                         raw[u]);
             }
         }
@@ -556,8 +564,7 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
         return NNTILE_B200_E_ALIGN;
     }
     const int64_t reach = std::min(max_seq, max_blocks*page_size);
-    const int64_t rows_per_cta = 64;
-    const int64_t chunks = (reach + rows_per_cta - 1)/rows_per_cta;
+    const int64_t chunks = (reach + GATHER_ROWS - 1)/GATHER_ROWS;
     if(chunks*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
     const dim3 grid((unsigned)(chunks*batch*kv_heads), 2);
     int shift = -1;                              // of a power of two, the usual page size
@@ -569,7 +576,7 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     cudaStream_t s = as_stream(stream);
 #define NB200_GATHER(E, V, L) return launch_chained(paged_gather_kernel<T, E, V, L>, grid, \
         ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
-        (int)max_seq, (int)rows_per_cta, (int)chunks, shift, lengths, block_table, k_pages, v_pages, \
+        (int)max_seq, (int)chunks, shift, lengths, block_table, k_pages, v_pages, \
         k_scales, v_scales, (T *)k, (T *)v, status)
 #define NB200_GATHER_L(E) \
     do { \
