@@ -212,7 +212,8 @@ __device__ __forceinline__ uint32_t quantise_row(const uint4 &raw, uint32_t (&c)
 template<typename T, bool E4M3, bool VEC, int LPR, bool BOUNDS>
 __global__ void __launch_bounds__(ROW_THREADS)
 paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int batch,
-        int kv_heads, int new_seq, int touched, const int32_t *__restrict__ lengths,
+        int kv_heads, int new_seq, int touched, int page_shift,
+        const int32_t *__restrict__ lengths,
         const int32_t *__restrict__ new_lens, const int32_t *__restrict__ block_table,
         const T *__restrict__ k, const T *__restrict__ v, void *__restrict__ k_pages,
         void *__restrict__ v_pages, uint8_t *__restrict__ k_scales,
@@ -232,7 +233,7 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     {
         report(status, NNTILE_B200_PAGED_BAD_LENGTH);
     }
-    const int block = start/page_size + j;
+    const int block = (page_shift >= 0 ? start >> page_shift : start/page_size) + j;
     int first, last;
     rows_in_block(start, count, block, page_size, first, last);
     const bool is_k = (blockIdx.y & 1) == 0;
@@ -339,11 +340,14 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
                 }
             }
         }
-#pragma unroll
-        for(int u = 0; u < ROWS_AHEAD; ++u)
+        if(r0 + ROWS_AHEAD*SLOTS < rows)
         {
-            const int row = r0 + (u + ROWS_AHEAD)*SLOTS + slot;
-            raw[u] = fetch_row<T, VEC, LPR>(src + (size_t)row*head, head, lane, row < rows);
+#pragma unroll
+            for(int u = 0; u < ROWS_AHEAD; ++u)
+            {
+                const int row = r0 + (u + ROWS_AHEAD)*SLOTS + slot;
+                raw[u] = fetch_row<T, VEC, LPR>(src + (size_t)row*head, head, lane, row < rows);
+            }
         }
     }
     if(!bounded)
@@ -487,6 +491,16 @@ static bool vector_rows(int64_t head, bool e4m3, const void *a, const void *b, c
     return head % 8 == 0 && (rows & 15) == 0 && (pages & (e4m3 ? 7 : 15)) == 0;
 }
 
+// Shift of a power of two, the usual page size; -1 for others.
+static int shift_of(int64_t page_size)
+{
+    for(int i = 0; i <= 16; ++i)
+    {
+        if(page_size == (int64_t)1 << i) return i;
+    }
+    return -1;
+}
+
 template<typename T>
 static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_size,
         int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t kv_heads, int64_t new_seq,
@@ -523,7 +537,7 @@ static int append_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     cudaStream_t s = as_stream(stream);
 #define NB200_APPEND(E, V, L) return launch_chained(bounds ? paged_append_kernel<T, E, V, L, true> \
         : paged_append_kernel<T, E, V, L, false>, grid, ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
-        (int)new_seq, (int)touched, lengths, new_lens, block_table, (const T *)k, (const T *)v, \
+        (int)new_seq, (int)touched, shift_of(page_size), lengths, new_lens, block_table, (const T *)k, (const T *)v, \
         k_pages, v_pages, k_scales, v_scales, (T *)bounds, status)
 #define NB200_APPEND_L(E) \
     do { \
@@ -567,16 +581,11 @@ static int gather_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     const int64_t chunks = (reach + GATHER_ROWS - 1)/GATHER_ROWS;
     if(chunks*batch*kv_heads > INT32_MAX) return NNTILE_B200_E_SHAPE;
     const dim3 grid((unsigned)(chunks*batch*kv_heads), 2);
-    int shift = -1;                              // of a power of two, the usual page size
-    for(int i = 0; i <= 16; ++i)
-    {
-        shift = page_size == (int64_t)1 << i ? i : shift;
-    }
     const bool vec = vector_rows(head, e4m3, k, v, k_pages, v_pages);
     cudaStream_t s = as_stream(stream);
 #define NB200_GATHER(E, V, L) return launch_chained(paged_gather_kernel<T, E, V, L>, grid, \
         ROW_THREADS, 0, s, (int)head, (int)page_size, (int)num_pages, (int)max_blocks, (int)batch, (int)kv_heads, \
-        (int)max_seq, (int)chunks, shift, lengths, block_table, k_pages, v_pages, \
+        (int)max_seq, (int)chunks, shift_of(page_size), lengths, block_table, k_pages, v_pages, \
         k_scales, v_scales, (T *)k, (T *)v, status)
 #define NB200_GATHER_L(E) \
     do { \
