@@ -354,12 +354,27 @@ paged_append_kernel(int head, int page_size, int num_pages, int max_blocks, int 
     {
         return;
     }
-    __shared__ float low_s[SLOTS][8*LPR], high_s[SLOTS][8*LPR];
-#pragma unroll
-    for(int i = 0; i < 8; ++i)
+    __shared__ __align__(16) float low_s[SLOTS][8*LPR], high_s[SLOTS][8*LPR];
+    if(VEC)
     {
-        low_s[slot][element<VEC, LPR>(lane, i)] = low[i];
-        high_s[slot][element<VEC, LPR>(lane, i)] = high[i];
+        const int h = element<VEC, LPR>(lane, 0);
+#pragma unroll
+        for(int i = 0; i < 8; i += 4)
+        {
+            *reinterpret_cast<float4 *>(&low_s[slot][h + i]) = make_float4(low[i], low[i + 1],
+                    low[i + 2], low[i + 3]);
+            *reinterpret_cast<float4 *>(&high_s[slot][h + i]) = make_float4(high[i],
+                    high[i + 1], high[i + 2], high[i + 3]);
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            low_s[slot][element<VEC, LPR>(lane, i)] = low[i];
+            high_s[slot][element<VEC, LPR>(lane, i)] = high[i];
+        }
     }
     __syncthreads();
 #pragma unroll
