@@ -403,8 +403,10 @@ size_t nntile_b200_decode_sdpa_noalloc_max_bytes(void);
  * below into *status, a 32-bit word that the caller clears and reads (NULL: no report).
  * Several sequences may share pages that are only read; a page that is written belongs to
  * one sequence.  head 1..256; any page_size, group and alignment to the element size is
- * right, rows of a multiple of 16 bytes on 16-byte boundaries in pages of a multiple of 16
- * positions are fast. */
+ * right.  Fast are rows of a multiple of 16 bytes on 16-byte boundaries; for the attention
+ * also pages of a multiple of 16 positions, fewer than 4096 sequences and pools of fewer than
+ * 2^31 positions times kv heads.  A batch, group or kv_heads of 0 is a call with nothing to
+ * do: it returns NNTILE_B200_OK and writes nothing. */
 #define NNTILE_B200_PAGES_SAME 0            /* page_format: pages hold T */
 #define NNTILE_B200_PAGES_E4M3 1            /* page_format: pages hold e4m3 and scales */
 #define NNTILE_B200_PAGED_BAD_PAGE 1u       /* a table entry is outside the pool */
@@ -480,8 +482,9 @@ size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, int64_t page_
  * `last_blocks` are always taken, then those of the highest score
  *     max over the group of  sum_d max(q_d, 0)*kmax_d + min(q_d, 0)*kmin_d,
  * an upper bound on every q.k of the block, until num_selected are chosen; equal scores go
- * to the lower block, a NaN score counts as the highest.  Scores are compared as sums in 64
- * bits.  `selected` (int32 [num_selected, batch, kv_heads]) receives the block numbers in
+ * to the lower block, a NaN score (also 0 times an infinite bound) counts as the highest, a
+ * block without a page as the lowest.  Scores are compared as sums in 64 bits.  Tables of
+ * sequences that are taken whole are not read.  `selected` (int32 [num_selected, batch, kv_heads]) receives the block numbers in
  * ascending order, then -1.  first_blocks + last_blocks <= num_selected.  `workspace`:
  * nntile_b200_paged_select_workspace_bytes(...) bytes, 16-byte aligned, of any content. */
 int nntile_b200_paged_select_bf16(nntile_b200_stream_t stream, int64_t head,

@@ -14,6 +14,11 @@
 // The bound: a truncating accumulation of 16 products and the running sum in fp32 loses at
 // most 17 units of 2^-23 of the sum of magnitudes a step; head <= 256 takes 32 steps, so
 // 32*17*2^-23 < 2^-13 of sum_d |q_d||k_d|, which a second product of magnitudes delivers.
+//
+// Measured on one B200: 128 of up to 2049 blocks for 24 sequences and 8 kv heads of 128 (85.6 MB
+// of bounds): 29-31 us, of which the scores are 20 and the ranking the rest, a chain of a
+// dozen short passes; 64 of 4096 blocks of one sequence with the attention over them: 27 us.
+// Scoring everything in 64 bits instead took 240 us for the first.
 #include <algorithm>
 #include <cfloat>
 
