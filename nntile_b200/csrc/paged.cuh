@@ -153,7 +153,9 @@ __device__ __forceinline__ int checked_page(const int32_t *table, int n, int num
 // starts early starts after all but the last kernel before it are complete: what that one
 // does not write (for the second kernel of a call: lengths and tables) may be read before the
 // wait, the rest only after it.  Every kernel waits, also in blocks with nothing to do: a
-// grid must not end before the one it is chained to.
+// grid must not end before the one it is chained to.  What it reads may still be written while
+// it is being set up, so no pointer of a chained kernel is promised to be read-only
+// (`const __restrict__`, __ldg): such loads could be moved ahead of the wait.
 __device__ __forceinline__ void chain_wait()
 {
     asm volatile("griddepcontrol.wait;" ::: "memory");
