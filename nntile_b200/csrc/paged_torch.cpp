@@ -82,12 +82,14 @@ P *address(const at::Tensor *t, int device)
     return static_cast<P *>(t->data_ptr());
 }
 
-// The attributes live in slots of the KVPages, which the caller holds.
+// The attributes are held until the call is on its way, whatever kind of object they are of.
 struct Pages
 {
     const at::Tensor *k, *v, *k_scales, *v_scales, *bounds;
     int64_t num_pages, kv_heads, page_size, head;
     bool e4m3;
+
+    Pages(const Pages &) = delete;
 
     explicit Pages(PyObject *o)
     {
@@ -123,7 +125,22 @@ struct Pages
     }
 
 private:
-    static const at::Tensor *attribute(PyObject *o, PyObject *name)
+    struct Held
+    {
+        PyObject *objects[5];
+        int count = 0;
+
+        ~Held()                                  // also when a check ends the constructor
+        {
+            while(count > 0)
+            {
+                Py_DECREF(objects[--count]);
+            }
+        }
+    };
+    Held held;
+
+    const at::Tensor *attribute(PyObject *o, PyObject *name)
     {
         PyObject *found = PyObject_GetAttr(o, name);
         if(!found)
@@ -131,7 +148,7 @@ private:
             PyErr_Clear();
             throw Refused();
         }
-        Py_DECREF(found);                        // the slot still refers to it
+        held.objects[held.count++] = found;
         return tensor(found);
     }
 };

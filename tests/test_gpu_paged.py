@@ -644,6 +644,28 @@ def test_on_another_stream_and_on_slices_of_larger_buffers():
         assert torch.equal(out, want)
 
 
+def test_pages_whose_buffers_are_made_on_access():
+    """Attributes of a pool may be computed: what they return lives until the call is made."""
+    class Views(KVPages):
+        __slots__ = ("whole",)
+        k = property(lambda self: self.whole[:1].view(self.whole.shape[1:]))
+        v = property(lambda self: self.whole[1:].view(self.whole.shape[1:]))
+        k_scales = v_scales = bounds = None
+        e4m3 = False
+
+        def __init__(self, whole):
+            self.whole = whole
+
+    g = gen(27)
+    H, D, P, n = 2, 64, 16, 70
+    table = make_table(g, [n, n], P, 20)
+    whole = randn(g, 2, 20, H, P, D).bfloat16()
+    q = randn(g, H, 3, 2, 1, D).bfloat16()
+    for _ in range(20):
+        got = paged_decode(q, Views(whole), ints(n, n), table)
+        assert torch.equal(got, paged_decode(q, KVPages(whole[0], whole[1]), ints(n, n), table))
+
+
 def test_two_calls_at_once():
     """Calls on two streams, each with the workspace it allocates, do not disturb each other."""
     g = gen(22)
