@@ -551,76 +551,101 @@ paged_decode_kernel(const PagedDecodeArgs a)
 
     chain_wait();
 
-    // ---- this worker's share: tiles [begin, end) of the row of all tiles
-    int *prefix = reinterpret_cast<int *>(merge);
-    tile_prefix(a, HU, prefix, scan_s, blockIdx.x == 0);
-    const int total = prefix[a.batch];
-    int wpw, worker, begin, end;
-    if(a.whole)
+    // zeros for query heads g0, g0 + step, .. of unit (b, hu), which has nothing to attend to
+    auto nothing = [&](int b, int hu, int g0, int step)
     {
-        // whole units, no joining: unit = sequence*HU + (kv head, head tile)
-        wpw = a.wpw;
-        worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
-        const long long units = (long long)a.batch*HU;
-        const int workers = gridDim.x*(WARPS/wpw);
-        int x[2];
-#pragma unroll
-        for(int i = 0; i < 2; ++i)
+        const int h0 = hu % htiles*8*MT, heads = min(8*MT, a.group - h0);
+        for(int g = g0; g < heads; g += step)
         {
-            const int u = (int)(units*(worker + i)/workers);
-            const int b = u/HU;
-            x[i] = b < a.batch ? prefix[b] + (prefix[b + 1] - prefix[b])/HU*(u - b*HU) : total;
-        }
-        begin = x[0];
-        end = x[1];
-        // units with nothing to attend to
-        const int u0 = (int)(units*worker/workers), u1 = (int)(units*(worker + 1)/workers);
-        for(int u = u0 + (wpw > 1 ? warp : 0); u < u1; u += wpw)
-        {
-            const int b = u/HU, hu = u - b*HU;
-            if(prefix[b + 1] == prefix[b])
+            const size_t qh = ((size_t)(hu/htiles)*a.group + h0 + g)*a.batch + b;
+            for(int d = lane; d < D; d += 32)
             {
-                const int h0 = hu % htiles*8*MT, heads = min(8*MT, a.group - h0);
-                for(int g = 0; g < heads; ++g)
-                {
-                    const size_t qh = ((size_t)(hu/htiles)*a.group + h0 + g)*a.batch + b;
-                    for(int d = lane; d < D; d += 32)
-                    {
-                        ((T *)a.out)[qh*D + d] = from_f<T>(0.0f);
-                    }
-                    if(lane == 0 && a.lse_out)
-                    {
-                        a.lse_out[qh] = -CUDART_INF_F;
-                    }
-                }
+                ((T *)a.out)[qh*D + d] = from_f<T>(0.0f);
             }
+            if(lane == 0 && a.lse_out)
+            {
+                a.lse_out[qh] = -CUDART_INF_F;
+            }
+        }
+    };
+
+    // ---- this worker's share: tiles [begin, end) of the row of all tiles, and the sequence b
+    // it begins in, whose own tiles begin at seq_begin
+    const int wpw = a.wpw, workers = gridDim.x*(WARPS/wpw);
+    const int worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
+    int begin, end, b = 0, seq_begin = 0;
+    if(a.whole && (long long)a.batch*HU <= workers)
+    {
+        // a unit each at most: no need to know where the others' tiles are
+        if(worker >= a.batch*HU)
+        {
+            return;
+        }
+        b = worker/HU;
+        const int hu = worker - b*HU;
+        const int nt = unit_tiles(a, checked_length(a.lengths, b, a.max_blocks*a.page_size,
+                lane == 0 ? a.status : nullptr));
+        begin = hu*nt;
+        end = begin + nt;
+        if(nt == 0)
+        {
+            nothing(b, hu, wpw > 1 ? warp : 0, wpw);
+            return;                           // the whole worker
         }
     }
     else
     {
-        const PagedShares sh = paged_shares<WARPS>(total, gridDim.x, a.wpw);
-        wpw = sh.wpw;
-        worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
-        begin = (int)min((long long)total, (long long)worker*sh.share);
-        end = (int)min((long long)total, (long long)begin + sh.share);
-    }
-    int b = 0;
-    if(begin < end)
-    {
-        int lo = 0, hi = a.batch;             // prefix[lo] <= begin < prefix[hi]
-        while(hi - lo > 1)
+        int *prefix = reinterpret_cast<int *>(merge);
+        tile_prefix(a, HU, prefix, scan_s, blockIdx.x == 0);
+        const int total = prefix[a.batch];
+        if(a.whole)
         {
-            const int mid = (lo + hi) >> 1;
-            if(prefix[mid] <= begin) lo = mid;
-            else hi = mid;
+            // whole units, no joining: unit = sequence*HU + (kv head, head tile)
+            const long long units = (long long)a.batch*HU;
+            int x[2];
+#pragma unroll
+            for(int i = 0; i < 2; ++i)
+            {
+                const int u = (int)(units*(worker + i)/workers);
+                const int ub = u/HU;
+                x[i] = ub < a.batch ? prefix[ub] + (prefix[ub + 1] - prefix[ub])/HU*(u - ub*HU)
+                        : total;
+            }
+            begin = x[0];
+            end = x[1];
+            const int u0 = (int)(units*worker/workers), u1 = (int)(units*(worker + 1)/workers);
+            for(int u = u0 + (wpw > 1 ? warp : 0); u < u1; u += wpw)
+            {
+                const int ub = u/HU;
+                if(prefix[ub + 1] == prefix[ub])
+                {
+                    nothing(ub, u - ub*HU, 0, 1);
+                }
+            }
         }
-        b = lo;
-    }
-    const int seq_begin = prefix[b];
-    __syncthreads();                          // the prefix sums give way to the merge buffer
-    if(begin >= end)
-    {
-        return;                               // the whole block when wpw > 1: same share
+        else
+        {
+            const PagedShares sh = paged_shares<WARPS>(total, gridDim.x, wpw);
+            begin = (int)min((long long)total, (long long)worker*sh.share);
+            end = (int)min((long long)total, (long long)begin + sh.share);
+        }
+        if(begin < end)
+        {
+            int lo = 0, hi = a.batch;         // prefix[lo] <= begin < prefix[hi]
+            while(hi - lo > 1)
+            {
+                const int mid = (lo + hi) >> 1;
+                if(prefix[mid] <= begin) lo = mid;
+                else hi = mid;
+            }
+            b = lo;
+        }
+        seq_begin = prefix[b];
+        __syncthreads();                      // the prefix sums give way to the merge buffer
+        if(begin >= end)
+        {
+            return;                           // the whole block when wpw > 1: same share
+        }
     }
 
     // ---- issuing side: runs STAGES - 1 tiles ahead of the consuming side
