@@ -28,9 +28,9 @@
 //
 // Measured on one B200 (copy bandwidth 6 553 GB/s), head 128: 64 sequences of 8192, 8 kv heads,
 // group 4, bf16: 326-330 us, 6.5 TB/s; 37 sequences of up to 16383, e4m3, group 8: 135-150 us,
-// 5.1-5.7 TB/s; one of 100003, 2 kv heads, group 7, fp16: 23-28 us, 3.7-4.4 TB/s, of which
-// 15.6 us are the bytes, about 4 the start (length, page and first row, one after the other)
-// and 5 the joining.  With 8-bit heads of 64 the instructions bound it (300 MB in 76 us, the
+// 5.1-5.7 TB/s; one of 100003, 2 kv heads, group 7, fp16: 19-20 us, 5.1-5.4 TB/s, of which
+// 15.6 us are the bytes and the rest the start (length, page and first row, one after the
+// other) and the joining.  With 8-bit heads of 64 the instructions bound it (300 MB in 76 us, the
 // copies alone 54), with 16-bit rows the copies do.
 #include <algorithm>
 #include <type_traits>
@@ -1358,9 +1358,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
 // Joins the parts of the units that fell into several shares, and answers those with
 // nothing to attend to.  A piece is 128 columns of a unit's heads, four neighbouring ones a
 // lane; `wpp` warps share the parts of a piece and meet in shared memory: one warp while
-// units are many and their parts few, up to eight when a few units have many parts each.
-constexpr int PD_JOIN_WARPS = 8;
-
+// units are many and their parts few, up to 32 when a few units have many parts each.
 __host__ __device__ inline int join_pieces(int heads, int dp)
 {
     return (heads*dp + 127)/128;
@@ -1372,30 +1370,46 @@ struct JoinState                         // four values of a head, not yet divid
     float4 o;
 };
 
-__device__ __forceinline__ void join_add(JoinState &s, float top, float sum, const float4 &o)
+// N more parts at once: one maximum, and weights that do not wait for one another.
+template<int N>
+__device__ __forceinline__ void join_add(JoinState &s, const float2 (&ts)[N], const float4 (&o)[N])
 {
-    const float ntop = fmaxf(s.top, top);
-    const float ref = ntop == -CUDART_INF_F ? 0.0f : ntop;
-    const float x = ex2(s.top - ref), y = ex2(top - ref);
-    s.top = ntop;
-    s.sum = s.sum*x + sum*y;
-    s.o.x = s.o.x*x + o.x*y;
-    s.o.y = s.o.y*x + o.y*y;
-    s.o.z = s.o.z*x + o.z*y;
-    s.o.w = s.o.w*x + o.w*y;
+    float top = s.top;
+#pragma unroll
+    for(int u = 0; u < N; ++u)
+    {
+        top = fmaxf(top, ts[u].x);
+    }
+    const float ref = top == -CUDART_INF_F ? 0.0f : top, x = ex2(s.top - ref);
+    s.top = top;
+    s.sum *= x;
+    s.o.x *= x;
+    s.o.y *= x;
+    s.o.z *= x;
+    s.o.w *= x;
+#pragma unroll
+    for(int u = 0; u < N; ++u)
+    {
+        const float y = ex2(ts[u].x - ref);
+        s.sum = fmaf(ts[u].y, y, s.sum);
+        s.o.x = fmaf(o[u].x, y, s.o.x);
+        s.o.y = fmaf(o[u].y, y, s.o.y);
+        s.o.z = fmaf(o[u].z, y, s.o.z);
+        s.o.w = fmaf(o[u].w, y, s.o.w);
+    }
 }
 
-template<typename T, bool E4M3, int DP, int MT>
-__global__ void __launch_bounds__(PD_JOIN_WARPS*32)
+template<typename T, bool E4M3, int DP, int MT, int JOIN_WARPS>
+__global__ void __launch_bounds__(JOIN_WARPS*32)
 paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
 {
     using L = PagedTile<E4M3, DP>;
     const int pieces = join_pieces(min(8*MT, a.group), DP);
-    __shared__ float2 sums_s[PD_JOIN_WARPS][32];
-    __shared__ float4 o_s[PD_JOIN_WARPS][32];
+    __shared__ float2 sums_s[JOIN_WARPS][32];
+    __shared__ float4 o_s[JOIN_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
-    const int id = (blockIdx.x*PD_JOIN_WARPS + warp)/wpp;
+    const int id = (blockIdx.x*JOIN_WARPS + warp)/wpp;
     const int unit = id/pieces, piece = id - unit*pieces;
     const int b = min(unit/HU, a.batch - 1), hu = unit - b*HU;
     // tiles of all sequences, and of those before this one
@@ -1439,11 +1453,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
                 o[u] = on ? *reinterpret_cast<const float4 *>(a.part_o + (p*MT + m)*8*DP + off)
                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
-#pragma unroll
-            for(int u = 0; u < 4; ++u)
-            {
-                join_add(s, ts[u].x, ts[u].y, o[u]);
-            }
+            join_add(s, ts, o);
         }
     }
     if(wpp > 1)
@@ -1455,10 +1465,19 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
         {
             return;
         }
-        for(int w = 1; w < wpp; ++w)
+        for(int w0 = 1; w0 < wpp; w0 += 4)
         {
-            const float2 ts = sums_s[warp + w][lane];
-            join_add(s, ts.x, ts.y, o_s[warp + w][lane]);
+            float2 ts[4];
+            float4 o[4];
+#pragma unroll
+            for(int u = 0; u < 4; ++u)
+            {
+                const bool on = w0 + u < wpp;
+                const int w = on ? warp + w0 + u : warp;
+                ts[u] = on ? sums_s[w][lane] : make_float2(-CUDART_INF_F, 0.0f);
+                o[u] = on ? o_s[w][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            join_add(s, ts, o);
         }
     }
     if(none)
@@ -1596,13 +1615,19 @@ static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDeco
     // starts while the first kernel still runs and waits for its results on the device
     const int htiles = (a.group + 8*MT - 1)/(8*MT);
     // warps a piece: about as many as it has parts by fours, were the lengths even; with
-    // uneven ones a unit may have more, so never one alone when blocks are the workers
-    const int wpp = a.wpw == 1 ? 1 : plan.grid <= 3*a.batch*a.kv_heads*htiles ? 4 : PD_JOIN_WARPS;
-    const unsigned warps = (unsigned)a.batch*a.kv_heads*htiles
-            *join_pieces(std::min(8*MT, a.group), DP)*wpp;
-    return launch_chained(paged_join_kernel<T, E4M3, DP, MT>,
-            dim3((warps + PD_JOIN_WARPS - 1)/PD_JOIN_WARPS), PD_JOIN_WARPS*32, 0, s, a, plan.grid,
-            wpp);
+    // uneven ones a unit may have more, so never one alone when blocks are the workers.
+    // Measured with 8, 16 and 32 (bf16, head 128, group 4): 64 parts 8.5, 8.2 and 8.8 us, 74
+    // parts 13.0, 12.7 and 12.7, 148 parts 10.8, 10.4 and 9.7; 18 parts 7.8 and 8.4 with 8 and 16.
+    const int64_t units = (int64_t)a.batch*a.kv_heads*htiles;
+    const int wpp = a.wpw == 1 ? 1 : plan.grid <= 3*units ? 4 : plan.grid <= 20*units ? 8
+            : plan.grid <= 72*units ? 16 : 32;
+    const int64_t warps = units*join_pieces(std::min(8*MT, a.group), DP)*wpp;
+    const int block = std::max(wpp, 8);
+    auto kernel = wpp == 32 ? paged_join_kernel<T, E4M3, DP, MT, 32>
+            : wpp == 16 ? paged_join_kernel<T, E4M3, DP, MT, 16>
+            : paged_join_kernel<T, E4M3, DP, MT, 8>;
+    return launch_chained(kernel, dim3((unsigned)((warps + block - 1)/block)), block*32, 0, s, a,
+            plan.grid, wpp);
 }
 
 template<typename T>
