@@ -8,8 +8,9 @@
 // design is about bytes in flight and about even shares:
 //   - work is cut into tiles of 16 positions.  All tiles of all (sequence, kv head) units
 //     stand in one row, and every worker takes the same number of neighbours, whatever
-//     the lengths are (they are only known on the device).  A unit that falls into several
-//     shares is joined by a second, small kernel;
+//     the lengths are (they are only known on the device), or, where few units allow it, an
+//     even piece of one unit.  A unit that falls into several shares is joined by a second,
+//     small kernel;
 //   - a warp copies its own tiles into a private ring in shared memory (cp.async, 16 bytes a
 //     lane, swizzled; rows behind the length are zero-filled, never read) and is its own
 //     consumer: no barrier inside a share.  24 KB a warp, 192 KB an SM, more than four times
@@ -28,7 +29,7 @@
 //
 // Measured on one B200 (copy bandwidth 6 553 GB/s), head 128: 64 sequences of 8192, 8 kv heads,
 // group 4, bf16: 326-330 us, 6.5 TB/s; 37 sequences of up to 16383, e4m3, group 8: 135-150 us,
-// 5.1-5.7 TB/s; one of 100003, 2 kv heads, group 7, fp16: 19-20 us, 5.1-5.4 TB/s, of which
+// 5.1-5.7 TB/s; one of 100003, 2 kv heads, group 7, fp16: 18-19 us, 5.4-5.6 TB/s, of which
 // 15.6 us are the bytes and the rest the start (length, page and first row, one after the
 // other) and the joining.  With 8-bit heads of 64 the instructions bound it (300 MB in 76 us, the
 // copies alone 54), with 16-bit rows the copies do.
@@ -55,6 +56,7 @@ struct PagedDecodeArgs
     float *lse_out;
     float *part_o, *part_lse;
     float2 *part_sums;
+    int2 *spans;                         // [unit]: first and last worker that has a part of it
     uint32_t *status;
     int wpw;                             // warps of a worker
     int whole;                           // workers take whole units, nothing is joined
@@ -281,8 +283,11 @@ struct PagedTile
     static constexpr int AHEAD = STAGES - ABREAST;       // tiles in flight or waiting
     static_assert(AHEAD >= ABREAST, "the ring must hold what is consumed and what is coming");
     static constexpr int MBLK = DP/16;                   // 16-column blocks of the output
-    // One tile of 8 heads of every warp, in two rounds where that is more than 32 KB.
-    static constexpr int ROUNDS = WARPS*8*DP*4 > 32768 ? 2 : 1;
+    // One tile of 8 heads of every warp, for 256 columns in two rounds: with 16-bit rows of
+    // 256 that leaves an SM room for blocks of the joining kernel, which then wait beside this
+    // one (16 kv heads of 512 positions 11.1 -> 8.7 us).  With 128 columns the second round
+    // costs as much as it gains.
+    static constexpr int ROUNDS = DP == 256 ? 2 : 1;
     static constexpr int MERGE = WARPS*8*DP*4/ROUNDS;
     static constexpr int SMEM = WARPS*STAGES*STAGE + MERGE;
 
@@ -514,6 +519,38 @@ __host__ __device__ inline PagedShares paged_shares(int total, int blocks, int w
     return s;
 }
 
+// ceil(tiles/size), 0 <= tiles < 2^30, the quotient below 2^20: exact, and shorter than the
+// division of integers that the start of a call would otherwise wait for several times.
+__device__ __forceinline__ int pieces_of(int tiles, int size)
+{
+    const int x = tiles + size - 1;
+    const int q = (int)__fdividef((float)x, (float)size), r = x - q*size;
+    return q + (r >= size ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+
+// Shares that end where units end.  A worker whose share reaches into a second unit starts and
+// ends twice, 2 us; it is cheaper to cut every unit into pieces of at most `size` tiles, a
+// worker each, when there are workers for that with a size at or little above the even share
+// (bf16, head 128, even shares against pieces: 32 units of 3000 positions 14.2 and 12.5 us, 144
+// units of 3000 in e4m3 30.9 and 26.7; pieces half as large again as the share lose: 96 units
+// of 2048 19.2 and 22.7).  Working it out costs 0.5 us where nothing is gained: 8 units of 512
+// 7.4 and 8.1.  Returns that size, or 0.  t0, t1: tiles of a unit of sequences lane, lane + 32.
+template<int WARPS>
+__device__ __forceinline__ int piece_size(int t0, int t1, int units_per_seq, int total,
+        int workers)
+{
+    const int even = pieces_of(total, workers*WARPS), more = even + even/4;
+    const int least = (int)__reduce_add_sync(0xffffffffu, pieces_of(t0, even*WARPS)
+            + pieces_of(t1, even*WARPS))*units_per_seq;
+    if(least <= workers)
+    {
+        return even*WARPS;
+    }
+    const int fewer = (int)__reduce_add_sync(0xffffffffu, pieces_of(t0, more*WARPS)
+            + pieces_of(t1, more*WARPS))*units_per_seq;
+    return fewer <= workers ? more*WARPS : 0;
+}
+
 // EXACT: the head size is DP.
 template<typename T, bool E4M3, int DP, int MT, bool EXACT>
 __global__ void __launch_bounds__(PagedTile<E4M3, DP>::WARPS*32, 1)
@@ -577,6 +614,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
     const int wpw = a.wpw, workers = gridDim.x*(WARPS/wpw);
     const int worker = blockIdx.x*(WARPS/wpw) + warp/wpw;
     int begin, end, b = 0, seq_begin = 0;
+    int share = 0;                            // tiles of this worker's neighbours as well
     if(a.whole && (long long)a.batch*HU <= workers)
     {
         // a unit each at most: no need to know where the others' tiles are
@@ -599,24 +637,26 @@ paged_decode_kernel(const PagedDecodeArgs a)
     else if(!a.whole && a.batch <= PD_BATCH)
     {
         // every warp finds the share by itself: no barrier before the first copies
-        int total = 0;
-        for(int i0 = 0; i0 < a.batch; i0 += 32)
+        int tiles[2];                         // of a unit of sequences lane, lane + 32
+#pragma unroll
+        for(int i = 0; i < 2; ++i)
         {
-            total += i0 + lane < a.batch ? unit_tiles(a, checked_length(a.lengths, i0 + lane,
-                    a.max_blocks*a.page_size, blockIdx.x == 0 && warp == 0 ? a.status
-                    : nullptr))*HU : 0;
+            tiles[i] = 32*i + lane < a.batch ? unit_tiles(a, checked_length(a.lengths,
+                    32*i + lane, a.max_blocks*a.page_size, blockIdx.x == 0 && warp == 0
+                    ? a.status : nullptr)) : 0;
         }
-        total = __reduce_add_sync(0xffffffffu, total);
+        const int total = (int)__reduce_add_sync(0xffffffffu, (tiles[0] + tiles[1])*HU);
+        const int size = wpw == 1 || total == 0 || a.batch*HU == 1 || a.batch*HU > workers ? 0
+                : piece_size<WARPS>(tiles[0], tiles[1], HU, total, workers);
         const PagedShares sh = paged_shares<WARPS>(total, gridDim.x, wpw);
-        begin = (int)min((long long)total, (long long)worker*sh.share);
-        end = (int)min((long long)total, (long long)begin + sh.share);
-        if(begin >= end)
+        // this worker's place in the row of all pieces, or of all tiles
+        const int place = size > 0 ? worker
+                : (int)min((long long)total, (long long)worker*sh.share);
+        int before = 0, k = 32;               // where the sequence it is in begins, its lane
+#pragma unroll
+        for(int i = 0; i < 2; ++i)
         {
-            return;                           // the whole worker
-        }
-        for(int i0 = 0; i0 < a.batch; i0 += 32)
-        {
-            const int mine = i0 + lane < a.batch ? unit_tiles(a, held_len(a, i0 + lane))*HU : 0;
+            const int mine = (size > 0 ? pieces_of(tiles[i], size) : tiles[i])*HU;
             int scan = mine;
 #pragma unroll
             for(int o = 1; o < 32; o <<= 1)
@@ -624,15 +664,39 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 const int up = __shfl_up_sync(0xffffffffu, scan, o);
                 scan += lane >= o ? up : 0;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, seq_begin + scan > begin);
+            const unsigned hit = __ballot_sync(0xffffffffu, before + scan > place);
             if(hit != 0u)
             {
-                const int k = __ffs((int)hit) - 1;
-                b = i0 + k;
-                seq_begin += __shfl_sync(0xffffffffu, scan - mine, k);
+                k = __ffs((int)hit) - 1;
+                b = 32*i + k;
+                before += __shfl_sync(0xffffffffu, scan - mine, k);
                 break;
             }
-            seq_begin += __shfl_sync(0xffffffffu, scan, 31);
+            before += __shfl_sync(0xffffffffu, scan, 31);
+        }
+        if(k == 32)
+        {
+            return;                           // nothing left for this worker
+        }
+        if(size > 0)
+        {
+            const int nt = __shfl_sync(0xffffffffu, b < 32 ? tiles[0] : tiles[1], k);
+            const int pieces = pieces_of(nt, size);
+            const int hu = pieces_of(place - before + 1, pieces) - 1;
+            share = ((nt + pieces - 1)/pieces + wpw - 1)/wpw*wpw;
+            begin = min((hu + 1)*nt, hu*nt + (place - before - hu*pieces)*share);
+            end = min((hu + 1)*nt, begin + share);
+            if(begin >= end)
+            {
+                return;
+            }
+        }
+        else
+        {
+            share = sh.share;
+            seq_begin = before;
+            begin = place;
+            end = (int)min((long long)total, (long long)begin + sh.share);
         }
     }
     else
@@ -668,6 +732,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
         else
         {
             const PagedShares sh = paged_shares<WARPS>(total, gridDim.x, wpw);
+            share = sh.share;
             begin = (int)min((long long)total, (long long)worker*sh.share);
             end = (int)min((long long)total, (long long)begin + sh.share);
         }
@@ -1218,6 +1283,12 @@ paged_decode_kernel(const PagedDecodeArgs a)
         // this share's part of it
         const bool complete = x == unit_begin && seg_end == unit_end;
         const int part = 2*worker + (x == unit_begin ? 1 : 0);
+        if(share > 0 && x == unit_begin && lane == 0 && slot0 == 0)
+        {
+            // the others of this unit follow, a share each
+            a.spans[b*HU + hu] = make_int2(worker, worker + (complete ? 0
+                    : (unit_end - end + share - 1)/share));
+        }
         const float vscale = E4M3 ? scale_value((uint32_t)vref) : 1.0f;
 #pragma unroll
         for(int m = 0; m < MT; ++m)
@@ -1401,35 +1472,23 @@ __device__ __forceinline__ void join_add(JoinState &s, const float2 (&ts)[N], co
 
 template<typename T, bool E4M3, int DP, int MT, int JOIN_WARPS>
 __global__ void __launch_bounds__(JOIN_WARPS*32)
-paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
+paged_join_kernel(const PagedDecodeArgs a, int workers, int wpp)
 {
-    using L = PagedTile<E4M3, DP>;
     const int pieces = join_pieces(min(8*MT, a.group), DP);
-    __shared__ float2 sums_s[JOIN_WARPS][32];
+    __shared__ float2 sums_s[JOIN_WARPS][2];             // of lanes 0-15 and 16-31: one head each
     __shared__ float4 o_s[JOIN_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int htiles = (a.group + 8*MT - 1)/(8*MT), HU = a.kv_heads*htiles;
     const int id = (blockIdx.x*JOIN_WARPS + warp)/wpp;
     const int unit = id/pieces, piece = id - unit*pieces;
     const int b = min(unit/HU, a.batch - 1), hu = unit - b*HU;
-    // tiles of all sequences, and of those before this one
-    int total = 0, before = 0;
-    for(int i = lane; i < a.batch; i += 32)
-    {
-        const int tiles = unit_tiles(a, held_len(a, i))*HU;
-        total += tiles;
-        before += i < b ? tiles : 0;
-    }
-    total = __reduce_add_sync(0xffffffffu, total);
-    before = __reduce_add_sync(0xffffffffu, before);
-    const int nt = unit_tiles(a, held_len(a, b));
-    const PagedShares sh = paged_shares<L::WARPS>(total, blocks, a.wpw);
-    const int x0 = before + hu*nt;
-    const int first = nt > 0 ? x0/sh.share : 0, last = nt > 0 ? (x0 + nt - 1)/sh.share : -1;
+    const bool some = unit < a.batch*HU && held_len(a, b) > 0;
     const int m = piece*128/(8*DP), off = piece*128 - m*8*DP + 4*lane;   // in the part's values
     const int head = off/DP, col = off - head*DP;
     const int kvh = hu/htiles, g = (hu - kvh*htiles)*8*MT + 8*m + head;
     chain_wait();
+    const int2 span = some ? a.spans[unit] : make_int2(0, -1);
+    const int first = max(span.x, 0), last = min(span.y, workers - 1);
     // one worker had it all and wrote it, or there is no such head, or (the last block) unit
     const bool none = first == last || g >= a.group || unit >= a.batch*HU;
     JoinState s = {-CUDART_INF_F, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
@@ -1458,7 +1517,10 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
     }
     if(wpp > 1)
     {
-        sums_s[warp][lane] = make_float2(s.top, s.sum);
+        if((lane & 15) == 0)
+        {
+            sums_s[warp][lane >> 4] = make_float2(s.top, s.sum);
+        }
         o_s[warp][lane] = s.o;
         __syncthreads();
         if(warp % wpp != 0)
@@ -1474,7 +1536,7 @@ paged_join_kernel(const PagedDecodeArgs a, int blocks, int wpp)
             {
                 const bool on = w0 + u < wpp;
                 const int w = on ? warp + w0 + u : warp;
-                ts[u] = on ? sums_s[w][lane] : make_float2(-CUDART_INF_F, 0.0f);
+                ts[u] = on ? sums_s[w][lane >> 4] : make_float2(-CUDART_INF_F, 0.0f);
                 o[u] = on ? o_s[w][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
             join_add(s, ts, o);
@@ -1540,9 +1602,9 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
         p.wpw = units >= 2*PD_SMS ? 1 : warps;
         // Whole units, nothing to join: short ones always; longer ones when they about fill
         // the SMs once, where a block streams a unit in the time that splitting and joining
-        // add.  Measured (bf16, head 128, group 4, whole against split): 512 positions 9.2
-        // against 11.2 us at 64 units and 9.4 against 11.7 at 144, 1024 positions 12.1 against
-        // 12.6 and 12.3 against 14.3; 2048 positions 17.0 against 15.7 and 28.3 against 29.2.
+        // add.  Measured (bf16, head 128, group 4, whole against split): 512 positions 7.5
+        // against 10.8 us at 64 units and 7.7 against 11.4 at 144, 1024 positions 10.1 against
+        // 12.1 and 10.5 against 14.1; 2048 positions 15.3 against 13.9 and 26.6 against 29.0.
         // Selections are equally long for all units, so that there more of them may be whole.
         const bool fills = units >= PD_SMS/3 && units <= PD_SMS;
         const bool even = num_selected > 0 && units >= 2*PD_SMS/3;
@@ -1555,7 +1617,8 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
         else
         {
             p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(PD_SMS, (total + warps - 1)/warps));
-            p.bytes = (size_t)2*p.grid*warps*p.mt*8*(p.dp*sizeof(float) + sizeof(float2));
+            p.bytes = (size_t)2*p.grid*warps*p.mt*8*(p.dp*sizeof(float) + sizeof(float2))
+                    + (size_t)units*sizeof(int2);
         }
     }
     const int64_t rows = listed*page_size;
@@ -1627,7 +1690,7 @@ static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDeco
             : wpp == 16 ? paged_join_kernel<T, E4M3, DP, MT, 16>
             : paged_join_kernel<T, E4M3, DP, MT, 8>;
     return launch_chained(kernel, dim3((unsigned)((warps + block - 1)/block)), block*32, 0, s, a,
-            plan.grid, wpp);
+            plan.grid*(paged_warps(E4M3, DP)/a.wpw), wpp);
 }
 
 template<typename T>
@@ -1698,6 +1761,8 @@ static int decode_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     a.part_lse = a.part_o + (size_t)heads*plan.nsplit*(size_t)head;      // generic kernel
     a.part_sums = reinterpret_cast<float2 *>(a.part_o + (plan.fast
             ? (size_t)2*plan.grid*paged_warps(e4m3, plan.dp)*plan.mt*8*plan.dp : 0));
+    a.spans = reinterpret_cast<int2 *>(a.part_sums + (plan.fast
+            ? (size_t)2*plan.grid*paged_warps(e4m3, plan.dp)*plan.mt*8 : 0));
     a.wpw = plan.wpw;
     a.whole = plan.whole;
     a.status = status;

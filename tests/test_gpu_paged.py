@@ -347,6 +347,22 @@ def test_decode_against_64_bits(D, P, H, G, lengths, e4m3, dtype):
     check_attention(q, pages, lens, table)
 
 
+@pytest.mark.parametrize("B,H,G,D", [(2, 3, 2, 128), (8, 4, 2, 256), (31, 1, 3, 64), (33, 2, 2, 128),
+                                     (64, 2, 1, 64), (65, 2, 1, 64)])
+@pytest.mark.parametrize("lengths", ["even", "ragged", "one"])
+def test_decode_cuts_units_into_pieces(B, H, G, D, lengths):
+    """Few units of several lengths: shares that end with the units and shares that do not."""
+    g = gen(100*B + D)
+    P, n = 16, 700
+    lens = [n]*B if lengths == "even" else [0]*(B - 1) + [5*n] if lengths == "one" else \
+        [int(x) for x in torch.randint(0, 2*n, (B,), generator=torch.Generator().manual_seed(B))]
+    num_pages = sum(-(-x//P) for x in lens) + 1
+    pages = make_pool(g, num_pages, P, H, D, torch.bfloat16, False)
+    table = make_table(g, lens, P, num_pages)
+    q = randn(g, H, G, B, 1, D).bfloat16()
+    check_attention(q, pages, ints(*lens), table)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_decode_with_far_apart_values(e4m3, dtype):
