@@ -23,6 +23,7 @@
 #include <cfloat>
 
 #include "paged.cuh"
+#include "paged_rank.hh"
 #include "per_device.hh"
 
 namespace nb200 {
@@ -39,17 +40,6 @@ __device__ __forceinline__ unsigned long long score_key(double s)
     }
     const unsigned long long u = (unsigned long long)__double_as_longlong(s + 0.0);   // -0 -> +0
     return (u >> 63) ? ~u : u | 0x8000000000000000ull;
-}
-// The same for a float that is not NaN.
-__device__ __forceinline__ uint32_t score_key32(float s)
-{
-    const uint32_t u = __float_as_uint(s + 0.0f);
-    return (u >> 31) ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ float score_of_key(uint32_t key)
-{
-    return __uint_as_float((key >> 31) ? key & 0x7FFFFFFFu : ~key);
 }
 
 struct PagedSelectArgs
@@ -602,7 +592,6 @@ paged_pick_kernel(const PagedSelectArgs a)
     __shared__ float list_score_s[PICK_LIST], last_s;
     __shared__ uint2 mask_s[PICK_THREADS];
     __shared__ int2 before_s[PICK_THREADS];
-    __shared__ uint32_t low_s, high_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int unit = blockIdx.x, b = unit % a.batch, kvh = unit/a.batch;
     // behind the scoring kernel the lengths are settled; as the first kernel of a call (a table
@@ -804,25 +793,24 @@ paged_pick_kernel(const PagedSelectArgs a)
     }
     if(want > 0 && !unsure && !decided)
     {
-        // The want-th highest score: count the scores in 256 equal bins of their range; the bin
-        // it lies in holds a few, which are ranked against one another - or, when they are
-        // more than the list, are the range of another round.  Missing pages (-inf) go into
-        // the lowest bin.
-        int rank = want;                         // from the top of [low, high]
-        low = fmaxf(low, -FLT_MAX);
-        high = fmaxf(high, -FLT_MAX);
-        while(low < high)
+        // The want-th highest score: count the scores in up to 256 equal bins of the range of
+        // their keys; the bin it lies in holds a few, which are ranked against one another - or,
+        // when they are more than the list, is the range of another round.  On keys and not on
+        // the scores, so that every round divides the range, whatever the scores are.  Missing
+        // pages (-inf) go into the lowest bin.
+        int rank = want;                         // from the top of the range
+        auto key = [&](int i) { return score_key32(fmaxf(score(i), -FLT_MAX)); };
+        RankRange range = rank_range(score_key32(fmaxf(low, -FLT_MAX)),
+                score_key32(fmaxf(high, -FLT_MAX)));
+        while(range.low < range.high)
         {
-            // halves: the range of finite numbers may itself not be one
-            const float origin = 0.5f*low, scale = 256.0f/(0.5f*high - origin);
-            auto bin = [&](float s) { return min(255, (int)((0.5f*s - origin)*scale)); };
 #pragma unroll 4
             for(int i = begin + tid; i < end; i += PICK_THREADS)
             {
-                const float s = fmaxf(score(i), -FLT_MAX);
-                if(s >= low && s <= high)
+                const uint32_t k = key(i);
+                if(rank_inside(range, k))
                 {
-                    atomicAdd(&bin_s[bin(s)], 1);
+                    atomicAdd(&bin_s[rank_bin(range, k)], 1);
                 }
             }
             __syncthreads();
@@ -831,17 +819,18 @@ paged_pick_kernel(const PagedSelectArgs a)
                 find_bin(bin_s, rank, hit_s);
             }
             __syncthreads();
-            const int hit = hit_s.x, hits = hit_s.y;
+            const int hits = hit_s.y;
             rank = hit_s.z;
-            if(hits <= PICK_LIST)
+            range = rank_narrowed(range, hit_s.x);
+            if(hits <= PICK_LIST && range.low < range.high)
             {
 #pragma unroll 4
                 for(int i = begin + tid; i < end; i += PICK_THREADS)
                 {
-                    const float s = fmaxf(score(i), -FLT_MAX);
-                    if(s >= low && s <= high && bin(s) == hit)
+                    const uint32_t k = key(i);
+                    if(rank_inside(range, k))
                     {
-                        list_score_s[atomicAdd(&listed_s, 1)] = s;
+                        list_score_s[atomicAdd(&listed_s, 1)] = score_of_key(k);
                     }
                 }
                 __syncthreads();
@@ -860,44 +849,17 @@ paged_pick_kernel(const PagedSelectArgs a)
                     }
                 }
                 __syncthreads();
-                low = high = last_s;
+                range.low = range.high = score_key32(last_s);
                 break;
             }
-            // the range of the scores in that bin
-            if(tid == 0)
-            {
-                low_s = ~0u;
-                high_s = 0u;
-            }
-            __syncthreads();
             for(int i = tid; i < 256; i += PICK_THREADS)
             {
                 bin_s[i] = 0;
             }
-            uint32_t least = ~0u, most = 0u;
-            for(int i = begin + tid; i < end; i += PICK_THREADS)
-            {
-                const float s = fmaxf(score(i), -FLT_MAX);
-                if(s >= low && s <= high && bin(s) == hit)
-                {
-                    const uint32_t key = score_key32(s);
-                    least = min(least, key);
-                    most = max(most, key);
-                }
-            }
-            least = __reduce_min_sync(0xffffffffu, least);
-            most = __reduce_max_sync(0xffffffffu, most);
-            if(lane == 0 && most != 0u)
-            {
-                atomicMin(&low_s, least);
-                atomicMax(&high_s, most);
-            }
-            __syncthreads();
-            low = score_of_key(low_s);
-            high = rank == hits ? low : score_of_key(high_s);     // the bin's least it is
             __syncthreads();
         }
-        const float last = low > -FLT_MAX ? low : -CUDART_INF_F;
+        const float lowest = score_of_key(range.low);
+        const float last = lowest > -FLT_MAX ? lowest : -CUDART_INF_F;
         // exact values are within `error` of the scores, the want-th of each as well; a few
         // units in the last place more cover these two sums
         const float band = last > -CUDART_INF_F ? 2.0f*error + fabsf(last)*4e-7f : 0.0f;
