@@ -58,6 +58,48 @@ template<> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
     return r;
 }
 
+// the same, cut off towards zero instead of rounded
+template<typename T> __device__ __forceinline__ uint32_t cut2(float lo, float hi);
+template<> __device__ __forceinline__ uint32_t cut2<bf16>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t cut2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// the larger and the smaller of two pairs; a NaN loses
+template<typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template<> __device__ __forceinline__ uint32_t max2<bf16>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<typename T> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
+template<> __device__ __forceinline__ uint32_t min2<bf16>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // two e4m3 codes (low byte first) -> two halves; exact, every e4m3 value is an fp16 value
 __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two_codes)
 {

@@ -152,21 +152,6 @@ __device__ __forceinline__ uint2 fetch_codes(const uint8_t *row, int head, int l
     return make_uint2(w[0], w[1]);
 }
 
-// The larger of two packed pairs of magnitudes; a NaN loses.
-template<typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
-template<> __device__ __forceinline__ uint32_t max2<bf16>(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-template<> __device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-
 // Quantise the eight elements a lane owns (its row shared by the LPR lanes around it):
 // returns the exponent byte, leaves the codes in `c`.  The largest magnitude is found on
 // packed pairs; only a row that holds an infinity goes through the elements one by one.

@@ -19,8 +19,8 @@
 //   - scores and weighted values go through the warp-level tensor instruction (m16n8k16, fp32
 //     accumulate), transposed: keys and columns of V are its 16 rows, 8 query heads its
 //     columns, so no row is idle for groups up to 8 and the accumulators take half the
-//     registers of the other way round.  The weights go in twice, rounded to 16 bits and what
-//     that rounding lost, and so count with 16 (bf16) or 22 (fp16) bits;
+//     registers of the other way round.  The weights go in twice, in 16 bits and what these
+//     lose, and so count with 16 (bf16) or 22 (fp16) bits;
 //   - weights refer to an exponent that follows the maximum only when a score passes it by
 //     2^4: most tiles need one vote instead of a maximum over lanes and a pass over the
 //     accumulators;
@@ -565,6 +565,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
     // those down to 2^-34 of the largest; bf16 has fp32's range.
     constexpr float LIFT = HALF ? 10.0f : 0.0f, SLACK = 4.0f;
     constexpr float LOWEST = -3.0e38f;                   // no score yet
+    constexpr uint32_t LEAST = HALF ? 0x00010001u : 0x00800080u;     // 2^-24, 2^-126, twice
     constexpr int KSTEPS = DP/16, MBLK = L::MBLK, WARPS = L::WARPS, STAGES = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int nv_s[WARPS][STAGES];
@@ -1170,10 +1171,18 @@ paged_decode_kernel(const PagedDecodeArgs a)
                                 p[y] *= rel;
                             }
                         }
-                        const uint32_t up = pack2<M>(p[0], p[1]);
+                        // Values of T may be infinite, and 0 * inf is NaN: the first part is cut
+                        // off, and what is left is raised to LEAST where it is less, so that
+                        // both parts are positive where the weight is (from LEAST on).
+                        const uint32_t up = E4M3 ? pack2<M>(p[0], p[1]) : cut2<M>(p[0], p[1]);
                         const float2 kept = unpack2<M>(up);
+                        uint32_t rest = pack2<M>(p[0] - kept.x, p[1] - kept.y);
+                        if(!E4M3)
+                        {
+                            rest = max2<M>(rest, min2<M>(up, LEAST));
+                        }
                         pb[m][j][0][h] = transpose8x8(up);
-                        pb[m][j][1][h] = transpose8x8(pack2<M>(p[0] - kept.x, p[1] - kept.y));
+                        pb[m][j][1][h] = transpose8x8(rest);
                     }
                 }
             // ---- O += P V
