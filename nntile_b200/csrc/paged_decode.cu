@@ -561,9 +561,17 @@ paged_decode_kernel(const PagedDecodeArgs a)
     constexpr bool HALF = std::is_same<M, __half>::value;
     // A weight is exp2(score - reference).  The reference moves to LIFT below the largest score,
     // and only when a score passes that by more than SLACK: weights stay below
-    // 2^(LIFT + SLACK) and most tiles do without a maximum.  fp16 weights are lifted to keep
-    // those down to 2^-34 of the largest; bf16 has fp32's range.
-    constexpr float LIFT = HALF ? 10.0f : 0.0f, SLACK = 4.0f;
+    // 2^(LIFT + SLACK) and most tiles do without a maximum.  bf16 has fp32's range.  fp16 has
+    // not, so there the reference follows what the weights are multiplied with as well: for
+    // 8-bit rows the score with the exponent of the value row's scale, and rows of zeros, which
+    // may have all of the weight, do not count.  The largest weight times scale then is at least
+    // 2^LIFT, and another counts down to 2^-34 of it.  The sums, in fp32, take all weights: they
+    // may be DEEPEST binades above the reference, so that rows which count may be 2^80 smaller
+    // than others that do not.  Whole binades here and in the scales: nothing rounds.
+    constexpr float LIFT = HALF ? 10.0f : 0.0f, SLACK = HALF ? 5.5f : 4.0f, DEEPEST = 90.0f;
+    // 8-bit values: accumulators count in units of 2^(vref - 127).  vref begins at the scale of
+    // values around one and moves when a row's scale is more than SPREAD binades away.
+    constexpr int USUAL = 119, SPREAD = 60;
     constexpr float LOWEST = -3.0e38f;                   // no score yet
     constexpr uint32_t LEAST = HALF ? 0x00010001u : 0x00800080u;     // 2^-24, 2^-126, twice
     constexpr int KSTEPS = DP/16, MBLK = L::MBLK, WARPS = L::WARPS, STAGES = L::STAGES;
@@ -953,9 +961,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 for(int r = 0; r < 4; ++r)
                     acc[m][i][r] = 0.0f;
         }
-        // 8-bit values: the accumulators count in units of 2^(vref - 127), the largest value
-        // scale so far
-        int vref = 0;
+        int vref = USUAL;
 
         // N tiles at once.  Keys and values are the 16-row operand, the query heads the 8
         // columns: this lane holds the scores of positions n and n + 8 of a tile for heads 2t
@@ -1046,8 +1052,8 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         }
                 }
             }
-            // factors of the scores, by position and head
-            float factor[MT][N][2][2];
+            // factors of the scores, by position and head; what is over `limit` moves the reference
+            float factor[MT][N][2][2], limit[N][2];
             int vbyte[N][2];
             bool moved = false;
 #pragma unroll
@@ -1056,13 +1062,15 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 for(int h = 0; h < 2; ++h)
                 {
                     float kscale = 1.0f;
+                    limit[j][h] = LIFT + SLACK;
                     if(E4M3)
                     {
                         const uint8_t *sc = st[j] + 2*L::KV_BYTES + 8*h + n;
                         kscale = __uint_as_float((uint32_t)sc[0] << 23);
                         // the scale of a row behind the length may be anything: keep it out
-                        vbyte[j][h] = FULL || 8*h + n < nv[j] ? (int)sc[PD_TILE] : 0;
-                        moved = moved || vbyte[j][h] > vref;
+                        vbyte[j][h] = FULL || 8*h + n < nv[j] ? (int)sc[PD_TILE] : vref;
+                        moved = moved || vbyte[j][h] > vref + SPREAD;
+                        limit[j][h] = fminf(limit[j][h] - (float)(vbyte[j][h] - vref), DEEPEST);
                     }
 #pragma unroll
                     for(int m = 0; m < MT; ++m)
@@ -1086,23 +1094,121 @@ paged_decode_kernel(const PagedDecodeArgs a)
                             d = 8*(r >> 1) + n < nv[j] ? d : -CUDART_INF_F;
                         }
                         s[m][j][0][r] = d;
-                        moved = moved || d > LIFT + SLACK;
+                        moved = moved || d > limit[j][r >> 1];
                     }
             if(__any_sync(0xffffffffu, moved))
             {
-                float back = 1.0f;
-                if(E4M3)
+                // rows that are zero, scales far from vref: all that is unusual comes first
+                bool odd = false;
+                uint32_t blank = 0u;                     // bit 2j + h: the value row is zero
+                float back = 1.0f, least[MT][2];         // of accumulators, for references
+                if(HALF)
                 {
-                    int vtop = vref;
+                    constexpr uint32_t SIZE = E4M3 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
 #pragma unroll
                     for(int j = 0; j < N; ++j)
+#pragma unroll
+                        for(int h = 0; h < 2; ++h)
+                        {
+                            // four words of a row first, seldom are they zero
+                            const uint32_t some = *reinterpret_cast<const uint32_t *>(st[j]
+                                    + L::KV_BYTES + L::offset(8*h + n, t, false)) & SIZE;
+                            odd = odd || some == 0u
+                                    || (E4M3 && abs(vbyte[j][h] - vref) > SPREAD);
+                        }
+                    odd = __any_sync(0xffffffffu, odd);
+                }
+#pragma unroll
+                for(int m = 0; m < MT; ++m)
+#pragma unroll
+                    for(int y = 0; y < 2; ++y)
+                        least[m][y] = top[m][y];
+                if(HALF && __builtin_expect(odd, 0))
+                {
+                    constexpr uint32_t SIZE = E4M3 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
+#pragma unroll
+                    for(int j = 0; j < N; ++j)
+#pragma unroll
+                        for(int h = 0; h < 2; ++h)
+                        {
+                            uint32_t some = 0u;          // in this lane's quarter of the row
+#pragma unroll
+                            for(int c = 0; c < L::CHUNKS; c += 4)
+                            {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(st[j]
+                                        + L::KV_BYTES + L::offset(8*h + n, t + c, false));
+                                some |= (v.x | v.y | v.z | v.w) & SIZE;
+                            }
+                            blank |= some == 0u ? 1u << (2*j + h) : 0u;
+                        }
+                    blank &= __shfl_xor_sync(0xffffffffu, blank, 1);
+                    blank &= __shfl_xor_sync(0xffffffffu, blank, 2);
+                    int grown = 0;
+                    if(E4M3)
                     {
-                        vtop = max(vtop, max(vbyte[j][0], vbyte[j][1]));
+                        bool fresh = true;               // nothing is counted in vref yet
+#pragma unroll
+                        for(int m = 0; m < MT; ++m)
+                        {
+                            fresh = fresh && top[m][0] == LOWEST && top[m][1] == LOWEST;
+                        }
+                        fresh = __all_sync(0xffffffffu, fresh);
+                        int vtop = 0;
+#pragma unroll
+                        for(int j = 0; j < N; ++j)
+#pragma unroll
+                            for(int h = 0; h < 2; ++h)
+                                if((blank >> (2*j + h) & 1u) == 0u)
+                                {
+                                    vtop = max(vtop, vbyte[j][h]);
+                                }
+                        vtop = __reduce_max_sync(0xffffffffu, vtop);
+                        if(vtop > 0 && (fresh || vtop > vref + SPREAD))
+                        {
+                            grown = fresh ? 0 : vtop - vref;
+                            back = ex2(-(float)grown);
+                            vref = vtop;
+                        }
                     }
-                    vtop = __reduce_max_sync(0xffffffffu, vtop);
-                    const int e = vref - vtop + 127;
-                    back = __uint_as_float((uint32_t)max(e, 0) << 23);
-                    vref = vtop;
+#pragma unroll
+                    for(int j = 0; j < N; ++j)
+#pragma unroll
+                        for(int h = 0; h < 2; ++h)
+                        {
+                            const bool zero = (blank >> (2*j + h) & 1u) != 0u;
+                            if(E4M3)
+                            {
+                                vbyte[j][h] = zero ? vref : vbyte[j][h];
+                                limit[j][h] = LIFT + SLACK - (float)(vbyte[j][h] - vref);
+                            }
+                            limit[j][h] = zero ? CUDART_INF_F : limit[j][h];
+                        }
+                    // What vref grows by the references give way, as far as the sums, which are
+                    // in fp32, have room for.
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+#pragma unroll
+                        for(int y = 0; y < 2; ++y)
+                        {
+                            float all = -CUDART_INF_F, most = sum[m][y];
+#pragma unroll
+                            for(int j = 0; j < N; ++j)
+#pragma unroll
+                                for(int h = 0; h < 2; ++h)
+                                    if(FULL || 8*h + n < nv[j])
+                                    {
+                                        all = fmaxf(all, s[m][j][1][2*h + y]*factor[m][j][h][y]);
+                                    }
+#pragma unroll
+                            for(int o = 4; o < 32; o <<= 1)
+                            {
+                                all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                            }
+                            const float give = fminf((float)grown, 100.0f
+                                    - fmaxf(0.0f, ceilf(__log2f(most))));
+                            least[m][y] = fmaxf(top[m][y] - give, ceilf(all) - DEEPEST);
+                        }
                 }
 #pragma unroll
                 for(int m = 0; m < MT; ++m)
@@ -1118,18 +1224,20 @@ paged_decode_kernel(const PagedDecodeArgs a)
                             for(int h = 0; h < 2; ++h)
                                 if(FULL || 8*h + n < nv[j])
                                 {
-                                    ntop = fmaxf(ntop, s[m][j][1][2*h + y]*factor[m][j][h][y]);
+                                    ntop = fmaxf(ntop, fmaf(s[m][j][1][2*h + y],
+                                            factor[m][j][h][y], HALF ? -limit[j][h] : 0.0f));
                                 }
 #pragma unroll
                         for(int o = 4; o < 32; o <<= 1)
                         {
                             ntop = fmaxf(ntop, __shfl_xor_sync(0xffffffffu, ntop, o));
                         }
-                        ntop = fmaxf(top[m][y], ntop - LIFT);
+                        // fp16: LIFT below what is over the limit, on a whole binade
+                        ntop = fmaxf(least[m][y], HALF ? floorf(ntop + SLACK) : ntop - LIFT);
                         const float shrink = ntop == top[m][y] ? 1.0f : ex2(top[m][y] - ntop);
                         top[m][y] = ntop;
                         sum[m][y] *= shrink;
-                        f[y] = shrink*back;
+                        f[y] = E4M3 ? shrink*back : shrink;
 #pragma unroll
                         for(int j = 0; j < N; ++j)
 #pragma unroll
@@ -1145,6 +1253,21 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                         for(int r = 0; r < 4; ++r)
                             acc[m][i][r] *= f[r & 1];
+                }
+                if(HALF && __builtin_expect(odd, 0))
+                {
+                    // weights of rows of zeros: only in the sum
+#pragma unroll
+                    for(int m = 0; m < MT; ++m)
+#pragma unroll
+                        for(int j = 0; j < N; ++j)
+#pragma unroll
+                            for(int r = 0; r < 4; ++r)
+                                if((blank >> (2*j + (r >> 1)) & 1u) != 0u)
+                                {
+                                    sum[m][r & 1] += ex2(s[m][j][0][r]);
+                                    s[m][j][0][r] = -CUDART_INF_F;
+                                }
                 }
             }
             // ---- weights, in two 16-bit parts, as the 8-column operand of the second product
@@ -1309,11 +1432,26 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 {
                     sum[m][y] += __shfl_xor_sync(0xffffffffu, sum[m][y], o);
                 }
+            if(HALF)
+            {
+                // sums to [1, 2): what is joined by its reference has no need of more range
+                float f[2];
 #pragma unroll
-            for(int i = 0; i < MBLK; ++i)
+                for(int y = 0; y < 2; ++y)
+                {
+                    const int e = sum[m][y] == 0.0f ? 0
+                            : max(-120, min(120, (int)(__float_as_uint(sum[m][y]) >> 23) - 127));
+                    f[y] = __uint_as_float((uint32_t)(127 - e) << 23);
+                    sum[m][y] *= f[y];
+                    f[y] *= vscale;
+                    top[m][y] += (float)e;
+                }
 #pragma unroll
-                for(int r = 0; r < 4; ++r)
-                    acc[m][i][r] *= vscale;
+                for(int i = 0; i < MBLK; ++i)
+#pragma unroll
+                    for(int r = 0; r < 4; ++r)
+                        acc[m][i][r] *= f[r & 1];
+            }
             if(wpw > 1)
             {
                 if(n == 0)

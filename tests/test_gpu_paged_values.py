@@ -18,7 +18,7 @@ import pytest
 import torch
 
 from nntile_b200.sdpa import KVPages, paged_append, paged_decode
-from test_gpu_paged import DT, gen, ints, make_table, randn, stored, two_to
+from test_gpu_paged import DT, gen, ints, make_pool, make_table, randn, stored, two_to
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,162 @@ def test_infinite_values_stay_infinite(D, P, G, n, dtype):
     assert bool((out[0, :, 1, 0, 1] == -math.inf).all())
     sel = torch.tensor([0, (n - 1)//P, n//2//P, -1], dtype=torch.int32, device="cuda").unique()
     check(q, pages, lengths, table, sel.expand(H, 2, -1).contiguous())
+
+
+# ------------------------------------------------------- value rows of very different size
+
+SHAPES = [(64, 16, 1), (64, 32, 9), (128, 16, 4), (128, 64, 12), (256, 16, 2), (80, 16, 3), (96, 16, 9),
+          (72, 5, 3)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,P,G", SHAPES)
+@pytest.mark.parametrize("n", [16, 100, 5000])
+def test_a_row_of_zeros_that_takes_the_weight(n, D, P, G, e4m3, dtype):
+    """One position, first, in the middle or last, has all of the weight and no value: what is
+    left of the others is the answer, also when it is very little."""
+    dt, g = DT[dtype], gen(n + D + G)
+    B = 6
+    N = B*(-(-n//P))
+    pages = KVPages.empty(N, P, 1, D, dt, e4m3)
+    table, lengths = make_table(g, [n]*B, P, N), ints(*[n]*B)
+    k, v = 0.02*randn(g, 1, B, n, D), randn(g, 1, B, n, D)
+    q = randn(g, 1, G, B, 1, D).to(dt)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    for b, (at, gap) in enumerate([(0, 8), (0, 14), (n//2, 16), (n - 1, 20), (3, 30), (n//3, 45)]):
+        k[:, b, at] = 0.0
+        k[:, b, at, 0] = gap*math.sqrt(D)
+        v[:, b, at] = 0.0
+    # small enough for an 8-bit row of them to have a small scale, large enough for the output
+    v *= 0.02 if dtype == "bf16" else 2.0**13
+    fill(pages, table, lengths, k.to(dt), v.to(dt))
+    check(q, pages, lengths, table)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,P,G", SHAPES)
+@pytest.mark.parametrize("n", [40, 3000])
+def test_large_rows_without_weight(n, D, P, G, e4m3, dtype):
+    """Value rows up to 2^60 (bf16) or 2^29 (fp16) larger than the others whose weight is next to
+    nothing, at the beginning, the end and in between, several in a sequence."""
+    dt, g = DT[dtype], gen(n + D + 2*G)
+    apart = [20, 28, 36, 60] if dtype == "bf16" else [16, 22, 29, 29]
+    B = len(apart)
+    N = B*(-(-n//P))
+    pages = KVPages.empty(N, P, 2, D, dt, e4m3)
+    table, lengths = make_table(g, [n]*B, P, N), ints(*[n]*B)
+    k, v = 0.05*randn(g, 2, B, n, D), randn(g, 2, B, n, D)
+    q = randn(g, 2, G, B, 1, D).to(dt)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    small = 1.0 if dtype == "bf16" else 2.0**-14
+    v *= small
+    for b, x in enumerate(apart):
+        for at in (0, 5, n//2, n - 1):
+            v[:, b, at] *= 2.0**x/4
+            k[:, b, at, 0] = -(x*0.7 + 10)*math.sqrt(D)
+    fill(pages, table, lengths, k.to(dt), v.to(dt))
+    check(q, pages, lengths, table)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,P,G", SHAPES)
+@pytest.mark.parametrize("size", [1.0, 5.0, 12.0])
+def test_scores_of_wide_spread(size, D, P, G, e4m3, dtype):
+    """Scores over up to a hundred binades and value rows over twelve, rows of zeros among
+    them."""
+    dt, g = DT[dtype], gen(D + P + G)
+    lens = [1, 17, 300, 2100, 0, 33]
+    H, n = 2, max(lens)
+    N = sum(-(-x//P) for x in lens) + 1
+    pages = KVPages.empty(N, P, H, D, dt, e4m3)
+    table, lengths = make_table(g, lens, P, N), ints(*lens)
+    k, v = randn(g, H, len(lens), n, D), randn(g, H, len(lens), n, D)
+    v *= torch.exp2(torch.randint(-6, 7, (H, len(lens), n, 1), generator=g, device="cuda").float())
+    v[torch.rand((H, len(lens), n), generator=g, device="cuda") < 0.1] = 0.0
+    fill(pages, table, lengths, k.to(dt), v.to(dt))
+    check((size*randn(g, H, G, len(lens), 1, D)).to(dt), pages, lengths, table)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,P,G", SHAPES)
+@pytest.mark.parametrize("power", [-110, -70, -40, 50, 100])
+def test_values_of_any_size(power, D, P, G, e4m3):
+    """All of a cache's values are tiny or huge, a row of zeros with half of the weight first."""
+    g, lens = gen(D + G - power), [1, 30, 700]
+    N = sum(-(-x//P) for x in lens)
+    pages = KVPages.empty(N, P, 1, D, torch.bfloat16, e4m3)
+    table, lengths = make_table(g, lens, P, N), ints(*lens)
+    k, v = randn(g, 1, 3, 700, D), randn(g, 1, 3, 700, D)*2.0**power
+    v[:, 2, 0] = 0.0
+    k[:, 2, 0, 0] = 5*math.sqrt(D)
+    q = randn(g, 1, G, 3, 1, D)
+    q[..., 0] = 1.0
+    fill(pages, table, lengths, k.bfloat16(), v.bfloat16())
+    check(q.bfloat16(), pages, lengths, table)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,P,G", SHAPES)
+def test_rows_that_grow_as_their_weights_shrink(D, P, G, e4m3, dtype):
+    """Rows over 70 binades (fp16: 26) along the sequence, up and down, with weights that make
+    all of them count the same, or only the small ones."""
+    dt, g = DT[dtype], gen(D + 3*G)
+    n, span = 1500, 70 if dtype == "bf16" else 26
+    N = 4*(-(-n//P))
+    pages = KVPages.empty(N, P, 1, D, dt, e4m3)
+    table, lengths = make_table(g, [n]*4, P, N), ints(*[n]*4)
+    k, v = 0.1*randn(g, 1, 4, n, D), randn(g, 1, 4, n, D)
+    binades = torch.arange(n, device="cuda")/n*span - span/2
+    for b, (x, y) in enumerate([(binades, 1.0), (-binades, 1.0), (binades, 1.6), (-binades, 1.6)]):
+        v[0, b] *= torch.exp2(x.round())[:, None]
+        k[0, b, :, 0] = -y*x*math.log(2)*math.sqrt(D)
+    q = 0.1*randn(g, 1, G, 4, 1, D)
+    q[..., 0] = 1.0
+    fill(pages, table, lengths, k.to(dt), v.to(dt))
+    check(q.to(dt), pages, lengths, table)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_scores_that_rise_fall_and_rise(e4m3):
+    """The largest scores of a tile climb and sink by hundreds of binades along the sequence."""
+    g = gen(40)
+    D, P, G, n = 64, 16, 4, 4000
+    for dt in DT.values():
+        pages = KVPages.empty(n//P, P, 1, D, dt, e4m3)
+        table, lengths = make_table(g, [n], P, n//P), ints(n)
+        k, v = 0.1*randn(g, 1, 1, n, D), randn(g, 1, 1, n, D)
+        at = torch.arange(n, device="cuda")
+        k[..., 0] = 8*(100*torch.sin(at/300.0) + 20*torch.sin(at/37.0))
+        q = randn(g, 1, G, 1, 1, D)
+        q[..., 0] = torch.tensor([1.0, -1.0, 0.25, 0.0], device="cuda")[:, None, None]
+        fill(pages, table, lengths, k.to(dt), v.to(dt))
+        check(q.to(dt), pages, lengths, table)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,P,G,lens", [(64, 16, 1, [1, 5, 130]), (128, 64, 8, [65, 700]), (256, 16, 2, [35]),
+                                        (96, 32, 12, [33, 1000])])
+def test_scales_behind_a_sequence_hold_anything(D, P, G, lens, dtype):
+    dt, g = DT[dtype], gen(D + 7)
+    N = sum(-(-x//P) for x in lens) + 2
+    pages = make_pool(g, N, P, 2, D, dt, True)
+    table, lengths = make_table(g, lens, P, N), ints(*lens)
+    q = randn(g, 2, G, len(lens), 1, D).to(dt)
+    live = torch.zeros((N, P), dtype=torch.bool, device="cuda")
+    for b, x in enumerate(lens):
+        for i in range(x):
+            live[int(table[b, i//P]), i % P] = True
+    want = check(q, pages, lengths, table)
+    for byte in (0, 1, 254, 255):
+        for t in (pages.k_scales, pages.v_scales):
+            t.masked_fill_(~live[:, None], byte)
+        assert torch.equal(paged_decode(q, pages, lengths, table), want)
+    for t in (pages.k, pages.v):
+        t.masked_fill_(~live[:, None, :, None], 0x7F)
+    assert torch.equal(paged_decode(q, pages, lengths, table), want)
