@@ -82,4 +82,11 @@ NB200_HD int held_block(int block, int blocks, int max_blocks, bool &bad)
     return block >= 0 && block < blocks ? block : -1;
 }
 
+// End of the list positions that split `split` of `chunk` positions each takes.
+NB200_HD int split_end(int listed, int split, int chunk)
+{
+    const int64_t end = ((int64_t)split + 1)*chunk;
+    return end < listed ? (int)end : listed;
+}
+
 } // namespace nb200

@@ -90,7 +90,7 @@ paged_decode_generic_kernel(const PagedDecodeArgs a)
         o[x] = 0.0f;
     }
     float top = -CUDART_INF_F, sum = 0.0f;
-    const int j_end = min(listed, (split + 1)*a.chunk);
+    const int j_end = split_end(listed, split, a.chunk);
     for(int j = split*a.chunk; j < j_end; ++j)
     {
         int block = j;
