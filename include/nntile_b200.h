@@ -486,7 +486,8 @@ size_t nntile_b200_paged_decode_sdpa_workspace_bytes(int64_t head, int64_t page_
  * block without a page as the lowest.  Scores are compared as sums in 64 bits.  Tables of
  * sequences that are taken whole are not read.  `selected` (int32 [num_selected, batch,
  * kv_heads]) receives the block numbers in
- * ascending order, then -1.  first_blocks + last_blocks <= num_selected.  `workspace`:
+ * ascending order, then -1.  first_blocks + last_blocks <= num_selected; max_blocks and
+ * num_selected up to 2^30.  `workspace`:
  * nntile_b200_paged_select_workspace_bytes(...) bytes, 16-byte aligned, of any content. */
 int nntile_b200_paged_select_bf16(nntile_b200_stream_t stream, int64_t head,
         int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,

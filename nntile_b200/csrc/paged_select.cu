@@ -1069,6 +1069,10 @@ paged_pick_kernel(const PagedSelectArgs a)
     }
 }
 
+// Blocks of a table and of a selection: loops of the kernels here step past their ends, in 32
+// bits.
+constexpr int64_t SELECT_MOST = (int64_t)1 << 30;
+
 static size_t select_bytes(int64_t units, int64_t max_blocks)
 {
     return (size_t)units*max_blocks*(sizeof(float2) + sizeof(unsigned long long));
@@ -1141,7 +1145,11 @@ static int select_impl(nntile_b200_stream_t stream, int64_t head, int64_t page_s
     {
         return NNTILE_B200_E_BADARG;
     }
-    if(group > 1 << 16 || batch*kv_heads*group > 1 << 24) return NNTILE_B200_E_SHAPE;
+    if(group > 1 << 16 || batch*kv_heads*group > 1 << 24 || max_blocks > SELECT_MOST
+            || num_selected > SELECT_MOST)
+    {
+        return NNTILE_B200_E_SHAPE;
+    }
     if(batch == 0 || group == 0 || kv_heads == 0 || num_selected == 0) return NNTILE_B200_OK;
     if(!lengths || !q || !selected || !workspace || (max_blocks > 0 && !block_table)
             || (num_pages > 0 && !bounds))
@@ -1205,7 +1213,7 @@ extern "C" size_t nntile_b200_paged_select_workspace_bytes(int64_t max_blocks, i
         int64_t kv_heads)
 {
     if(check_paged(1, 1, 0, max_blocks, batch, kv_heads, NNTILE_B200_PAGES_SAME)
-            != NNTILE_B200_OK)
+            != NNTILE_B200_OK || max_blocks > SELECT_MOST)
     {
         return 0;
     }
