@@ -315,6 +315,7 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t n)
         check_query(q, p);
         check(p.bounds && p.bounds->scalar_type() == q.scalar_type() && count >= 0);
         const int64_t group = q.size(1), batch = q.size(2);
+        check(group > 0 || given);               // otherwise there is a result to fill in
         const int64_t blocks = table_blocks(lengths, table, batch);
         check(!given || (given->scalar_type() == at::kInt && given->dim() == 3
                 && given->size(0) == p.kv_heads && given->size(1) == batch

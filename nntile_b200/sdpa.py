@@ -587,6 +587,8 @@ def paged_select(q, pages, lengths, block_table, num_selected, first_blocks=1, l
     _check_status(status)
     if out is None:
         out = torch.empty((H, B, num_selected), dtype=torch.int32, device=q.device)
+        if G == 0:                              # no query, nothing selected: the call writes nothing
+            out.fill_(-1)
     elif out.shape != (H, B, num_selected) or out.dtype != torch.int32:
         raise ValueError("out must be int32 (kv_heads, batch, num_selected)")
     if workspace is None:
