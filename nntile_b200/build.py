@@ -24,6 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libnntile_b200.so")
 TORCH_MODULE = os.path.join(HERE, "_paged_torch.so")
+TORCH_STAMP = os.path.join(OBJ_DIR, "paged_torch.version")
 SOURCES = [
     "vanilla_ops.cu", "flash_generic.cu", "flash_api.cu", "decode.cu",
     "flash_fwd_sm100.cu", "flash_bwd_sm100.cu", "host_tensor.cu", "gemm_cublas.cu",
@@ -75,14 +76,28 @@ def _compile(job, force: bool) -> str:
     return obj
 
 
-def _build_torch_module(force: bool) -> str:
-    """The extension module; it finds the library beside it and torch's in the process."""
+def _torch_version() -> str:
+    """What the extension module is made for: it uses the internals of both."""
+    import torch
+    return f"Python {sys.version} torch {torch.__version__}"
+
+
+def _torch_module_stale() -> bool:
     src = os.path.join(CSRC, "paged_torch.cpp")
     header = os.path.join(os.path.dirname(HERE), "include", "nntile_b200.h")
-    if force or _stale(TORCH_MODULE, [src, header]):
+    if _stale(TORCH_MODULE, [src, header]) or not os.path.exists(TORCH_STAMP):
+        return True
+    with open(TORCH_STAMP) as f:
+        return f.read() != _torch_version()
+
+
+def _build_torch_module(force: bool) -> str:
+    """The extension module; it finds the library beside it and torch's in the process."""
+    if force or _torch_module_stale():
         import sysconfig
 
         import torch
+        src = os.path.join(CSRC, "paged_torch.cpp")
         base = os.path.dirname(torch.__file__)
         cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -95,6 +110,8 @@ def _build_torch_module(force: bool) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"g++ failed on paged_torch.cpp:\n{res.stdout}{res.stderr}")
+        with open(TORCH_STAMP, "w") as f:
+            f.write(_torch_version())
     return TORCH_MODULE
 
 
