@@ -17,17 +17,30 @@ from __future__ import annotations
 import ctypes
 import itertools
 import math
+import os
+import warnings
 
 import numpy as np
 import torch
 
-from . import _lib, ops
-try:
-    # the paged calls without the interpreter between the tensors and the library; what it
-    # does not take (and every mistake) goes the way through ops
-    from . import _paged_torch
-except ImportError:
-    _paged_torch = None
+from . import _lib, build, ops
+
+
+def _load_paged_torch():
+    """The paged calls without the interpreter between the tensors and the library; what the
+    module does not take (and every mistake) goes the way through ops, as everything does when
+    it was not built.  One that was built and does not load is said."""
+    try:
+        from . import _paged_torch
+        return _paged_torch
+    except ImportError as e:
+        if os.path.exists(build.TORCH_MODULE):
+            warnings.warn(f"{build.TORCH_MODULE} does not load ({e}): paged calls take longer on the "
+                          "host. Build it again: python -m nntile_b200.build", RuntimeWarning)
+        return None
+
+
+_paged_torch = _load_paged_torch()
 
 
 def from_fortran(arr: np.ndarray, device="cuda") -> torch.Tensor:
