@@ -19,8 +19,8 @@
 //   - scores and weighted values go through the warp-level tensor instruction (m16n8k16, fp32
 //     accumulate), transposed: keys and columns of V are its 16 rows, 8 query heads its
 //     columns, so no row is idle for groups up to 8 and the accumulators take half the
-//     registers of the other way round.  The weights go in twice, in 16 bits and what these
-//     lose, and so count with 16 (bf16) or 22 (fp16) bits;
+//     registers of the other way round.  The weights go in twice (fp16) or three times (bf16),
+//     in 16 bits and what these lose, and so count with 22 or 24 bits;
 //   - weights refer to an exponent that follows the maximum only when a score passes it by
 //     2^4: most tiles need one vote instead of a maximum over lanes and a pass over the
 //     accumulators;
@@ -362,6 +362,30 @@ __device__ __forceinline__ void mma16<__half>(float (&c)[4], uint32_t a0, uint32
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// a + b and a - b of two values an instruction
+__device__ __forceinline__ void plus2(float (&r)[2], const float (&a)[2], const float (&b)[2])
+{
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+            "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(r[0]), "=f"(r[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+__device__ __forceinline__ void minus2(float (&r)[2], const float (&a)[2], const float (&b)[2])
+{
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+            "sub.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(r[0]), "=f"(r[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+// c += o, two values an instruction
+__device__ __forceinline__ void add4(float (&c)[4], const float (&o)[4])
+{
+#pragma unroll
+    for(int i = 0; i < 4; i += 2)
+    {
+        asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+                "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+                : "+f"(c[i]), "+f"(c[i + 1]) : "f"(o[i]), "f"(o[i + 1]));
+    }
+}
 // transposes an 8x8 matrix of 16-bit values held as an accumulator's words
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t w)
 {
@@ -573,8 +597,13 @@ paged_decode_kernel(const PagedDecodeArgs a)
     // values around one and moves when a row's scale is more than SPREAD binades away.
     constexpr int USUAL = 119, SPREAD = 60;
     constexpr float LOWEST = -3.0e38f;                   // no score yet
+    constexpr int PARTS = HALF ? 2 : 3;                  // a weight's 16-bit pieces
     constexpr uint32_t LEAST = HALF ? 0x00010001u : 0x00800080u;     // 2^-24, 2^-126, twice
     constexpr int KSTEPS = DP/16, MBLK = L::MBLK, WARPS = L::WARPS, STAGES = L::STAGES;
+    // Two tiles of heads are two chains already, and leave no registers for more (300 MB of 8-bit
+    // rows of 128, group 16, a ragged batch of 64: 79 us, with two tiles of positions 91).
+    constexpr int ABREAST = MT == 2 && L::ABREAST > 1 ? L::ABREAST/2 : L::ABREAST;
+    constexpr int AHEAD = STAGES - ABREAST;              // tiles in flight or waiting
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int nv_s[WARPS][STAGES];
     __shared__ float top_s[WARPS][8], sum_s[WARPS][8];
@@ -877,7 +906,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
         copy_commit();
     };
 #pragma unroll 1
-    for(int s = 0; s < L::AHEAD; ++s)
+    for(int s = 0; s < AHEAD; ++s)
     {
         issue(s);                                        // once in the code: it is long
     }
@@ -949,12 +978,13 @@ paged_decode_kernel(const PagedDecodeArgs a)
                     }
             }
         }
-        float acc[MT][MBLK][4], top[MT][2], sum[MT][2];
+        // the sum of weights is sum - over
+        float acc[MT][MBLK][4], top[MT][2], sum[MT][2], over[MT][2];
 #pragma unroll
         for(int m = 0; m < MT; ++m)
         {
             top[m][0] = top[m][1] = LOWEST;
-            sum[m][0] = sum[m][1] = 0.0f;
+            sum[m][0] = sum[m][1] = over[m][0] = over[m][1] = 0.0f;
 #pragma unroll
             for(int i = 0; i < MBLK; ++i)
 #pragma unroll
@@ -973,7 +1003,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
             constexpr bool FULL = decltype(filled)::value;
             const uint8_t *st[N];
             int nv[N];
-            int to = stage + L::AHEAD;
+            int to = stage + AHEAD;
             to -= to >= STAGES ? STAGES : 0;
 #pragma unroll 1
             for(int j = 0; j < N; ++j)
@@ -1237,6 +1267,7 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         const float shrink = ntop == top[m][y] ? 1.0f : ex2(top[m][y] - ntop);
                         top[m][y] = ntop;
                         sum[m][y] *= shrink;
+                        over[m][y] *= shrink;
                         f[y] = E4M3 ? shrink*back : shrink;
 #pragma unroll
                         for(int j = 0; j < N; ++j)
@@ -1270,8 +1301,12 @@ paged_decode_kernel(const PagedDecodeArgs a)
                                 }
                 }
             }
-            // ---- weights, in two 16-bit parts, as the 8-column operand of the second product
-            uint32_t pb[MT][N][2][2];                    // part, positions >= 8
+            // ---- weights, in 16-bit parts, as the 8-column operand of the second product
+            uint32_t pb[MT][N][PARTS][2];                // part, positions >= 8
+            float more[MT][2];                           // to the sums
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+                more[m][0] = more[m][1] = 0.0f;
 #pragma unroll
             for(int j = 0; j < N; ++j)
 #pragma unroll
@@ -1288,26 +1323,49 @@ paged_decode_kernel(const PagedDecodeArgs a)
                         for(int y = 0; y < 2; ++y)
                         {
                             p[y] = ex2(s[m][j][0][2*h + y]);
-                            sum[m][y] += p[y];
+                            more[m][y] += p[y];
                             if(E4M3)
                             {
                                 p[y] *= rel;
                             }
                         }
-                        // Values of T may be infinite, and 0 * inf is NaN: the first part is cut
-                        // off, and what is left is raised to LEAST where it is less, so that
-                        // both parts are positive where the weight is (from LEAST on).
-                        const uint32_t up = E4M3 ? pack2<M>(p[0], p[1]) : cut2<M>(p[0], p[1]);
-                        const float2 kept = unpack2<M>(up);
-                        uint32_t rest = pack2<M>(p[0] - kept.x, p[1] - kept.y);
-                        if(!E4M3)
+                        // Values of T may be infinite, and 0 * inf is NaN: all parts but the last
+                        // are cut off, and those after the first raised to LEAST where they
+                        // are less, so that all are positive where the weight is (from LEAST on).
+                        uint32_t up = 0u;
+#pragma unroll
+                        for(int part = 0; part < PARTS; ++part)
                         {
-                            rest = max2<M>(rest, min2<M>(up, LEAST));
+                            uint32_t w = E4M3 || part == PARTS - 1 ? pack2<M>(p[0], p[1])
+                                    : cut2<M>(p[0], p[1]);
+                            if(part == 0)
+                            {
+                                up = w;
+                            }
+                            else if(!E4M3)
+                            {
+                                w = max2<M>(w, min2<M>(up, LEAST));
+                            }
+                            pb[m][j][part][h] = transpose8x8(w);
+                            const float2 kept = unpack2<M>(w);
+                            p[0] -= kept.x;
+                            p[1] -= kept.y;
                         }
-                        pb[m][j][0][h] = transpose8x8(up);
-                        pb[m][j][1][h] = transpose8x8(rest);
                     }
                 }
+            // Like weights, thousands of them, would all round the same way (2^-14 of the sum of
+            // 131072): what a sum takes too much is kept and taken off again.
+#pragma unroll
+            for(int m = 0; m < MT; ++m)
+            {
+                float part[2], next[2];
+                minus2(part, more[m], over[m]);
+                plus2(next, sum[m], part);
+                minus2(over[m], next, sum[m]);
+                minus2(over[m], over[m], part);
+                sum[m][0] = next[0];
+                sum[m][1] = next[1];
+            }
             // ---- O += P V
 #pragma unroll
             for(int j = 0; j < N; ++j)
@@ -1324,9 +1382,19 @@ paged_decode_kernel(const PagedDecodeArgs a)
 #pragma unroll
                         for(int m = 0; m < MT; ++m)
 #pragma unroll
-                            for(int part = 0; part < 2; ++part)
-                                mma16<M>(acc[m][i], va[0], va[1], va[2], va[3],
-                                        pb[m][j][part][0], pb[m][j][part][1]);
+                        {
+                            // The instruction cuts its sums off, always downwards in size; over
+                            // a long chain that adds up (means of 131072 fp16 positions: one in
+                            // three not the nearest number).  So a tile's sum, smallest parts
+                            // first, is added as an ordinary fp32 number (64 sequences of 8192:
+                            // 325 -> 331 us, 37 ragged ones in 8 bits 134 -> 137).
+                            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for(int part = PARTS - 1; part >= 0; --part)
+                                mma16<M>(o, va[0], va[1], va[2], va[3], pb[m][j][part][0],
+                                        pb[m][j][part][1]);
+                            add4(acc[m][i], o);
+                        }
                     }
                 }
                 else
@@ -1373,10 +1441,14 @@ paged_decode_kernel(const PagedDecodeArgs a)
                                 const int i = 8*q4 + 2*w + pair;
 #pragma unroll
                                 for(int m = 0; m < MT; ++m)
+                                {
+                                    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                                    for(int part = 0; part < 2; ++part)
-                                        mma16<M>(acc[m][i], a0, a1, a2, a3, pb[m][j][part][0],
+                                    for(int part = PARTS - 1; part >= 0; --part)
+                                        mma16<M>(o, a0, a1, a2, a3, pb[m][j][part][0],
                                                 pb[m][j][part][1]);
+                                    add4(acc[m][i], o);
+                                }
                             }
                     }
                 }
@@ -1384,25 +1456,25 @@ paged_decode_kernel(const PagedDecodeArgs a)
         };
         while(mine < seg_end)
         {
-            copy_wait<L::AHEAD - L::ABREAST>();
+            copy_wait<AHEAD - ABREAST>();
             // every lane's copies are there, and what was consumed last is free
             __syncwarp();
-            bool full = L::ABREAST > 1 && mine + (L::ABREAST - 1)*step < seg_end;
+            bool full = ABREAST > 1 && mine + (ABREAST - 1)*step < seg_end;
             int at = stage;
 #pragma unroll
-            for(int j = 0; j < L::ABREAST; ++j)
+            for(int j = 0; j < ABREAST; ++j)
             {
                 full = full && nv_s[warp][at] == PD_TILE;
                 at = at + 1 == STAGES ? 0 : at + 1;
             }
-            if(L::ABREAST == 1)
+            if(ABREAST == 1)
             {
                 full = nv_s[warp][stage] == PD_TILE;
             }
             if(full)
             {
-                mine += L::ABREAST*step;
-                process(std::integral_constant<int, L::ABREAST>(), std::true_type());
+                mine += ABREAST*step;
+                process(std::integral_constant<int, ABREAST>(), std::true_type());
             }
             else
             {
@@ -1427,11 +1499,14 @@ paged_decode_kernel(const PagedDecodeArgs a)
         {
 #pragma unroll
             for(int y = 0; y < 2; ++y)
+            {
+                sum[m][y] -= over[m][y];
 #pragma unroll
                 for(int o = 4; o < 32; o <<= 1)
                 {
                     sum[m][y] += __shfl_xor_sync(0xffffffffu, sum[m][y], o);
                 }
+            }
             if(HALF)
             {
                 // sums to [1, 2): what is joined by its reference has no need of more range
