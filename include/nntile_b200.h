@@ -436,7 +436,9 @@ int nntile_b200_paged_kv_append_fp16(nntile_b200_stream_t stream, int64_t head,
 
 /* Read a cache back: k, v (T [head, max_seq, batch, kv_heads]) rows 0 .. lengths[b] - 1 of
  * every sequence, e4m3 values rounded once to T; rows behind are left as they are.  A
- * length above max_seq is cut there (PAGED_BAD_LENGTH). */
+ * length above max_seq is cut there (PAGED_BAD_LENGTH).  The e4m3 value of an fp16 element of
+ * 63488 or more is 65536, which is an infinity in fp16, here and in the bounds; the attention
+ * reads it as 65536. */
 int nntile_b200_paged_kv_gather_bf16(nntile_b200_stream_t stream, int64_t head,
         int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch,
         int64_t kv_heads, int64_t max_seq, int page_format, const int32_t *lengths,
@@ -456,8 +458,11 @@ int nntile_b200_paged_kv_gather_fp16(nntile_b200_stream_t stream, int64_t head,
  * nntile_b200_paged_select_* writes it) take part: a negative entry and a block behind the
  * sequence's length add nothing, a block that is listed twice counts twice, the order is
  * free.  Nothing to attend to (length 0, an empty selection, scores that are all -inf):
- * out = 0, lse = -inf.  `workspace`: nntile_b200_paged_decode_sdpa_workspace_bytes(...) bytes, 16-byte
- * aligned, of any content; calls that may overlap on the GPU need workspaces of their own.
+ * out = 0, lse = -inf.  Scores and sums are fp32; a weight counts with 24 bits (bf16 rows) or 22
+ * (fp16 and e4m3 rows), these down to 2^-34 of the largest weight of the sequence, e4m3 rows
+ * taken with their scale, rows of zeros left out.  An infinite value makes its column infinite,
+ * and NaN where its weight is below that (bf16: below 2^-126).  `workspace`:
+ * nntile_b200_paged_decode_sdpa_workspace_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the GPU need workspaces of their own.
  * Results do not depend on the order in which CTAs run. */
 int nntile_b200_paged_decode_sdpa_bf16(nntile_b200_stream_t stream, int64_t head,
         int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,

@@ -25,14 +25,18 @@
 //     2^4: most tiles need one vote instead of a maximum over lanes and a pass over the
 //     accumulators;
 //   - 8-bit rows are widened to fp16, exactly, on their way into the operands; their scales go
-//     into scores and weights, where they are powers of two.
+//     into scores and weights, where they are powers of two;
+//   - sums are fp32 and round to nearest: a tile's products leave the tensor instruction, which
+//     cuts off, before they are added to the others, and sums of weights are compensated.
 //
 // Measured on one B200 (copy bandwidth 6 553 GB/s), head 128: 64 sequences of 8192, 8 kv heads,
-// group 4, bf16: 326-330 us, 6.5 TB/s; 37 sequences of up to 16383, e4m3, group 8: 135-150 us,
-// 5.1-5.7 TB/s; one of 100003, 2 kv heads, group 7, fp16: 18-19 us, 5.4-5.6 TB/s, of which
-// 15.6 us are the bytes and the rest the start (length, page and first row, one after the
-// other) and the joining.  With 8-bit heads of 64 the instructions bound it (300 MB in 76 us, the
-// copies alone 54), with 16-bit rows the copies do.
+// group 4, bf16: 332-338 us, 6.4 TB/s; 37 sequences of up to 16383, e4m3, group 8: 138-158 us,
+// 4.9-5.6 TB/s; one of 100003, 2 kv heads, group 7, fp16: 25 us, 4.1 TB/s, of which 15.6 us are
+// the bytes and the rest the start (length, page and first row, one after the other), the
+// slowest SM and the joining (18-19 us where the cache, 102 MB, is in L2 from the call before).
+// With 8-bit heads of 64 the instructions bound it (300 MB in 75 us), with 16-bit rows the copies
+// do.  The choices below were measured with inputs that together exceed L2, unless they say
+// otherwise.
 #include <algorithm>
 #include <type_traits>
 
@@ -252,12 +256,13 @@ paged_decode_join_kernel(const PagedDecodeArgs a, int heads)
 constexpr int PD_SMS = 148;
 constexpr int PD_TILE = 16;                  // positions of a tile
 // Sequences up to which a warp adds up their tiles by itself: against the block's prefix sums
-// 21.6 us and 22.2 for one, 15.7 and 16.1 for 33, 72.6 and 72.3 for 100.
+// 25.6 us and 26.5 for one of 100003, 15.1 and 17.2 for 33 of 2000, 90.7 and 91.6 for 64 of 2000
+// with 8 kv heads.
 constexpr int PD_BATCH = 64;
 
 // Warps of a block, one block per SM: with four, 16-bit rows of 256 columns still have three
 // tiles (48 KB) a warp in the ring; their 8-bit rows are bound by instructions and take eight
-// (66 us for 300 MB against 79 with four).
+// (59 us for 300 MB against 72 with four).
 __host__ __device__ constexpr int paged_warps(bool e4m3, int dp)
 {
     return dp == 256 && !e4m3 ? 4 : 8;
@@ -277,15 +282,15 @@ struct PagedTile
     static constexpr int STAGES = RING/STAGE < 12 ? RING/STAGE : 12;
     // Tiles a warp takes at once.  A tile is one chain (scores, weights, values) of several
     // hundred cycles; short rows put two or four side by side, so that 8 warps ask for bytes
-    // as fast as HBM delivers them (8-bit heads of 64 with four 77 us for 300 MB, with two 83;
-    // 8-bit heads of 128 with two 64, with one 69; 16 warps instead were no faster).
+    // as fast as HBM delivers them (8-bit heads of 64 with four 75 us for 300 MB, with two 82;
+    // 8-bit heads of 128 with two 61, with one 65; 16-bit heads of 64 with two 55, with one 56).
     static constexpr int ABREAST = 8192/(2*KV_BYTES) < 1 ? 1 : 8192/(2*KV_BYTES);
     static constexpr int AHEAD = STAGES - ABREAST;       // tiles in flight or waiting
     static_assert(AHEAD >= ABREAST, "the ring must hold what is consumed and what is coming");
     static constexpr int MBLK = DP/16;                   // 16-column blocks of the output
     // One tile of 8 heads of every warp, for 256 columns in two rounds: with 16-bit rows of
     // 256 that leaves an SM room for blocks of the joining kernel, which then wait beside this
-    // one (16 kv heads of 512 positions 11.1 -> 8.7 us).  With 128 columns the second round
+    // one (16 kv heads of 512 positions 12.1 -> 11.3 us).  With 128 columns the second round
     // costs as much as it gains.
     static constexpr int ROUNDS = DP == 256 ? 2 : 1;
     static constexpr int MERGE = WARPS*8*DP*4/ROUNDS;
@@ -555,10 +560,11 @@ __device__ __forceinline__ int pieces_of(int tiles, int size)
 // Shares that end where units end.  A worker whose share reaches into a second unit starts and
 // ends twice, 2 us; it is cheaper to cut every unit into pieces of at most `size` tiles, a
 // worker each, when there are workers for that with a size at or little above the even share
-// (bf16, head 128, even shares against pieces: 32 units of 3000 positions 14.2 and 12.5 us, 144
-// units of 3000 in e4m3 30.9 and 26.7; pieces half as large again as the share lose: 96 units
-// of 2048 19.2 and 22.7).  Working it out costs 0.5 us where nothing is gained: 8 units of 512
-// 7.4 and 8.1.  Returns that size, or 0.  t0, t1: tiles of a unit of sequences lane, lane + 32.
+// (bf16, head 128, even shares against pieces: 32 units of 3000 positions 18.1 and 16.6 us, 144
+// units of 3000 in e4m3 32.9 and 28.9; pieces half as large again as the share lose: 96 units
+// of 2048, in L2, 19.2 and 22.7).  Working it out costs 0.5 us where nothing is gained: 8 units of
+// 512 8.2 and 8.7, 96 of 2048 25.2 and 25.7.  Returns that size, or 0.  t0, t1: tiles of a unit of
+// sequences lane, lane + 32.
 template<int WARPS>
 __device__ __forceinline__ int piece_size(int t0, int t1, int units_per_seq, int total,
         int workers)
@@ -1824,9 +1830,9 @@ static PagedDecodePlan paged_decode_plan(int64_t head, int64_t page_size, int64_
         p.wpw = units >= 2*PD_SMS ? 1 : warps;
         // Whole units, nothing to join: short ones always; longer ones when they about fill
         // the SMs once, where a block streams a unit in the time that splitting and joining
-        // add.  Measured (bf16, head 128, group 4, whole against split): 512 positions 7.5
-        // against 10.8 us at 64 units and 7.7 against 11.4 at 144, 1024 positions 10.1 against
-        // 12.1 and 10.5 against 14.1; 2048 positions 15.3 against 13.9 and 26.6 against 29.0.
+        // add.  Measured (bf16, head 128, group 4, whole against split): 512 positions 9.7
+        // against 12.6 us at 64 units and 11.8 against 14.5 at 144, 1024 positions 13.3 against
+        // 14.9 and 16.8 against 19.4; 2048 positions 20.5 against 19.4 and 27.8 against 30.5.
         // Selections are equally long for all units, so that there more of them may be whole.
         const bool fills = units >= PD_SMS/3 && units <= PD_SMS;
         const bool even = num_selected > 0 && units >= 2*PD_SMS/3;
@@ -1901,8 +1907,9 @@ static int launch_fast(cudaStream_t s, const PagedDecodeArgs &a, const PagedDeco
     const int htiles = (a.group + 8*MT - 1)/(8*MT);
     // warps a piece: about as many as it has parts by fours, were the lengths even; with
     // uneven ones a unit may have more, so never one alone when blocks are the workers.
-    // Measured with 8, 16 and 32 (bf16, head 128, group 4): 64 parts 8.5, 8.2 and 8.8 us, 74
-    // parts 13.0, 12.7 and 12.7, 148 parts 10.8, 10.4 and 9.7; 18 parts 7.8 and 8.4 with 8 and 16.
+    // Measured with 8, 16 and 32 (bf16, head 128, group 4): 64 parts 10.4, 9.9 and 10.6 us, 74
+    // parts 26.8, 25.4 and 25.5, 148 parts 18.5, 18.1 and 17.7; 18 parts 10.4 and 10.8 with 8 and
+    // 16.
     const int64_t units = (int64_t)a.batch*a.kv_heads*htiles;
     const int wpp = a.wpw == 1 ? 1 : plan.grid <= 3*units ? 4 : plan.grid <= 20*units ? 8
             : plan.grid <= 72*units ? 16 : 32;

@@ -16,8 +16,9 @@
 // 32*17*2^-23 < 2^-13 of sum_d |q_d||k_d|, which a second product of magnitudes delivers.
 //
 // Measured on one B200: 128 of up to 2049 blocks for 24 sequences and 8 kv heads of 128 (85.6 MB
-// of bounds): 29-31 us, of which the scores are 20 and the ranking the rest, a chain of a
-// dozen short passes; 64 of 4096 blocks of one sequence with the attention over them: 27 us.
+// of bounds): 31-32 us, of which the scores are 20 and the ranking the rest, a chain of a
+// dozen short passes; 64 of 4096 blocks of one sequence with the attention over them: 28 us, 30
+// when the cache is not in L2.
 // Scoring everything in 64 bits instead took 240 us for the first.
 #include <algorithm>
 #include <cfloat>
@@ -919,7 +920,8 @@ paged_pick_kernel(const PagedSelectArgs a)
             }
             else
             {
-                // one by one, near or not: this is for rows of NaN and infinities
+                // More than the list holds: rows of NaN and infinities, a query of zeros, blocks
+                // whose bounds are all alike.  Every block is summed again, near or not.
                 for(int i0 = begin; i0 < end; i0 += PICK_LIST)
                 {
                     const int count = min(PICK_LIST, end - i0);
