@@ -1380,27 +1380,42 @@ paged_decode_kernel(const PagedDecodeArgs a)
                 if(!E4M3)
                 {
                     const int r = (lane & 7) + ((lane >> 4) << 3), col = (lane >> 3) & 1;
+                    // Four blocks of columns side by side, each a chain of PARTS products (300 MB of
+                    // heads of 256, group 16: 82 us, one after the other 92).
+                    constexpr int SIDE = 4;
 #pragma unroll
-                    for(int i = 0; i < MBLK; ++i)
+                    for(int i0 = 0; i0 < MBLK; i0 += SIDE)
                     {
-                        uint32_t va[4];
-                        ldmatrix4_trans(va, smem_addr(sv + L::offset(r, 2*i + col, false)));
+                        uint32_t va[SIDE][4];
+                        float o[SIDE][MT][4];
 #pragma unroll
-                        for(int m = 0; m < MT; ++m)
+                        for(int i = 0; i < SIDE; ++i)
+                            ldmatrix4_trans(va[i], smem_addr(sv + L::offset(r, 2*(i0 + i) + col,
+                                    false)));
+                        // The instruction cuts its sums off, always downwards in size; over
+                        // a long chain that adds up (means of 131072 fp16 positions: one in
+                        // three not the nearest number).  So a tile's sum, smallest parts
+                        // first, is added as an ordinary fp32 number (64 sequences of 8192:
+                        // 325 -> 331 us, 37 ragged ones in 8 bits 134 -> 137).
 #pragma unroll
-                        {
-                            // The instruction cuts its sums off, always downwards in size; over
-                            // a long chain that adds up (means of 131072 fp16 positions: one in
-                            // three not the nearest number).  So a tile's sum, smallest parts
-                            // first, is added as an ordinary fp32 number (64 sequences of 8192:
-                            // 325 -> 331 us, 37 ragged ones in 8 bits 134 -> 137).
-                            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for(int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                            for(int part = PARTS - 1; part >= 0; --part)
-                                mma16<M>(o, va[0], va[1], va[2], va[3], pb[m][j][part][0],
-                                        pb[m][j][part][1]);
-                            add4(acc[m][i], o);
-                        }
+                            for(int i = 0; i < SIDE; ++i)
+#pragma unroll
+                                for(int m = 0; m < MT; ++m)
+                                {
+                                    if(part == PARTS - 1)
+                                    {
+                                        o[i][m][0] = o[i][m][1] = o[i][m][2] = o[i][m][3] = 0.0f;
+                                    }
+                                    mma16<M>(o[i][m], va[i][0], va[i][1], va[i][2], va[i][3],
+                                            pb[m][j][part][0], pb[m][j][part][1]);
+                                }
+#pragma unroll
+                        for(int i = 0; i < SIDE; ++i)
+#pragma unroll
+                            for(int m = 0; m < MT; ++m)
+                                add4(acc[m][i0 + i], o[i][m]);
                     }
                 }
                 else
