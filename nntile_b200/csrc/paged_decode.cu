@@ -85,15 +85,31 @@ paged_decode_generic_kernel(const PagedDecodeArgs a)
             ? a.selected + ((size_t)kvh*a.batch + b)*a.num_selected : nullptr;
     const int32_t *table = a.block_table + (size_t)b*a.max_blocks;
     const T *q = (const T *)a.q + (size_t)qh*D;
-    float qv[EPL], o[EPL];
+    // sums of RUN positions, and of what was summed before: like terms, thousands of them in a
+    // row, would all round the same way
+    constexpr int RUN = 64;
+    float qv[EPL], o[EPL], run_o[EPL];
 #pragma unroll
     for(int x = 0; x < EPL; ++x)
     {
         const int h = lane + 32*x;
         qv[x] = h < D ? to_f(q[h])*a.scale_log2 : 0.0f;
-        o[x] = 0.0f;
+        o[x] = run_o[x] = 0.0f;
     }
-    float top = -CUDART_INF_F, sum = 0.0f;
+    float top = -CUDART_INF_F, sum = 0.0f, run_sum = 0.0f;
+    int run = 0;
+    auto end_run = [&]()
+    {
+        sum += run_sum;
+        run_sum = 0.0f;
+        run = 0;
+#pragma unroll
+        for(int x = 0; x < EPL; ++x)
+        {
+            o[x] += run_o[x];
+            run_o[x] = 0.0f;
+        }
+    };
     const int j_end = split_end(listed, split, a.chunk);
     for(int j = split*a.chunk; j < j_end; ++j)
     {
@@ -142,10 +158,20 @@ paged_decode_generic_kernel(const PagedDecodeArgs a)
             const float s = warp_sum(part)*ks;
             const float ntop = fmaxf(top, s);
             // every score so far -inf: nothing to weigh yet (and no inf - inf below)
-            const float shrink = top == ntop ? 1.0f : exp2f(top - ntop);
             const float p = s == -CUDART_INF_F ? 0.0f : exp2f(s - ntop);
-            sum = sum*shrink + p;
-            top = ntop;
+            if(top != ntop)
+            {
+                const float shrink = exp2f(top - ntop);
+                end_run();
+                sum *= shrink;
+#pragma unroll
+                for(int x = 0; x < EPL; ++x)
+                {
+                    o[x] *= shrink;
+                }
+                top = ntop;
+            }
+            run_sum += p;
 #pragma unroll
             for(int x = 0; x < EPL; ++x)
             {
@@ -156,10 +182,15 @@ paged_decode_generic_kernel(const PagedDecodeArgs a)
                     vv = E4M3 ? e4m3x2_to_f2(((const uint8_t *)a.v_pages)[at + h]).x*vs
                             : to_f(((const T *)a.v_pages)[at + h]);
                 }
-                o[x] = fmaf(p, vv, o[x]*shrink);
+                run_o[x] = fmaf(p, vv, run_o[x]);
+            }
+            if(++run == RUN)
+            {
+                end_run();
             }
         }
     }
+    end_run();
     __shared__ float o_s[PD_WARPS][PAGED_MAX_HEAD];
     __shared__ float top_s[PD_WARPS], sum_s[PD_WARPS];
     if(lane == 0)
