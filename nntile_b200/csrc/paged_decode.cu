@@ -631,7 +631,8 @@ paged_decode_kernel(const PagedDecodeArgs a)
     // than others that do not.  Whole binades here and in the scales: nothing rounds.
     constexpr float LIFT = HALF ? 10.0f : 0.0f, SLACK = HALF ? 5.5f : 4.0f, DEEPEST = 90.0f;
     // 8-bit values: accumulators count in units of 2^(vref - 127).  vref begins at the scale of
-    // values around one and moves when a row's scale is more than SPREAD binades away.
+    // values around one, or of the first rows when those are more than SPREAD binades away, and
+    // grows when a row is that much above it.
     constexpr int USUAL = 119, SPREAD = 60;
     constexpr float LOWEST = -3.0e38f;                   // no score yet
     constexpr int PARTS = HALF ? 2 : 3;                  // a weight's 16-bit pieces
