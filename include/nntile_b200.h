@@ -460,10 +460,12 @@ int nntile_b200_paged_kv_gather_fp16(nntile_b200_stream_t stream, int64_t head,
  * free.  Nothing to attend to (length 0, an empty selection, scores that are all -inf):
  * out = 0, lse = -inf.  Scores and sums are fp32; a weight counts with 24 bits (bf16 rows) or 22
  * (fp16 and e4m3 rows), these down to 2^-34 of the largest weight of the sequence, e4m3 rows
- * taken with their scale, rows of zeros left out.  An infinite value makes its column infinite,
+ * taken with their scale (scales of rows that count within 2^80 of all others), rows of zeros
+ * left out.  An infinite value makes its column infinite,
  * and NaN where its weight is below that (bf16: below 2^-126).  `workspace`:
- * nntile_b200_paged_decode_sdpa_workspace_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the GPU need workspaces of their own.
- * Results do not depend on the order in which CTAs run. */
+ * nntile_b200_paged_decode_sdpa_workspace_bytes(...) bytes, 16-byte aligned, of any content;
+ * calls that may overlap on the GPU need workspaces of their own.  Results do not depend on the
+ * order in which CTAs run. */
 int nntile_b200_paged_decode_sdpa_bf16(nntile_b200_stream_t stream, int64_t head,
         int64_t page_size, int64_t num_pages, int64_t max_blocks, int64_t batch, int64_t group,
         int64_t kv_heads, int64_t num_selected, int page_format, const int32_t *lengths,
